@@ -336,17 +336,16 @@ MAX_STEPS_IN_FLIGHT = 2
 
 def ensure_side_stream(device=None) -> "torch.cuda.Stream":
     """The side stream of `device` (default: the current device), created on first use -- ONE per device per process,
-    high priority.  Call it right after torch.cuda.set_device() and BEFORE torch.distributed.init_process_group in a
-    multi-rank process, so that the order in which the process creates its streams (and with it the stream -> hardware
+    at the default priority (streams of unlike priorities in one process have hung the GPU).  Call it right after
+    torch.cuda.set_device() and BEFORE torch.distributed.init_process_group in a multi-rank process, so that the order in which the process creates its streams (and with it the stream -> hardware
     queue assignment) is the same on every rank and in every run: main (the null stream, exists), side, collective."""
     dev = torch.cuda.current_device() if device is None else torch.device(device).index
     if dev is None:
         dev = torch.cuda.current_device()
     s = _SIDE_STREAMS.get(dev)
     if s is None:
-        prio = int(__import__("os").environ.get("LATTE_DIAG_SIDE_PRIORITY", "-1"))  # small dependent kernels: ahead of the big ones
         with torch.cuda.device(dev):
-            s = _SIDE_STREAMS[dev] = torch.cuda.Stream(priority=prio)
+            s = _SIDE_STREAMS[dev] = torch.cuda.Stream()
     return s
 
 
@@ -595,7 +594,7 @@ class LatteStep:
 
         Stream plan (side stream on, the default): everything that depends on the INPUTS only and needs host syncs --
         the index structures of the backbone, the in-FOV tables, the geometry of both HR calls -- runs on a
-        high-priority side stream; the main stream carries the two forwards, the HR feature kernels, the losses and
+        side stream; the main stream carries the two forwards, the HR feature kernels, the losses and
         the backward without a single host sync, so the host stays ahead of the GPU for the whole iteration."""
         if self.timers is not None:
             import time
