@@ -308,6 +308,43 @@ int lt_devoxelize_cell_bwd(const float* gout, const int32_t* cells, const int32_
                            const int32_t* p2v_idx /*[N]*/, const int32_t* v2p_idx /*[N,8]*/, const float* w /*[N,8]*/,
                            float* gfeats /*[V,C]*/, int64_t N, int64_t V, int32_t C, lt_stream_t stream);
 
+/* ------------------------------------------------------------------ dense layers: linear, 8-bit checkpoints
+ * nn.Linear with its epilogue and its backward (point branches and heads: latte/models/spvcnn.py:95-111,
+ * latte/models/xmuda_arch.py:326-335), where a layer trains or keeps its activations in 8 bits.  Matrices are row-major
+ * with a row stride (ld*, in elements; rows may start at any element, a stride of 0 repeats a row); y, deriv and the
+ * gradients are contiguous.  dt = LT_DT_*: the type of x, w, bias, res, y and of the gradients; sums are fp32.
+ * mx8: e4m3 values [M][K] and one scale byte per 32 neighbours [M][ceil(K/32)], value * 2^(scale - 127); the scale is the
+ * smallest power of two that brings the block's largest finite magnitude to at most 448, rounding is to nearest even,
+ * non-finite elements are held as NaN. */
+#define LT_DT_F32 0
+#define LT_DT_BF16 1
+#define LT_DT_F16 2
+#define LT_ACT_NONE 0
+#define LT_ACT_RELU 1
+#define LT_ACT_GELU 2 /* z Phi(z) */
+#define LT_ACT_SILU 3 /* z / (1 + exp(-z)) */
+/* what the forward keeps of act'(z): nothing (act none, or no backward will come); bits uint16 [M][ceil(N/16)] (ReLU);
+ * bytes [M][N], (c - 32) / 192 (GELU, SiLU); values [M][N] of type dt (GELU, SiLU) */
+#define LT_DERIV_NONE 0
+#define LT_DERIV_BITS 1
+#define LT_DERIV_BYTE 2
+#define LT_DERIV_FULL 3
+int lt_mx8_quantize(const void* x, int64_t ldx, int64_t M, int32_t K, int32_t dt, void* values, void* scales,
+                    lt_stream_t stream);
+int lt_mx8_dequantize(const void* values, const void* scales, int64_t M, int32_t K, int32_t dt, void* out,
+                      lt_stream_t stream);
+/* y[M][N] = act(x[M][K] w[N][K]^T + bias[N]) + res[M][N]; bias, res, deriv may be NULL */
+int64_t lt_linear_workspace_bytes(int64_t M, int32_t K, int32_t N, int32_t dt);
+int lt_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res, int64_t ldres,
+                  int32_t act, int64_t M, int32_t K, int32_t N, int32_t dt, void* y, void* deriv, int32_t deriv_kind, void* ws,
+                  int64_t ws_bytes, lt_stream_t stream);
+/* dz = dy * deriv;  dx[M][K] = dz w;  dw[N][K] = dz^T x;  db[N] = column sums of dz; dx, dw, db may be NULL.  x_scales not
+ * NULL: x is mx8 (ldx == K).  Sums are split and joined in a fixed order: the same bits every time. */
+int64_t lt_linear_bwd_workspace_bytes(int64_t M, int32_t K, int32_t N, int32_t dt);
+int lt_linear_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* x_scales, const void* w, int64_t ldw,
+                  const void* deriv, int32_t deriv_kind, int64_t M, int32_t K, int32_t N, int32_t dt, void* dx, void* dw,
+                  void* db, void* ws, int64_t ws_bytes, lt_stream_t stream);
+
 /* ------------------------------------------------------------------ ST-voxel aggregation (HR_Block / CR_Block)
  * see latte/models/hr_module.py:135-331 and :344-420; declared in the second half of this header */
 #include "latte_hip_st.h"

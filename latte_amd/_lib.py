@@ -85,6 +85,12 @@ SIGNATURES = {
     "lt_devoxelize_csr_bwd": (ctypes.c_int, [P, P, P, P, P, I64, I32, P]),
     "lt_devoxelize_cells": (ctypes.c_int, [P, P, P, P, I64, I64, I64, P]),
     "lt_devoxelize_cell_bwd": (ctypes.c_int, [P, P, P, P, P, P, P, P, I64, I64, I32, P]),
+    "lt_mx8_quantize": (ctypes.c_int, [P, I64, I64, I32, I32, P, P, P]),
+    "lt_mx8_dequantize": (ctypes.c_int, [P, P, I64, I32, I32, P, P]),
+    "lt_linear_workspace_bytes": (I64, [I64, I32, I32, I32]),
+    "lt_linear_fwd": (ctypes.c_int, [P, I64, P, I64, P, P, I64, I32, I64, I32, I32, I32, P, P, I32, P, I64, P]),
+    "lt_linear_bwd_workspace_bytes": (I64, [I64, I32, I32, I32]),
+    "lt_linear_bwd": (ctypes.c_int, [P, I64, P, I64, P, P, I64, P, I32, I64, I32, I32, I32, P, P, P, P, I64, P]),
     # include/latte_hip_st.h
     "lt_softmax_entropy": (ctypes.c_int, [P, I64, I32, P, P, P]),
     "lt_softmax_bwd": (ctypes.c_int, [P, P, I64, I32, P, P]),

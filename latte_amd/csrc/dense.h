@@ -1,0 +1,238 @@
+// Dense operators (linear, rms_norm, 8-bit checkpoints): types, 8-bit formats, epilogue.  gfx950.
+#pragma once
+#include "common.h"
+#include "../../include/latte_hip.h"
+
+typedef __bf16 lt_bf16;
+typedef _Float16 lt_f16;
+typedef float lt_f32x4 __attribute__((ext_vector_type(4)));
+typedef int lt_i32x4 __attribute__((ext_vector_type(4)));
+typedef int lt_i32x8 __attribute__((ext_vector_type(8)));
+typedef short lt_s16x4 __attribute__((ext_vector_type(4)));
+typedef short lt_s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 lt_bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 lt_f16x8 __attribute__((ext_vector_type(8)));
+#define LT_LDS_PTR(T, p) ((__attribute__((address_space(3))) T*)(p))
+
+template <class T> struct LtType;   // kMaxExp: the exponent of the type's last binade
+template <> struct LtType<float> { static constexpr int id = LT_DT_F32, kMaxExp = 127; };
+template <> struct LtType<lt_bf16> { static constexpr int id = LT_DT_BF16, kMaxExp = 127; };
+template <> struct LtType<lt_f16> { static constexpr int id = LT_DT_F16, kMaxExp = 15; };
+static inline int lt_dt_size(int dt) { return dt == LT_DT_F32 ? 4 : 2; }
+
+// ---- guarded vector access: n = elements that exist (<= 0: none); rows may start at any element, the hardware takes
+// unaligned 16-, 8- and 4-byte accesses, so only the end of a row goes element by element
+template <class T, int V>
+__device__ __forceinline__ void lt_ldv(const T* p, int64_t n, float (&o)[V]) {
+  if (n >= V) {
+    T t[V];
+    __builtin_memcpy(t, p, sizeof(t));
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = (float)t[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = i < n ? (float)p[i] : 0.f;
+  }
+}
+template <class T, int V>
+__device__ __forceinline__ void lt_stv(T* p, int64_t n, const float (&o)[V]) {
+  if (n >= V) {
+    T t[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) t[i] = (T)o[i];
+    __builtin_memcpy(p, t, sizeof(t));
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < n) p[i] = (T)o[i];
+  }
+}
+
+// i = q * d + r; 64-bit division costs some hundred instructions, so it is left to indexes that need it
+__device__ __forceinline__ void lt_divmod(int64_t i, int d, int64_t& q, int& r) {
+  if ((uint64_t)i >> 32 == 0) {
+    const unsigned u = (unsigned)i / (unsigned)d;
+    q = u;
+    r = (int)((unsigned)i - u * (unsigned)d);
+  } else {
+    q = i / d;
+    r = (int)(i - q * d);
+  }
+}
+
+// ---- mx8: 32 neighbours of a row share the scale 2^E, E the smallest integer with amax <= 448 * 2^E (amax over the
+// finite values; 448 is e4m3's largest), never below -126; the scale byte is E + 127.  Nothing saturates, so a value that
+// is held reads back within 2^-4 of itself (2^-10 * 2^E at the bottom).  A block that reaches into the last binade of its
+// type is cut at 240 * 2^E: 256 * 2^E would be infinite there, and 240 is still within 2^-4 of everything above it.
+// Infinities and NaN are held as NaN, each in its own place.
+__device__ __forceinline__ int lt_mx8_exp(float amax) {
+  const unsigned u = __float_as_uint(amax);            // finite and >= 0
+  int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0);   // mantissa over 1.75: one more
+  return e < -126 ? -126 : e;
+}
+__device__ __forceinline__ float lt_two_to(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }   // -126 <= e <= 127
+__device__ __forceinline__ float lt_finite_abs(float v) {
+  const float a = fabsf(v);
+  return a <= 3.4028234663852886e38f ? a : 0.f;
+}
+// two values at scale inv = 2^-E, |v * inv| <= 448, cut at lim -> two e4m3 bytes in the low half
+__device__ __forceinline__ int lt_mx8_pack2(float a, float b, float inv, float lim) {
+  const float u = __builtin_amdgcn_fmed3f(a * inv, -lim, lim) + (a - a);   // a - a: 0, or NaN where a is not finite
+  const float v = __builtin_amdgcn_fmed3f(b * inv, -lim, lim) + (b - b);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(u, v, 0, false);
+}
+__device__ __forceinline__ float lt_mx8_lim(float amax, int max_exp) {
+  return (int)(__float_as_uint(amax) >> 23) - 127 >= max_exp ? 240.f : 448.f;
+}
+template <int WHICH>   // bytes 2 * WHICH, 2 * WHICH + 1 of a word of four e4m3 values, times s = 2^E
+__device__ __forceinline__ void lt_mx8_get2(int word, float s, float& a, float& b) {
+  auto v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(word, s, WHICH != 0);
+  a = v[0];
+  b = v[1];
+}
+
+// ---- activations and their derivatives
+// act'(z) in a byte: (c - 32) / 192, c = 0..254 (0 and 1 exactly; gelu' and silu' stay inside [-0.13, 1.13]); 255 is NaN.
+__device__ __forceinline__ unsigned lt_deriv_byte(float d) {
+  const float c = rintf(__builtin_amdgcn_fmed3f(__fmaf_rn(d, 192.f, 32.f), 0.f, 254.f));
+  return d == d ? (unsigned)c : 255u;
+}
+__device__ __forceinline__ float lt_deriv_value(unsigned c) {
+  return c == 255u ? __builtin_nanf("") : ((float)(int)c - 32.f) * (1.f / 192.f);
+}
+// y = act(z), d = act'(z).  FAST (16-bit results): erfc by Abramowitz & Stegun 7.1.26 (|error| <= 1.5e-7) and the
+// hardware's exp2 and reciprocal; otherwise the library's functions.
+template <int ACT, bool FAST>
+__device__ __forceinline__ void lt_act(float z, float& y, float& d) {
+  if constexpr (ACT == LT_ACT_RELU) {
+    const bool off = z <= 0.f;   // NaN: neither value nor gradient is cut
+    y = off ? 0.f : z;
+    d = off ? 0.f : 1.f;
+  } else if constexpr (ACT == LT_ACT_GELU) {
+    float cdf, e;
+    if constexpr (FAST) {
+      const float x = fabsf(z) * 0.70710678118654752f;
+      e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);   // exp(-z^2 / 2)
+      const float t = __builtin_amdgcn_rcpf(__fmaf_rn(0.3275911f, x, 1.f));
+      float p = __fmaf_rn(1.061405429f, t, -1.453152027f);
+      p = __fmaf_rn(p, t, 1.421413741f);
+      p = __fmaf_rn(p, t, -0.284496736f);
+      p = __fmaf_rn(p, t, 0.254829592f);
+      const float half = 0.5f * p * t * e;   // erfc(|z| / sqrt 2) / 2
+      cdf = z < 0.f ? half : 1.f - half;
+    } else {
+      cdf = 0.5f * erfcf(z * -0.70710678118654752f);
+      e = expf(-0.5f * z * z);
+    }
+    y = z * cdf;
+    d = __fmaf_rn(z * 0.39894228040143268f, e, cdf);
+  } else if constexpr (ACT == LT_ACT_SILU) {
+    float s;
+    if constexpr (FAST) s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
+    else s = 1.f / (1.f + expf(-z));
+    y = z * s;
+    d = s * __fmaf_rn(z, 1.f - s, 1.f);
+  } else {
+    y = z;
+    d = 1.f;
+  }
+}
+
+// ---- epilogue of a product: y = act(z + bias) + residual, and what the backward pass keeps of act'
+struct LtEpi {
+  const void* bias;     // [cols], the type of y, or NULL
+  const void* res;      // [rows][ldres], or NULL
+  int64_t ldres;
+  void* out;            // [rows][ldo]
+  int64_t ldo;
+  void* deriv;          // LT_DERIV_BITS: uint16 [rows][ceil(cols/16)]; _BYTE: uint8 [rows][cols]; _FULL: type of y
+  int dkind;
+  int64_t rows;
+  int cols;
+};
+
+template <class T>
+__device__ __forceinline__ void lt_epi_bias(const LtEpi& e, int col, float (&b)[4]) {
+  b[0] = b[1] = b[2] = b[3] = 0.f;
+  if (e.bias) lt_ldv<T, 4>((const T*)e.bias + col, e.cols - col, b);
+}
+template <class T>
+__device__ __forceinline__ void lt_epi_res(const LtEpi& e, int64_t row, int col, float (&r)[4]) {
+  r[0] = r[1] = r[2] = r[3] = 0.f;
+  if (e.res && row < e.rows) lt_ldv<T, 4>((const T*)e.res + row * e.ldres + col, e.cols - col, r);
+}
+// four neighbours (row, col..col+3) of the product with their bias and residual (loaded ahead: the stores in between
+// would hold the loads back); nib = their ReLU bits (the caller joins four lanes into 16 bits)
+template <class T, int ACT>
+__device__ __forceinline__ void lt_epi4(const LtEpi& e, lt_f32x4 acc, const float (&b)[4], const float (&r)[4], int64_t row, int col,
+                                        unsigned& nib) {
+  nib = 0;
+  const int n = row < e.rows ? e.cols - col : 0;
+  if (n <= 0) return;
+  float y[4], d[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) lt_act<ACT, sizeof(T) == 2>(acc[i] + b[i], y[i], d[i]);
+  if constexpr (ACT != LT_ACT_NONE) {
+    if (e.dkind == LT_DERIV_BITS) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) nib |= (d[i] != 0.f && i < n) ? 1u << i : 0u;
+    } else if (e.dkind == LT_DERIV_BYTE) {
+      uint8_t* p = (uint8_t*)e.deriv + row * e.cols + col;
+      uint8_t c[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i] = (uint8_t)lt_deriv_byte(d[i]);
+      if (n >= 4) __builtin_memcpy(p, c, 4);
+      else
+        for (int i = 0; i < n; ++i) p[i] = c[i];
+    } else if (e.dkind == LT_DERIV_FULL) {
+      lt_stv<T, 4>((T*)e.deriv + row * e.cols + col, n, d);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] += r[i];
+  lt_stv<T, 4>((T*)e.out + row * e.ldo + col, n, y);
+}
+
+// ---- host side
+// dispatch over the value types: expression F<T>(...) with T bound
+#define LT_DENSE_TYPES(dt, ...)                                    \
+  do {                                                             \
+    if ((dt) == LT_DT_F32) { using T = float; __VA_ARGS__; }       \
+    else if ((dt) == LT_DT_BF16) { using T = lt_bf16; __VA_ARGS__; } \
+    else { using T = lt_f16; __VA_ARGS__; }                        \
+  } while (0)
+
+// Launches go to `stream`'s device, whatever device the calling thread has current (the null stream: the current device).
+struct LtOnStream {
+  int prev = -1;
+  bool switched = false;
+  int enter(hipStream_t stream) {
+    if (!stream) return LT_OK;
+    int dev = -1;
+    LT_CHECK_HIP(hipGetDevice(&prev));
+    LT_CHECK_HIP(hipStreamGetDevice(stream, &dev));
+    if (dev != prev) {
+      LT_CHECK_HIP(hipSetDevice(dev));
+      switched = true;
+    }
+    return LT_OK;
+  }
+  ~LtOnStream() {
+    if (switched) (void)hipSetDevice(prev);
+  }
+};
+
+// a product out[i][j] = sum_k Q(i,k) P(j,k), i < rows, j < cols, k < depth, for the dispatchers in dense_*.hip.
+// *_kmajor: the operand lies [k][i or j] instead of [i or j][k].
+struct LtGemm {
+  const void* P;
+  const void* Q;
+  int64_t ldp, ldq;
+  int64_t rows, depth;
+  int cols;
+  int dt;
+  bool p_kmajor, q_kmajor;
+  const uint8_t* p_scales;   // P is mx8 (k-major only): e4m3 values [k][ldp], scales [k][ceil(cols/32)]
+  int act;
+  LtEpi epi;
+};

@@ -1,0 +1,359 @@
+// linear: y = act(x W^T + b) + r, its backward, and what the backward pass keeps in 8 bits.
+//
+//   forward    z = x W^T + b (fp32 sums);  y = act(z) + r;  kept: x (or mx8(x)), W, act'(z)
+//   backward   dz = dy act'(z);  dx = dz W;  dW = dz^T x;  db = sum_rows dz;  dr = dy
+// act' is kept instead of z: the ReLU's is one bit, the others fit a uniform 8-bit grid (|error| <= 1/384), and the
+// backward pass needs no exponential.  dz is rounded to the operands' type, as the matrix instructions take it.
+//
+// Replaces the library products of nn.Linear (point branches and heads: latte/models/spvcnn.py:95-111,
+// latte/models/xmuda_arch.py:326-335) where a layer trains or keeps its activations in 8 bits.
+#include "dense_gemm.h"
+
+template <> int lt_gemm_launch<float>(const LtGemm&, const LtPlan&, float*, hipStream_t);
+template <> int lt_gemm_launch<lt_bf16>(const LtGemm&, const LtPlan&, float*, hipStream_t);
+template <> int lt_gemm_launch<lt_f16>(const LtGemm&, const LtPlan&, float*, hipStream_t);
+
+static int64_t part_bytes(const LtPlan& p, int64_t rows, int cols) {
+  return p.splits > 1 ? lt_align_up(p.splits * rows * cols * 4, 256) : 0;
+}
+
+// the larger of what the two staging paths want: which one runs depends on the operands' alignment
+static int64_t gemm_ws_bytes(int64_t rows, int cols, int64_t depth, int dt, bool nn) {
+  const int64_t a = part_bytes(lt_gemm_plan(rows, cols, depth, dt, nn, true, true), rows, cols);
+  const int64_t b = part_bytes(lt_gemm_plan(rows, cols, depth, dt, nn, false, true), rows, cols);
+  return a > b ? a : b;
+}
+
+static int gemm_run(const LtGemm& g, void* ws, int64_t ws_bytes, hipStream_t stream) {
+  const int sz = lt_dt_size(g.dt), ch = 16 / sz;
+  auto aligned = [&](const void* p, int64_t ld, int64_t run, bool kmajor) {
+    // whole 16-byte chunks along memory, and a tile's offsets within the 31 bits of a buffer descriptor
+    return ((uintptr_t)p & 15) == 0 && ld * sz % 16 == 0 && run % ch == 0 && (kmajor ? 64 : 256) * ld * sz < (int64_t)1 << 31;
+  };
+  const bool direct = !g.p_scales && aligned(g.P, g.ldp, g.p_kmajor ? g.cols : g.depth, g.p_kmajor) &&
+                      aligned(g.Q, g.ldq, g.q_kmajor ? g.rows : g.depth, g.q_kmajor);
+  const LtPlan p = lt_gemm_plan(g.rows, g.cols, g.depth, g.dt, !g.p_kmajor && !g.q_kmajor, direct, true);
+  LT_REQUIRE(part_bytes(p, g.rows, g.cols) <= ws_bytes, LT_ERR_WORKSPACE, "linear: workspace too small (%lld bytes)",
+             (long long)ws_bytes);
+  LT_REQUIRE((int64_t)p.tr * p.tc * p.splits < (int64_t)1 << 31, LT_ERR_RANGE, "linear: too many tiles");
+  LT_DENSE_TYPES(g.dt, return lt_gemm_launch<T>(g, p, (float*)ws, stream));
+}
+
+// ------------------------------------------------------------------ dz = dy act'(z) and its column sums
+// HBM-bound: one pass over dy and act', dz written once (not at all without an activation, where dz is dy).  A thread owns
+// four columns, a workgroup a slab of rows; the slabs' sums are joined in a fixed order by k_col_join.
+template <class T, int DK>
+__global__ __launch_bounds__(256) void k_dz(const T* __restrict__ dy, int64_t lddy, const void* __restrict__ deriv, int64_t M,
+                                            int N, int tx, int64_t rows_per, T* __restrict__ dz, float* __restrict__ part) {
+  __shared__ lt_f32x4 s_sum[256];
+  const int x = threadIdx.x % tx, yy = threadIdx.x / tx, ty = 256 / tx;
+  const int col = (blockIdx.x * tx + x) * 4;
+  const int n = N - col;
+  const int64_t r0 = blockIdx.y * rows_per, r1 = r0 + rows_per < M ? r0 + rows_per : M;
+  lt_f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  if (n > 0) {
+#pragma unroll 4
+    for (int64_t row = r0 + yy; row < r1; row += ty) {
+      float g[4], d[4];
+      lt_ldv<T, 4>(dy + row * lddy + col, n, g);
+      if constexpr (DK == LT_DERIV_BITS) {
+        const unsigned m = ((const uint16_t*)deriv)[row * ((N + 15) >> 4) + (col >> 4)] >> (col & 15);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) g[i] = (m >> i) & 1 ? g[i] : 0.f;
+      } else if constexpr (DK == LT_DERIV_BYTE) {
+        const uint8_t* p = (const uint8_t*)deriv + row * N + col;
+        uint8_t c[4] = {0, 0, 0, 0};
+        if (n >= 4) __builtin_memcpy(c, p, 4);
+        else
+          for (int i = 0; i < n; ++i) c[i] = p[i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) g[i] *= lt_deriv_value(c[i]);
+      } else if constexpr (DK == LT_DERIV_FULL) {
+        lt_ldv<T, 4>((const T*)deriv + row * N + col, n, d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) g[i] *= d[i];
+      }
+      if constexpr (DK != LT_DERIV_NONE) lt_stv<T, 4>(dz + row * N + col, n, g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] += i < n ? g[i] : 0.f;
+    }
+  }
+  if (!part) return;
+  s_sum[threadIdx.x] = sum;
+  __syncthreads();
+  if (yy == 0 && n > 0) {
+    for (int j = 1; j < ty; ++j) sum += s_sum[j * tx + x];
+    const float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+    lt_stv<float, 4>(part + (int64_t)blockIdx.y * N + col, n, v);
+  }
+}
+
+// out[c] = sum over slabs of part[slab][c]: 16 columns a workgroup, 16 threads a column, fixed order
+template <class T>
+__global__ __launch_bounds__(256) void k_col_join(const float* __restrict__ part, int slabs, int N, T* __restrict__ out) {
+  __shared__ float s_sum[16][17];
+  const int c = threadIdx.x & 15, l = threadIdx.x >> 4;
+  const int col = blockIdx.x * 16 + c;
+  float s = 0.f;
+  if (col < N) {
+#pragma unroll 8
+    for (int i = l; i < slabs; i += 16) s += part[(int64_t)i * N + col];
+  }
+  s_sum[l][c] = s;
+  __syncthreads();
+  if (l == 0 && col < N) {
+    for (int i = 1; i < 16; ++i) s += s_sum[i][c];
+    out[col] = (T)s;
+  }
+}
+
+struct DzPlan {
+  int tx, gx, slabs;
+  int64_t rows_per;
+};
+static DzPlan dz_plan(int64_t M, int N) {
+  DzPlan p;
+  const int cg = (N + 3) / 4;
+  p.tx = 1;
+  while (p.tx < cg && p.tx < 64) p.tx <<= 1;
+  p.gx = (cg + p.tx - 1) / p.tx;
+  const int ty = 256 / p.tx;
+  int64_t s = (2048 + p.gx - 1) / p.gx, most = (M + ty * 4 - 1) / (ty * 4);   // four rows a thread at least
+  if (s > most) s = most;
+  if (s < 1) s = 1;
+  p.rows_per = (M + s - 1) / s;
+  if (p.rows_per < 1) p.rows_per = 1;
+  p.slabs = (int)((M + p.rows_per - 1) / p.rows_per);
+  return p;
+}
+
+template <class T>
+static int dz_run(const void* dy, int64_t lddy, const void* deriv, int dkind, int64_t M, int N, void* dz, float* part, void* db,
+                  hipStream_t stream) {
+  const DzPlan p = dz_plan(M, N);
+  if (p.slabs > 0 && (part || dkind != LT_DERIV_NONE)) {
+    const dim3 grid(p.gx, p.slabs), block(256);
+    const T* g = (const T*)dy;
+    switch (dkind) {
+      case LT_DERIV_BITS: hipLaunchKernelGGL((k_dz<T, LT_DERIV_BITS>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, part); break;
+      case LT_DERIV_BYTE: hipLaunchKernelGGL((k_dz<T, LT_DERIV_BYTE>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, part); break;
+      case LT_DERIV_FULL: hipLaunchKernelGGL((k_dz<T, LT_DERIV_FULL>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, part); break;
+      default: hipLaunchKernelGGL((k_dz<T, LT_DERIV_NONE>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, part); break;
+    }
+    LT_LAUNCH_CHECK();
+  }
+  if (db) {
+    hipLaunchKernelGGL((k_col_join<T>), dim3((N + 15) / 16), dim3(256), 0, stream, part, p.slabs, N, (T*)db);
+    LT_LAUNCH_CHECK();
+  }
+  return LT_OK;
+}
+
+// ------------------------------------------------------------------ mx8 (layout and rounding: dense.h)
+// HBM-bound, one pass: a lane holds 8 neighbours, four lanes a block of 32.
+template <class T>
+__global__ __launch_bounds__(256) void k_mx8_quantize(const T* __restrict__ x, int64_t ldx, int64_t M, int K,
+                                                      uint8_t* __restrict__ q, uint8_t* __restrict__ sc) {
+  const int nb = (K + 31) >> 5, L = nb * 4;
+  const int64_t n = M * L, stride = (int64_t)gridDim.x * 256;
+  for (int64_t b = blockIdx.x * (int64_t)256; b < n; b += stride) {
+    const int64_t i = b + threadIdx.x;
+    int64_t row = 0;
+    int l = 0;
+    const bool live = i < n;
+    if (live) lt_divmod(i, L, row, l);
+    const int col = l * 8;
+    float v[8];
+    lt_ldv<T, 8>(x + row * ldx + col, live ? K - col : 0, v);
+    float a = 0.f;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) a = fmaxf(a, lt_finite_abs(v[t]));
+    a = fmaxf(a, __shfl_xor(a, 1, 64));
+    a = fmaxf(a, __shfl_xor(a, 2, 64));
+    if (!live) continue;
+    const int e = lt_mx8_exp(a);
+    const float inv = lt_two_to(-e), lim = lt_mx8_lim(a, LtType<T>::kMaxExp);
+    int w[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      w[t] = (lt_mx8_pack2(v[4 * t], v[4 * t + 1], inv, lim) & 0xFFFF) | (lt_mx8_pack2(v[4 * t + 2], v[4 * t + 3], inv, lim) << 16);
+    uint8_t* o = q + row * K + col;
+    if (K - col >= 8) __builtin_memcpy(o, w, 8);
+    else
+      for (int t = 0; t < K - col; ++t) o[t] = (uint8_t)(w[t >> 2] >> (8 * (t & 3)));
+    if ((threadIdx.x & 3) == 0) sc[row * nb + (l >> 2)] = (uint8_t)(e + 127);
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void k_mx8_dequantize(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sc, int64_t M,
+                                                        int K, T* __restrict__ out) {
+  const int nb = (K + 31) >> 5, L = nb * 4;
+  const int64_t n = M * L, stride = (int64_t)gridDim.x * 256;
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += stride) {
+    int64_t row;
+    int l;
+    lt_divmod(i, L, row, l);
+    const int col = l * 8, m = K - col;
+    if (m <= 0) continue;
+    const uint8_t* p = q + row * K + col;
+    int w[2] = {0, 0};
+    if (m >= 8) __builtin_memcpy(w, p, 8);
+    else
+      for (int t = 0; t < m; ++t) w[t >> 2] |= (int)p[t] << (8 * (t & 3));
+    const float s = __uint_as_float((unsigned)sc[row * nb + (l >> 2)] << 23);
+    float v[8];
+    lt_mx8_get2<0>(w[0], s, v[0], v[1]);
+    lt_mx8_get2<1>(w[0], s, v[2], v[3]);
+    lt_mx8_get2<0>(w[1], s, v[4], v[5]);
+    lt_mx8_get2<1>(w[1], s, v[6], v[7]);
+    lt_stv<T, 8>(out + row * K + col, m, v);
+  }
+}
+
+// ------------------------------------------------------------------ the C entry points
+static int check_dense(const char* who, int64_t M, int64_t K, int64_t N, int dt) {
+  LT_REQUIRE(dt == LT_DT_F32 || dt == LT_DT_BF16 || dt == LT_DT_F16, LT_ERR_ARG, "%s: type %d is none of LT_DT_*", who, dt);
+  LT_REQUIRE(M >= 0 && K >= 1 && N >= 1 && K <= INT32_MAX - 1024 && N <= INT32_MAX - 1024, LT_ERR_ARG,
+             "%s: bad sizes M=%lld K=%lld N=%lld", who, (long long)M, (long long)K, (long long)N);
+  LT_REQUIRE(M <= (int64_t)1 << 40, LT_ERR_RANGE, "%s: M=%lld is too large", who, (long long)M);
+  return LT_OK;
+}
+
+extern "C" int lt_mx8_quantize(const void* x, int64_t ldx, int64_t M, int32_t K, int32_t dt, void* values, void* scales,
+                               hipStream_t stream) {
+  int rc = check_dense("lt_mx8_quantize", M, K, 1, dt);
+  if (rc) return rc;
+  if (M == 0) return LT_OK;
+  LT_REQUIRE(x && values && scales, LT_ERR_ARG, "lt_mx8_quantize: null pointer");
+  LtOnStream on;
+  if ((rc = on.enter(stream))) return rc;
+  const int64_t n = M * (int64_t)((K + 31) / 32 * 4);
+  LT_DENSE_TYPES(dt, hipLaunchKernelGGL((k_mx8_quantize<T>), dim3(lt_grid(n, 256)), dim3(256), 0, stream, (const T*)x, ldx, M, K,
+                                        (uint8_t*)values, (uint8_t*)scales));
+  LT_LAUNCH_CHECK();
+  return LT_OK;
+}
+
+extern "C" int lt_mx8_dequantize(const void* values, const void* scales, int64_t M, int32_t K, int32_t dt, void* out,
+                                 hipStream_t stream) {
+  int rc = check_dense("lt_mx8_dequantize", M, K, 1, dt);
+  if (rc) return rc;
+  if (M == 0) return LT_OK;
+  LT_REQUIRE(out && values && scales, LT_ERR_ARG, "lt_mx8_dequantize: null pointer");
+  LtOnStream on;
+  if ((rc = on.enter(stream))) return rc;
+  const int64_t n = M * (int64_t)((K + 31) / 32 * 4);
+  LT_DENSE_TYPES(dt, hipLaunchKernelGGL((k_mx8_dequantize<T>), dim3(lt_grid(n, 256)), dim3(256), 0, stream, (const uint8_t*)values,
+                                        (const uint8_t*)scales, M, K, (T*)out));
+  LT_LAUNCH_CHECK();
+  return LT_OK;
+}
+
+extern "C" int64_t lt_linear_workspace_bytes(int64_t M, int32_t K, int32_t N, int32_t dt) {
+  if (check_dense("lt_linear_workspace_bytes", M, K, N, dt)) return -1;
+  return gemm_ws_bytes(M, N, K, dt, true);
+}
+
+extern "C" int lt_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res,
+                             int64_t ldres, int32_t act, int64_t M, int32_t K, int32_t N, int32_t dt, void* y, void* deriv,
+                             int32_t deriv_kind, void* ws, int64_t ws_bytes, hipStream_t stream) {
+  int rc = check_dense("lt_linear_fwd", M, K, N, dt);
+  if (rc) return rc;
+  LT_REQUIRE(act >= LT_ACT_NONE && act <= LT_ACT_SILU, LT_ERR_ARG, "lt_linear_fwd: act=%d is none of LT_ACT_*", act);
+  LT_REQUIRE(deriv_kind == LT_DERIV_NONE || (deriv_kind == LT_DERIV_BITS && act == LT_ACT_RELU) ||
+                 ((deriv_kind == LT_DERIV_BYTE || deriv_kind == LT_DERIV_FULL) && act >= LT_ACT_GELU),
+             LT_ERR_ARG, "lt_linear_fwd: deriv_kind=%d does not go with act=%d", deriv_kind, act);
+  if (M == 0) return LT_OK;
+  LT_REQUIRE(x && w && y && (deriv_kind == LT_DERIV_NONE || deriv), LT_ERR_ARG, "lt_linear_fwd: null pointer");
+  LtOnStream on;
+  if ((rc = on.enter(stream))) return rc;
+  LtGemm g = {};
+  g.P = w;
+  g.ldp = ldw;
+  g.Q = x;
+  g.ldq = ldx;
+  g.rows = M;
+  g.cols = N;
+  g.depth = K;
+  g.dt = dt;
+  g.act = act;
+  g.epi = LtEpi{bias, res, ldres, y, N, deriv, deriv_kind, M, N};
+  return gemm_run(g, ws, ws ? ws_bytes : 0, stream);
+}
+
+struct BwdWs {
+  int64_t dz, part, gemm, bytes;
+};
+static BwdWs bwd_ws(int64_t M, int K, int N, int dt) {
+  BwdWs w;
+  int64_t off = 0;
+  w.dz = off;
+  off += lt_align_up(M * N * lt_dt_size(dt), 256);
+  w.part = off;
+  off += lt_align_up((int64_t)dz_plan(M, N).slabs * N * 4, 256);
+  w.gemm = off;
+  const int64_t a = gemm_ws_bytes(M, K, N, dt, false), b = gemm_ws_bytes(N, K, M, dt, false);
+  off += a > b ? a : b;
+  w.bytes = off;
+  return w;
+}
+
+extern "C" int64_t lt_linear_bwd_workspace_bytes(int64_t M, int32_t K, int32_t N, int32_t dt) {
+  if (check_dense("lt_linear_bwd_workspace_bytes", M, K, N, dt)) return -1;
+  return bwd_ws(M, K, N, dt).bytes;
+}
+
+extern "C" int lt_linear_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* x_scales, const void* w,
+                             int64_t ldw, const void* deriv, int32_t deriv_kind, int64_t M, int32_t K, int32_t N, int32_t dt,
+                             void* dx, void* dw, void* db, void* ws, int64_t ws_bytes, hipStream_t stream) {
+  int rc = check_dense("lt_linear_bwd", M, K, N, dt);
+  if (rc) return rc;
+  LT_REQUIRE(deriv_kind >= LT_DERIV_NONE && deriv_kind <= LT_DERIV_FULL, LT_ERR_ARG, "lt_linear_bwd: deriv_kind=%d", deriv_kind);
+  LT_REQUIRE(!x_scales || ldx == K, LT_ERR_ARG, "lt_linear_bwd: an mx8 x has rows of K values, not ldx=%lld", (long long)ldx);
+  const BwdWs o = bwd_ws(M, K, N, dt);
+  LT_REQUIRE(ws_bytes >= o.bytes && (ws || o.bytes == 0), LT_ERR_WORKSPACE, "lt_linear_bwd: workspace too small");
+  if (M > 0)
+    LT_REQUIRE(dy && (deriv_kind == LT_DERIV_NONE || deriv) && (!dx || w) && (!dw || x), LT_ERR_ARG, "lt_linear_bwd: null pointer");
+  LtOnStream on;
+  if ((rc = on.enter(stream))) return rc;
+  char* wsb = (char*)ws;
+  const void* dz = dy;
+  int64_t lddz = lddy;
+  if (deriv_kind != LT_DERIV_NONE) {
+    dz = wsb + o.dz;
+    lddz = N;
+  }
+  LT_DENSE_TYPES(dt, rc = dz_run<T>(dy, lddy, deriv, deriv_kind, M, N, wsb + o.dz, db ? (float*)(wsb + o.part) : nullptr, db, stream));
+  if (rc) return rc;
+  LtGemm g = {};
+  g.dt = dt;
+  g.act = LT_ACT_NONE;
+  if (dx && M > 0) {
+    g.P = w;
+    g.ldp = ldw;
+    g.p_kmajor = true;
+    g.Q = dz;
+    g.ldq = lddz;
+    g.rows = M;
+    g.cols = K;
+    g.depth = N;
+    g.epi = LtEpi{nullptr, nullptr, 0, dx, K, nullptr, LT_DERIV_NONE, M, K};
+    if ((rc = gemm_run(g, wsb + o.gemm, ws_bytes - o.gemm, stream))) return rc;
+  }
+  if (dw) {
+    g.P = x;
+    g.ldp = ldx;
+    g.p_kmajor = true;
+    g.p_scales = (const uint8_t*)x_scales;
+    g.Q = dz;
+    g.ldq = lddz;
+    g.q_kmajor = true;
+    g.rows = N;
+    g.cols = K;
+    g.depth = M;
+    g.epi = LtEpi{nullptr, nullptr, 0, dw, K, nullptr, LT_DERIV_NONE, N, K};
+    if ((rc = gemm_run(g, wsb + o.gemm, ws_bytes - o.gemm, stream))) return rc;
+  }
+  return LT_OK;
+}

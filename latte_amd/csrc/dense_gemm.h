@@ -1,0 +1,595 @@
+// The tiled product of the dense operators, and its joins.  out[i][j] = sum_k Q(i,k) P(j,k).
+//
+// The matrix instructions compute D = A B with A = P (output columns) and B = Q (output rows): a lane then holds four
+// neighbouring COLUMNS of one output row, so bias, residual and result move 8 or 16 bytes at a time.  A workgroup owns a
+// BR x BC tile of the output and walks k in steps of 128 bytes (64 16-bit or 32 fp32 values) through two LDS buffers, one
+// barrier a step: while the step's matrix instructions run, the next step's tiles are on the way.
+//
+// LDS images, 16-byte chunks:
+//   operand [i][k]  (k runs along memory)  : tile [R][128 B], chunk c of row i at position c ^ (i & 7)
+//   operand [k][i]  (i runs along memory)  : tile [BK][R], chunk c of line k at position c ^ f(k), see kswz(); 16-bit
+//                                            fragments are read with the transposing LDS read (4 lines x 16 columns)
+// Both keep every fragment read free of bank conflicts between the lanes that are served together.
+#pragma once
+#include "dense.h"
+
+struct LtTileArgs {
+  const char* P;
+  const char* Q;
+  int64_t ldp, ldq;       // bytes
+  int64_t rows, depth;
+  int cols;
+  int tr, tc;             // tiles along rows / columns
+  int splits;
+  int64_t slice;          // k per split, a multiple of BK
+  float* part;            // [splits][rows][cols] when splits > 1
+  const uint8_t* ps;      // scales of an mx8 P
+  int64_t ldps;
+  LtEpi epi;
+};
+
+template <class T> struct LtMma;
+template <> struct LtMma<lt_bf16> {
+  typedef lt_bf16x8 frag;
+  static __device__ __forceinline__ lt_f32x4 mma(frag a, frag b, lt_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct LtMma<lt_f16> {
+  typedef lt_f16x8 frag;
+  static __device__ __forceinline__ lt_f32x4 mma(frag a, frag b, lt_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct LtMma<float> {
+  typedef lt_f32x4 frag;   // four k of one row: k = 16 j + 4 g + t goes into instruction t (the same for both operands)
+  static __device__ __forceinline__ lt_f32x4 mma(frag a, frag b, lt_f32x4 c) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[t], b[t], c, 0, 0, 0);
+    return c;
+  }
+};
+
+template <class T, bool KM, int R>   // an operand's tile: R rows (or columns) of the product, 128 bytes' worth of k
+struct LtTile {
+  static constexpr int SZ = sizeof(T), CH = 16 / SZ, BK = 128 / SZ;
+  static constexpr int BYTES = R * 128, SEGS = BYTES / 1024;
+  static constexpr int CPL = KM ? R / CH : 8;   // chunks per line
+  // k-major lines of one fragment read must not meet in a bank: 16-bit reads take 32 bytes of lines k0 + {0..3} per 16
+  // lanes, fp32 reads 64 bytes of lines k0 + {0, 4, 8, 12}
+  static __device__ __forceinline__ int kswz(int k) {
+    if constexpr (SZ == 2) return (((k & 3) | ((k >> 1) & 4)) << 1) & (CPL - 1);
+    else return (((k >> 2) & 3) << 2) & (CPL - 1);
+  }
+  // chunk L (linear position in the image) -> its line and its chunk within the line in memory
+  static __device__ __forceinline__ void where(int L, int& line, int& c) {
+    line = L / CPL;
+    c = (L % CPL) ^ (KM ? kswz(line) : (line & 7));
+  }
+  // fragment kk of the 16 rows from i0: k = kk * KF + ..., KF = 32 (16-bit) or 16 (fp32)
+  static __device__ __forceinline__ typename LtMma<T>::frag frag(const char* t, int i0, int kk, int lane) {
+    const int r = lane & 15, g = lane >> 4;
+    if constexpr (!KM) {
+      const int i = i0 + r, c = kk * 4 + g;
+      return *reinterpret_cast<const typename LtMma<T>::frag*>(t + i * 128 + ((c ^ (i & 7)) << 4));
+    } else if constexpr (SZ == 2) {
+      const int k = kk * 32 + 8 * g + (r >> 2), col = i0 + 4 * (r & 3);
+      const char* p = t + k * (R * 2) + (((col >> 3) ^ kswz(k)) << 4) + (col & 7) * 2;   // kswz(k + 4) == kswz(k)
+      union { lt_s16x4 h[2]; typename LtMma<T>::frag f; } u;
+      u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LT_LDS_PTR(lt_s16x4, p));
+      u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LT_LDS_PTR(lt_s16x4, p + 4 * (R * 2)));
+      return u.f;
+    } else {
+      const int col = i0 + r;
+      typename LtMma<T>::frag f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int k = kk * 16 + 4 * g + q;
+        f[q] = *reinterpret_cast<const float*>(t + k * (R * 4) + (((col >> 2) ^ kswz(k)) << 4) + (col & 3) * 4);
+      }
+      return f;
+    }
+  }
+};
+
+// 64 lanes x 16 bytes from memory to 1024 consecutive bytes of LDS (device pass only: the host pass knows no 16-byte form)
+__device__ __forceinline__ void lt_load_lds16(const char* base, char* lds, unsigned off) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, 0x7FFFFFFF, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, LT_LDS_PTR(void, lds), 16, off, 0, 0, 0);
+#endif
+}
+
+// ---- staging straight into LDS.  Lines or chunks that do not exist get an offset past the descriptor's range, which
+// loads zeros.  Needs 16-byte aligned lines, k (or the columns, k-major) in whole chunks, and tiles below 2 GiB.
+template <class TL, bool KM, int NW>
+struct LtDirect {
+  static constexpr int N = TL::SEGS / NW;
+  unsigned off[N];
+  __device__ __forceinline__ void init(int64_t ld, int64_t n_lines_or_cols, int wave, int lane) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      int line, c;
+      TL::where((wave + i * NW) * 64 + lane, line, c);
+      const bool ok = KM ? c * TL::CH < n_lines_or_cols : line < n_lines_or_cols;
+      off[i] = ok ? (unsigned)(line * ld + c * 16) : 0x80000000u;
+    }
+  }
+  // kleft: how much of k is left from this step on (may exceed BK)
+  __device__ __forceinline__ void load(const char* base, char* lds, int64_t kleft, int wave, int lane) const {
+    if (kleft >= TL::BK) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        lt_load_lds16(base, lds + (wave + i * NW) * 1024, off[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        int line, c;
+        TL::where((wave + i * NW) * 64 + lane, line, c);
+        const bool ok = KM ? line < kleft : c * TL::CH < kleft;
+        lt_load_lds16(base, lds + (wave + i * NW) * 1024, ok ? off[i] : 0x80000000u);
+      }
+    }
+  }
+};
+
+// ---- staging through registers: any alignment, any length; an mx8 operand is widened on the way
+template <class T, class TL, bool KM, bool MX8, int NT>
+struct LtStaged {
+  static constexpr int N = TL::BYTES / 16 / NT;
+  lt_i32x4 v[N];
+  __device__ __forceinline__ void load(const char* base, int64_t ld, int64_t n_lines_or_cols, int64_t kleft, const uint8_t* sc,
+                                       int64_t ldsc, int col0, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      int line, c;
+      TL::where(tid + i * NT, line, c);
+      const bool line_ok = KM ? line < kleft : line < n_lines_or_cols;
+      const int64_t n = line_ok ? (KM ? n_lines_or_cols : kleft) - c * TL::CH : 0;
+      lt_i32x4 w = {0, 0, 0, 0};
+      if constexpr (MX8) {
+        if (n > 0) {
+          const char* p = base + line * ld + c * TL::CH;
+          const float s = __uint_as_float((unsigned)sc[line * ldsc + ((col0 + c * TL::CH) >> 5)] << 23);
+          int q[2] = {0, 0};
+          if (n >= TL::CH) __builtin_memcpy(q, p, TL::CH);
+          else {
+            unsigned long long b = 0;
+            for (int j = 0; j < n; ++j) b |= (unsigned long long)(uint8_t)p[j] << (8 * j);
+            q[0] = (int)b;
+            q[1] = (int)(b >> 32);
+          }
+          if constexpr (sizeof(T) == 4) {
+            float a[4];
+            lt_mx8_get2<0>(q[0], s, a[0], a[1]);
+            lt_mx8_get2<1>(q[0], s, a[2], a[3]);
+            __builtin_memcpy(&w, a, 16);
+          } else {
+            T a[8];   // e4m3 times a power of two has 4 bits: exact in either 16-bit type
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float f[4];
+              lt_mx8_get2<0>(q[j], s, f[0], f[1]);
+              lt_mx8_get2<1>(q[j], s, f[2], f[3]);
+#pragma unroll
+              for (int t = 0; t < 4; ++t) a[4 * j + t] = (T)f[t];
+            }
+            __builtin_memcpy(&w, a, 16);
+          }
+        }
+      } else {
+        const char* p = base + line * ld + c * 16;
+        if (n >= TL::CH) __builtin_memcpy(&w, p, 16);
+        else if (n > 0) {
+          T a[TL::CH];
+#pragma unroll
+          for (int j = 0; j < TL::CH; ++j) a[j] = j < n ? reinterpret_cast<const T*>(p)[j] : (T)0.f;
+          __builtin_memcpy(&w, a, 16);
+        }
+      }
+      v[i] = w;
+    }
+  }
+  __device__ __forceinline__ void store(char* lds, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) *reinterpret_cast<lt_i32x4*>(lds + (tid + i * NT) * 16) = v[i];
+  }
+};
+
+// workgroup id -> work: consecutive pieces go to one XCD (ids are dealt to the 8 XCDs in turn), so tiles that share
+// operands share an L2; a bijection for any count
+__device__ __forceinline__ unsigned lt_xcd_map(unsigned b, unsigned n) {
+  const unsigned per = n >> 3, rem = n & 7, x = b & 7;
+  return x * per + (x < rem ? x : rem) + (b >> 3);
+}
+
+template <class T, bool PKM, bool QKM, int BR, int BC, int WR, int WC, bool DIRECT, bool P8, int ACT>
+__global__ __launch_bounds__(64 * WR * WC) void k_dense(LtTileArgs a) {
+  typedef LtTile<T, PKM, BC> TP;
+  typedef LtTile<T, QKM, BR> TQ;
+  constexpr int NW = WR * WC, NT = 64 * NW, FR = BR / WR / 16, FC = BC / WC / 16;
+  constexpr int BUF = TP::BYTES + TQ::BYTES;
+  extern __shared__ __attribute__((aligned(1024))) char s_tile[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // eight row tiles x all column tiles form a group: its operands stay in the L2 of the XCD that works on it
+  const unsigned tiles = (unsigned)a.tr * a.tc;
+  const unsigned L = lt_xcd_map(blockIdx.x, tiles * a.splits);
+  const unsigned split = L / tiles, t_ = L % tiles;
+  const unsigned grp = t_ / (8u * a.tc), in = t_ - grp * 8u * a.tc;
+  const unsigned gr = (unsigned)a.tr - grp * 8u < 8u ? (unsigned)a.tr - grp * 8u : 8u;
+  const int64_t row0 = (int64_t)(grp * 8u + in % gr) * BR;
+  const int col0 = (int)(in / gr) * BC;
+  const int64_t k0 = split * a.slice;
+  const int64_t kend = k0 + a.slice < a.depth ? k0 + a.slice : a.depth;
+  const int nk = (int)((kend - k0 + TP::BK - 1) / TP::BK);
+  constexpr int PS = P8 ? 1 : (int)sizeof(T);
+  const char* pb = a.P + (PKM ? k0 * a.ldp + (int64_t)col0 * PS : col0 * a.ldp + k0 * PS);
+  const char* qb = a.Q + (QKM ? k0 * a.ldq + row0 * (int64_t)sizeof(T) : row0 * a.ldq + k0 * (int64_t)sizeof(T));
+  const int64_t pstep = PKM ? TP::BK * a.ldp : TP::BK * PS, qstep = QKM ? TQ::BK * a.ldq : 128;
+  const int64_t pn = a.cols - col0, qn = a.rows - row0;
+  const uint8_t* psc = P8 ? a.ps + k0 * a.ldps : nullptr;
+
+  lt_f32x4 acc[FR][FC];
+#pragma unroll
+  for (int i = 0; i < FR; ++i)
+#pragma unroll
+    for (int j = 0; j < FC; ++j) acc[i][j] = (lt_f32x4){0.f, 0.f, 0.f, 0.f};
+  const int wr = (wave / WC) * (BR / WR), wc = (wave % WC) * (BC / WC);
+
+  auto compute = [&](const char* buf) {
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      typename LtMma<T>::frag p[FC], q[FR];
+#pragma unroll
+      for (int j = 0; j < FC; ++j) p[j] = TP::frag(buf, wc + 16 * j, kk, lane);
+#pragma unroll
+      for (int i = 0; i < FR; ++i) q[i] = TQ::frag(buf + TP::BYTES, wr + 16 * i, kk, lane);
+#pragma unroll
+      for (int i = 0; i < FR; ++i)
+#pragma unroll
+        for (int j = 0; j < FC; ++j) acc[i][j] = LtMma<T>::mma(p[j], q[i], acc[i][j]);
+    }
+  };
+
+  if constexpr (DIRECT) {
+    LtDirect<TP, PKM, NW> sp;
+    LtDirect<TQ, QKM, NW> sq;
+    sp.init(a.ldp, pn, wave, lane);
+    sq.init(a.ldq, qn, wave, lane);
+    sp.load(pb, s_tile, kend - k0, wave, lane);
+    sq.load(qb, s_tile + TP::BYTES, kend - k0, wave, lane);
+    for (int t = 0; t < nk; ++t) {
+      char* cur = s_tile + (t & 1) * BUF;
+      char* nxt = s_tile + ((t + 1) & 1) * BUF;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();   // this step's tiles have landed, and nobody reads the other buffer any more
+      if (t + 1 < nk) {
+        const int64_t left = kend - k0 - (int64_t)(t + 1) * TP::BK;
+        sp.load(pb + (t + 1) * pstep, nxt, left, wave, lane);
+        sq.load(qb + (t + 1) * qstep, nxt + TP::BYTES, left, wave, lane);
+      }
+      compute(cur);
+    }
+  } else {
+    LtStaged<T, TP, PKM, P8, NT> sp;
+    LtStaged<T, TQ, QKM, false, NT> sq;
+    sp.load(pb, a.ldp, pn, kend - k0, psc, a.ldps, col0, tid);
+    sq.load(qb, a.ldq, qn, kend - k0, nullptr, 0, 0, tid);
+    for (int t = 0; t < nk; ++t) {
+      char* cur = s_tile + (t & 1) * BUF;
+      sp.store(cur, tid);      // its last readers passed the barrier of step t - 1
+      sq.store(cur + TP::BYTES, tid);
+      __syncthreads();
+      if (t + 1 < nk) {
+        const int64_t left = kend - k0 - (int64_t)(t + 1) * TP::BK;
+        if (P8) psc += TP::BK * a.ldps;
+        sp.load(pb + (t + 1) * pstep, a.ldp, pn, left, psc, a.ldps, col0, tid);
+        sq.load(qb + (t + 1) * qstep, a.ldq, qn, left, nullptr, 0, 0, tid);
+      }
+      compute(cur);
+    }
+  }
+
+  const int r = lane & 15, g = lane >> 4;
+  if (a.splits > 1) {
+#pragma unroll
+    for (int i = 0; i < FR; ++i)
+#pragma unroll
+      for (int j = 0; j < FC; ++j) {
+        const int64_t row = row0 + wr + 16 * i + r;
+        const int col = col0 + wc + 16 * j + 4 * g;
+        if (row < a.rows && col < a.cols) {
+          const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+          lt_stv<float, 4>(a.part + ((int64_t)split * a.rows + row) * a.cols + col, a.cols - col, v);
+        }
+      }
+    return;
+  }
+  float b[FC][4];
+#pragma unroll
+  for (int j = 0; j < FC; ++j) lt_epi_bias<T>(a.epi, col0 + wc + 16 * j + 4 * g, b[j]);
+#pragma unroll
+  for (int i = 0; i < FR; ++i) {
+    const int64_t row = row0 + wr + 16 * i + r;
+    float res[FC][4];
+#pragma unroll
+    for (int j = 0; j < FC; ++j) lt_epi_res<T>(a.epi, row, col0 + wc + 16 * j + 4 * g, res[j]);
+#pragma unroll
+    for (int j = 0; j < FC; ++j) {
+      const int col = col0 + wc + 16 * j + 4 * g;
+      unsigned nib;
+      lt_epi4<T, ACT>(a.epi, acc[i][j], b[j], res[j], row, col, nib);
+      if constexpr (ACT == LT_ACT_RELU) {
+        if (a.epi.dkind == LT_DERIV_BITS) {   // the four lanes of a row join their bits: 16 columns
+          nib <<= 4 * g;
+          nib |= __shfl_xor(nib, 16, 64);
+          nib |= __shfl_xor(nib, 32, 64);
+          if (g == 0 && row < a.rows && col < a.cols)
+            ((uint16_t*)a.epi.deriv)[row * ((a.cols + 15) >> 4) + (col >> 4)] = (uint16_t)nib;
+        }
+      }
+    }
+  }
+}
+
+// out = epilogue(sum over the splits, in a fixed order: the same bits every time).  G threads share four neighbours and take
+// the splits in turn; one thread adding up 256 splits alone would wait for memory 256 times.
+template <class T, int ACT, int G>
+__global__ __launch_bounds__(256) void k_dense_join(const float* __restrict__ part, int splits, LtEpi e) {
+  constexpr int EL = 256 / G;
+  __shared__ lt_f32x4 s_sum[G][EL];
+  const int el = threadIdx.x % EL, sl = threadIdx.x / EL;
+  const int c4 = ((e.cols + 15) >> 4) * 4;   // four lanes to 16 columns
+  const int64_t n = e.rows * c4, stride = (int64_t)gridDim.x * EL;
+  const int64_t plane = e.rows * e.cols;
+  for (int64_t b = blockIdx.x * (int64_t)EL; b < n; b += stride) {
+    const int64_t i = b + el;
+    int64_t row = e.rows;
+    int col = 0;
+    if (i < n) lt_divmod(i, c4, row, col);
+    col *= 4;
+    lt_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    if (row < e.rows && col < e.cols) {
+      const float* p = part + row * e.cols + col;
+#pragma unroll 8
+      for (int s = sl; s < splits; s += G) {
+        float v[4];
+        lt_ldv<float, 4>(p + s * plane, e.cols - col, v);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[t] += v[t];
+      }
+    }
+    if constexpr (G > 1) {
+      __syncthreads();   // the previous turn's sums have been read
+      s_sum[sl][el] = acc;
+      __syncthreads();
+      if (sl != 0) continue;
+#pragma unroll
+      for (int s = 1; s < G; ++s) acc += s_sum[s][el];
+    }
+    unsigned nib;
+    float bias[4], res[4];
+    lt_epi_bias<T>(e, col, bias);
+    lt_epi_res<T>(e, row, col, res);
+    lt_epi4<T, ACT>(e, acc, bias, res, row, col, nib);
+    if constexpr (ACT == LT_ACT_RELU) {
+      if (e.dkind == LT_DERIV_BITS) {
+        nib <<= 4 * (threadIdx.x & 3);
+        nib |= __shfl_xor(nib, 1, 64);
+        nib |= __shfl_xor(nib, 2, 64);
+        if ((threadIdx.x & 3) == 0 && row < e.rows && col < e.cols)
+          ((uint16_t*)e.deriv)[row * ((e.cols + 15) >> 4) + (col >> 4)] = (uint16_t)nib;
+      }
+    }
+  }
+}
+
+// ---- few rows: y[rows <= 64][cols].  Bound by reading P once: a workgroup takes 16 columns, its 8 waves share k in
+// turns of four fragments (256 bytes of each of the 16 lines of P), operands go from memory straight into the matrix
+// instructions' registers (nothing is used twice but the few rows of Q, which the caches hold), and the waves' sums are
+// added through LDS in wave order.
+template <class T, int FR, int ACT>
+__global__ __launch_bounds__(512) void k_dense_few(LtTileArgs a) {
+  typedef typename LtMma<T>::frag Frag;
+  constexpr int CH = 16 / sizeof(T), KF = 4 * CH, U = 4;
+  __shared__ lt_f32x4 s_acc[8][FR][64];
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col0 = blockIdx.x * 16;
+  const bool pok = col0 + r < a.cols;
+  const T* p = (const T*)(a.P + (int64_t)(pok ? col0 + r : 0) * a.ldp);
+  lt_f32x4 acc[FR];
+#pragma unroll
+  for (int f = 0; f < FR; ++f) acc[f] = (lt_f32x4){0.f, 0.f, 0.f, 0.f};
+  auto get = [&](const T* line, bool ok, int64_t k) -> Frag {
+    Frag v;
+    const int64_t n = ok ? a.depth - k : 0;
+    if (n >= CH) __builtin_memcpy(&v, line + k, 16);
+    else {
+#pragma unroll
+      for (int j = 0; j < CH; ++j) v[j] = j < n ? line[k + j] : (T)0.f;
+    }
+    return v;
+  };
+  for (int64_t k = (int64_t)wave * U * KF; k < a.depth; k += 8 * U * KF) {
+    Frag pf[U], qf[FR][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) pf[u] = get(p, pok, k + u * KF + g * CH);
+#pragma unroll
+    for (int f = 0; f < FR; ++f) {
+      const bool ok = f * 16 + r < a.rows;
+      const T* q = (const T*)(a.Q + (int64_t)(ok ? f * 16 + r : 0) * a.ldq);
+#pragma unroll
+      for (int u = 0; u < U; ++u) qf[f][u] = get(q, ok, k + u * KF + g * CH);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int f = 0; f < FR; ++f) acc[f] = LtMma<T>::mma(pf[u], qf[f][u], acc[f]);
+  }
+#pragma unroll
+  for (int f = 0; f < FR; ++f) s_acc[wave][f][lane] = acc[f];
+  __syncthreads();
+  if (wave < FR) {
+    lt_f32x4 s = s_acc[0][wave][lane];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) s += s_acc[w][wave][lane];
+    const int64_t row = wave * 16 + r;
+    const int col = col0 + 4 * g;
+    unsigned nib;
+    float b[4], res[4];
+    lt_epi_bias<T>(a.epi, col, b);
+    lt_epi_res<T>(a.epi, row, col, res);
+    lt_epi4<T, ACT>(a.epi, s, b, res, row, col, nib);
+    if constexpr (ACT == LT_ACT_RELU) {
+      if (a.epi.dkind == LT_DERIV_BITS) {
+        nib <<= 4 * g;
+        nib |= __shfl_xor(nib, 16, 64);
+        nib |= __shfl_xor(nib, 32, 64);
+        if (g == 0 && row < a.rows && col < a.cols)
+          ((uint16_t*)a.epi.deriv)[row * ((a.cols + 15) >> 4) + (col >> 4)] = (uint16_t)nib;
+      }
+    }
+  }
+}
+
+// ---- host: which kernel, which tile, how many splits
+// tile shapes (rows x columns of the output)
+enum { LT_TILE_256x256, LT_TILE_128x128, LT_TILE_128x64, LT_TILE_256x32, LT_TILE_64x64 };
+
+struct LtPlan {
+  int tile, tr, tc, splits;
+  int64_t slice;
+  bool few, direct;
+};
+
+static inline LtPlan lt_gemm_plan(int64_t rows, int cols, int64_t depth, int dt, bool nn, bool direct, bool few_ok) {
+  LtPlan p = {};
+  p.direct = direct;
+  p.splits = 1;
+  p.slice = depth;
+  // up to 64 rows the tile kernels would leave most of a tile idle; both operands must run along k
+  p.few = few_ok && nn && rows <= 64;
+  if (p.few || rows <= 0 || depth <= 0) return p;
+  const int bk = dt == LT_DT_F32 ? 32 : 64;
+  auto tiles = [&](int br, int bc) { return ((rows + br - 1) / br) * ((cols + bc - 1) / bc); };
+  int br, bc;
+  if (direct && dt != LT_DT_F32 && cols >= 192 && tiles(256, 256) >= 192) p.tile = LT_TILE_256x256, br = 256, bc = 256;
+  else if (cols <= 32 && direct) p.tile = LT_TILE_256x32, br = 256, bc = 32;
+  else if (cols <= 64 && direct) p.tile = LT_TILE_128x64, br = 128, bc = 64;
+  else if (tiles(128, 128) >= 128 || rows * (int64_t)cols >= 128 * 128 * 32) p.tile = LT_TILE_128x128, br = 128, bc = 128;
+  else p.tile = LT_TILE_64x64, br = 64, bc = 64;
+  p.tr = (int)((rows + br - 1) / br);
+  p.tc = (cols + bc - 1) / bc;
+  // fewer tiles than the chip runs at once: split k, at least four steps each
+  const int64_t t = (int64_t)p.tr * p.tc, steps = (depth + bk - 1) / bk;
+  if (p.tile != LT_TILE_256x256 && t < 256) {
+    int64_t s = (512 + t - 1) / t;
+    if (s > steps / 4) s = steps / 4;
+    if (s > 256) s = 256;
+    if (s > 1) {
+      const int64_t per = (steps + s - 1) / s;
+      p.slice = per * bk;
+      p.splits = (int)((steps + per - 1) / per);
+    }
+  }
+  return p;
+}
+
+// the launches for one value type (dense_f32.hip, dense_bf16.hip, dense_f16.hip)
+template <class T> int lt_gemm_launch(const LtGemm& g, const LtPlan& p, float* part, hipStream_t stream);
+
+template <class T, bool PKM, bool QKM, int BR, int BC, int WR, int WC, bool DIRECT, bool P8, int ACT>
+static int lt_launch_tile(const LtTileArgs& a, hipStream_t stream) {
+  const int smem = 2 * (BR + BC) * 128;
+  if (smem > 65536)
+    LT_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_dense<T, PKM, QKM, BR, BC, WR, WC, DIRECT, P8, ACT>),
+                                     hipFuncAttributeMaxDynamicSharedMemorySize, smem));
+  hipLaunchKernelGGL((k_dense<T, PKM, QKM, BR, BC, WR, WC, DIRECT, P8, ACT>), dim3((unsigned)a.tr * a.tc * a.splits),
+                     dim3(64 * WR * WC), smem, stream, a);
+  LT_LAUNCH_CHECK();
+  return LT_OK;
+}
+
+template <class T, bool PKM, bool QKM, int ACT>
+static int lt_launch_shape(const LtPlan& p, const LtTileArgs& a, bool p8, hipStream_t stream) {
+  if constexpr (PKM && QKM) {
+    if (p8) {
+      if (p.tile == LT_TILE_128x128) return lt_launch_tile<T, true, true, 128, 128, 2, 2, false, true, LT_ACT_NONE>(a, stream);
+      return lt_launch_tile<T, true, true, 64, 64, 2, 2, false, true, LT_ACT_NONE>(a, stream);
+    }
+  }
+  if (p.direct) {
+    switch (p.tile) {
+      case LT_TILE_256x256:
+        if constexpr (sizeof(T) == 2) return lt_launch_tile<T, PKM, QKM, 256, 256, 2, 4, true, false, ACT>(a, stream);
+        break;
+      case LT_TILE_128x128: return lt_launch_tile<T, PKM, QKM, 128, 128, 2, 2, true, false, ACT>(a, stream);
+      case LT_TILE_128x64: return lt_launch_tile<T, PKM, QKM, 128, 64, 2, 2, true, false, ACT>(a, stream);
+      case LT_TILE_256x32: return lt_launch_tile<T, PKM, QKM, 256, 32, 4, 1, true, false, ACT>(a, stream);
+      default: return lt_launch_tile<T, PKM, QKM, 64, 64, 2, 2, true, false, ACT>(a, stream);
+    }
+  }
+  if (p.tile == LT_TILE_128x128) return lt_launch_tile<T, PKM, QKM, 128, 128, 2, 2, false, false, ACT>(a, stream);
+  return lt_launch_tile<T, PKM, QKM, 64, 64, 2, 2, false, false, ACT>(a, stream);
+}
+
+template <class T, int ACT>
+static int lt_launch_few(const LtTileArgs& a, hipStream_t stream) {
+  const dim3 grid((a.cols + 15) / 16), block(512);
+  const int fr = (int)((a.rows + 15) / 16);
+  if (fr == 1) hipLaunchKernelGGL((k_dense_few<T, 1, ACT>), grid, block, 0, stream, a);
+  else if (fr == 2) hipLaunchKernelGGL((k_dense_few<T, 2, ACT>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((k_dense_few<T, 4, ACT>), grid, block, 0, stream, a);
+  LT_LAUNCH_CHECK();
+  return LT_OK;
+}
+
+template <class T, int ACT>
+static int lt_launch_join(const LtEpi& e, const float* part, int splits, hipStream_t stream) {
+  const int64_t n = e.rows * (int64_t)(((e.cols + 15) >> 4) * 4);
+  if (splits >= 64) hipLaunchKernelGGL((k_dense_join<T, ACT, 16>), dim3(lt_grid(n, 16)), dim3(256), 0, stream, part, splits, e);
+  else if (splits >= 8) hipLaunchKernelGGL((k_dense_join<T, ACT, 4>), dim3(lt_grid(n, 64)), dim3(256), 0, stream, part, splits, e);
+  else hipLaunchKernelGGL((k_dense_join<T, ACT, 1>), dim3(lt_grid(n, 256)), dim3(256), 0, stream, part, splits, e);
+  LT_LAUNCH_CHECK();
+  return LT_OK;
+}
+
+template <class T, int ACT>
+static int lt_gemm_launch_act(const LtGemm& g, const LtPlan& p, const LtTileArgs& a, float* part, hipStream_t stream) {
+  int rc = LT_OK;
+  if (g.depth > 0) {
+    if (p.few) return lt_launch_few<T, ACT>(a, stream);
+    if (!g.p_kmajor) rc = lt_launch_shape<T, false, false, ACT>(p, a, false, stream);
+    else if constexpr (ACT == LT_ACT_NONE) {
+      if (!g.q_kmajor) rc = lt_launch_shape<T, true, false, ACT>(p, a, false, stream);
+      else rc = lt_launch_shape<T, true, true, ACT>(p, a, g.p_scales != nullptr, stream);
+    }
+    if (rc) return rc;
+    if (p.splits == 1) return LT_OK;
+  }
+  return lt_launch_join<T, ACT>(g.epi, part, g.depth > 0 ? p.splits : 0, stream);   // no k at all: the sum is zero
+}
+
+template <class T>
+static int lt_gemm_launch_impl(const LtGemm& g, const LtPlan& p, float* part, hipStream_t stream) {
+  LtTileArgs a = {};
+  a.P = (const char*)g.P;
+  a.Q = (const char*)g.Q;
+  a.ldp = g.ldp * (g.p_scales ? 1 : (int64_t)sizeof(T));
+  a.ldq = g.ldq * (int64_t)sizeof(T);
+  a.rows = g.rows;
+  a.depth = g.depth;
+  a.cols = g.cols;
+  a.tr = p.tr;
+  a.tc = p.tc;
+  a.splits = p.splits;
+  a.slice = p.slice;
+  a.part = part;
+  a.ps = g.p_scales;
+  a.ldps = (g.cols + 31) / 32;
+  a.epi = g.epi;
+  switch (g.act) {
+    case LT_ACT_RELU: return lt_gemm_launch_act<T, LT_ACT_RELU>(g, p, a, part, stream);
+    case LT_ACT_GELU: return lt_gemm_launch_act<T, LT_ACT_GELU>(g, p, a, part, stream);
+    case LT_ACT_SILU: return lt_gemm_launch_act<T, LT_ACT_SILU>(g, p, a, part, stream);
+    default: return lt_gemm_launch_act<T, LT_ACT_NONE>(g, p, a, part, stream);
+  }
+}

@@ -1,0 +1,207 @@
+"""Dense layers on the HIP kernels: linear with its epilogue and its backward, and activations kept in 8 bits ("mx8").
+
+Tensor-level calls and autograd nodes over the `lt_mx8_*` and `lt_linear_*` entry points of include/latte_hip.h; the public
+names are re-exported by latte_amd.functional, the modules are latte_amd.sparse_modules.Linear / RMSNorm.  Types: fp32,
+bfloat16, float16 (all operands of a call share one); sums are fp32.  GPU tensors only: there is no CPU fallback."""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .ops import _p, _ws_bytes
+
+__all__ = ["Mx8", "quantize_mx8", "linear"]
+
+_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ACT = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+_BITS, _BYTE, _FULL = 1, 2, 3     # LT_DERIV_*
+
+
+def _dt(t: torch.Tensor, name: str) -> int:
+    if not t.is_cuda:
+        raise _lib.LatteHipError(f"{name}: tensor must be on the GPU (no CPU fallback in the product path)")
+    d = _DT.get(t.dtype)
+    if d is None:
+        raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    return d
+
+
+def _like(t, ref: torch.Tensor, shape, name: str):
+    """`t` checked against the operand it goes with: type, device, shape"""
+    if t.dtype != ref.dtype:
+        raise TypeError(f"{name}: expected {ref.dtype}, got {t.dtype}")
+    if t.device != ref.device:
+        raise ValueError(f"{name}: on {t.device}, the other operands on {ref.device}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    return t
+
+
+def _rows(t: torch.Tensor, cols: int):
+    """-> (2-D tensor with neighbouring columns, its row stride): a view wherever the strides allow one"""
+    t2 = t if t.dim() == 2 else t.reshape(-1, cols)
+    if t2.stride(1) != 1 and cols > 1:
+        t2 = t2.contiguous()
+    # a single row's stride means nothing; negative strides do not exist in torch
+    return t2, (t2.stride(0) if t2.shape[0] > 1 else cols)
+
+
+def _stream_of(t: torch.Tensor):
+    """the current stream of the tensor's own device, whatever device is current"""
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(t.device.index))
+
+
+def _buf(nbytes: int, device) -> torch.Tensor:
+    """workspace of one call: torch's allocator (and a graph's private pool) keeps it from any other stream or graph"""
+    return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+
+
+# ------------------------------------------------------------------ mx8
+class Mx8:
+    """A matrix held in 8 bits: `values` float8_e4m3fn [M, K] and `scales` uint8 [M, ceil(K / 32)] -- element (i, j) stands for
+    values[i, j] * 2^(scales[i, j // 32] - 127)."""
+
+    __slots__ = ("values", "scales")
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor):
+        if values.dtype != torch.float8_e4m3fn or values.dim() != 2:
+            raise TypeError(f"Mx8: values must be a float8_e4m3fn matrix, got {values.dtype} {tuple(values.shape)}")
+        if scales.dtype != torch.uint8 or tuple(scales.shape) != (values.shape[0], (values.shape[1] + 31) // 32):
+            raise ValueError(f"Mx8: scales must be uint8 [M, ceil(K / 32)], got {scales.dtype} {tuple(scales.shape)} "
+                             f"for values {tuple(values.shape)}")
+        if values.device != scales.device:
+            raise ValueError(f"Mx8: values on {values.device}, scales on {scales.device}")
+        self.values = values.contiguous()
+        self.scales = scales.contiguous()
+
+    @property
+    def shape(self):
+        return self.values.shape
+
+    @property
+    def device(self):
+        return self.values.device
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """the values it stands for (exact in float32 and bfloat16)"""
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        dt = _dt(out, "Mx8.dequantize")
+        M, K = self.shape
+        _lib.call("lt_mx8_dequantize", _p(self.values), _p(self.scales), M, K, dt, _p(out), _stream_of(out))
+        return out
+
+    @staticmethod
+    def empty(M: int, K: int, device) -> "Mx8":
+        return Mx8(torch.empty((M, K), dtype=torch.float8_e4m3fn, device=device),
+                   torch.empty((M, (K + 31) // 32), dtype=torch.uint8, device=device))
+
+
+def quantize_mx8(x: torch.Tensor) -> Mx8:
+    """x [..., K] -> Mx8 [rows, K]: 32 neighbours share the smallest power of two that brings their largest finite magnitude
+    to at most 448; nearest even e4m3.  Infinities and NaN are held as NaN."""
+    dt = _dt(x, "quantize_mx8")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"quantize_mx8: expected rows of at least one element, got shape {tuple(x.shape)}")
+    K = x.shape[-1]
+    x2, ld = _rows(x.detach(), K)
+    q = Mx8.empty(x2.shape[0], K, x.device)
+    _lib.call("lt_mx8_quantize", _p(x2), ld, x2.shape[0], K, dt, _p(q.values), _p(q.scales), _stream_of(x2))
+    return q
+
+
+# ------------------------------------------------------------------ linear
+def _linear_fwd(x2, ldx, w, ldw, bias, res, act: str, deriv_kind: int):
+    """-> (y [M, N], deriv | None)"""
+    M, K = x2.shape
+    N = w.shape[0]
+    dt = _DT[x2.dtype]
+    dev = x2.device
+    y = torch.empty((M, N), dtype=x2.dtype, device=dev)
+    deriv = None
+    if deriv_kind == _BITS:
+        deriv = torch.empty((M, (N + 15) // 16), dtype=torch.int16, device=dev)
+    elif deriv_kind == _BYTE:
+        deriv = torch.empty((M, N), dtype=torch.uint8, device=dev)
+    elif deriv_kind == _FULL:
+        deriv = torch.empty((M, N), dtype=x2.dtype, device=dev)
+    nb = _ws_bytes("lt_linear_workspace_bytes", M, K, N, dt)
+    ws = _buf(nb, dev) if nb > 0 else None
+    r2, ldr = _rows(res, N) if res is not None else (None, 0)
+    _lib.call("lt_linear_fwd", _p(x2), ldx, _p(w), ldw, _p(bias), _p(r2), ldr, _ACT[act], M, K, N, dt, _p(y), _p(deriv),
+              deriv_kind, _p(ws), nb, _stream_of(x2))
+    return y, deriv
+
+
+class _Linear(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act, checkpoint):
+        K, N = x.shape[-1], weight.shape[0]
+        x2, ldx = _rows(x, K)
+        w2, ldw = _rows(weight, K)
+        need = ctx.needs_input_grad
+        grads = need[0] or need[1] or need[2]
+        kind = 0
+        if grads and act != "none":
+            kind = _BITS if act == "relu" else (_BYTE if checkpoint == "mx8" else _FULL)
+        b = bias.contiguous() if bias is not None else None
+        y, deriv = _linear_fwd(x2, ldx, w2, ldw, b, residual, act, kind)
+        keep_x, x_scales = None, None
+        if need[1]:
+            if checkpoint == "mx8":
+                q = quantize_mx8(x2)
+                keep_x, x_scales = q.values, q.scales
+            else:
+                keep_x = x2
+        ctx.kind, ctx.x_shape = kind, x.shape
+        ctx.save_for_backward(keep_x, x_scales, w2 if need[0] else None, deriv)
+        ctx.meta = (K, N, weight.dtype)
+        return y.view(*x.shape[:-1], N)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x2, xs, w2, deriv = ctx.saved_tensors
+        K, N, dtype = ctx.meta
+        need = ctx.needs_input_grad
+        dev = dy.device
+        dy2, lddy = _rows(dy, N)
+        M = dy2.shape[0]
+        dx = torch.empty((M, K), dtype=dtype, device=dev) if need[0] else None
+        dw = torch.empty((N, K), dtype=dtype, device=dev) if need[1] else None
+        db = torch.empty((N,), dtype=dtype, device=dev) if need[2] else None
+        if dx is not None or dw is not None or db is not None:
+            dt = _DT[dtype]
+            nb = _ws_bytes("lt_linear_bwd_workspace_bytes", M, K, N, dt)
+            ws = _buf(nb, dev)
+            ldx = 0 if x2 is None else (K if xs is not None else _rows(x2, K)[1])
+            ldw = 0 if w2 is None else _rows(w2, K)[1]
+            _lib.call("lt_linear_bwd", _p(dy2), lddy, _p(x2), ldx, _p(xs), _p(w2), ldw, _p(deriv), ctx.kind, M, K, N, dt,
+                      _p(dx), _p(dw), _p(db), _p(ws), ws.numel(), _stream_of(dy2))
+        return (dx.view(ctx.x_shape) if dx is not None else None), dw, db, (dy if need[3] else None), None, None
+
+
+def linear(x, weight, bias=None, act: str = "none", residual=None, checkpoint: str | None = None):
+    """act(x @ weight.T + bias) + residual as one kernel; act: "none" | "relu" | "gelu" (exact) | "silu".
+
+    x [..., K], weight [N, K], bias [N], residual [..., N] -> [..., N], all of one type (float32, bfloat16, float16), sums in
+    fp32.  Differentiable in all four; the backward pass reads x, weight and act'.  checkpoint="mx8" keeps what it reads of x
+    in 8 bits (quantize_mx8: relative error at most 2^-4 an element) and act' of GELU / SiLU on a uniform 8-bit grid
+    (error at most 1/384); the ReLU's act' is one bit either way.  The output does not depend on `checkpoint`."""
+    if act not in _ACT:
+        raise ValueError(f"linear: act must be one of {sorted(_ACT)}, got {act!r}")
+    if checkpoint not in (None, "mx8"):
+        raise ValueError(f"linear: checkpoint must be None or 'mx8', got {checkpoint!r}")
+    _dt(x, "linear x")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or min(weight.shape) < 1:
+        raise ValueError(f"linear: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not go together")
+    N, K = weight.shape
+    _like(weight, x, (N, K), "linear weight")
+    if bias is not None:
+        _like(bias, x, (N,), "linear bias")
+    if residual is not None:
+        _like(residual, x, (*x.shape[:-1], N), "linear residual")
+    return _Linear.apply(x, weight, bias, residual, act, checkpoint)

@@ -10,9 +10,10 @@ import torch
 from torch.autograd import Function
 
 from . import ops
+from .dense import Mx8, linear, quantize_mx8
 
 __all__ = ["KernelMap", "get_kernel_offsets", "sparse_conv", "conv_bn", "batch_norm", "spvoxelize", "spdevoxelize",
-           "invalidate_packed", "bump_pack_epoch"]
+           "invalidate_packed", "bump_pack_epoch", "Mx8", "quantize_mx8", "linear"]
 
 _OFFSET_CACHE: dict = {}
 
