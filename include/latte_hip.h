@@ -345,6 +345,37 @@ int lt_linear_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, cons
                   const void* deriv, int32_t deriv_kind, int64_t M, int32_t K, int32_t N, int32_t dt, void* dx, void* dw,
                   void* db, void* ws, int64_t ws_bytes, lt_stream_t stream);
 
+/* h = x + res;  y = h / sqrt(mean over the row of h^2 + eps) * w  (res NULL: h = x).  A norm without batch statistics, beside
+ * lt_bn_* (latte/models/basic_blocks.py:22-75).  Written where not NULL: h [M][C], y [M][C] (type dt), y8 / y8_scales (y in
+ * mx8), h8 / h8_scales (h in mx8, for the backward), rstd [M].  C <= 16384. */
+int lt_rms_norm_fwd(const void* x, int64_t ldx, const void* res, int64_t ldres, const void* w, float eps, int64_t M, int32_t C,
+                    int32_t dt, void* h, void* y, void* y8, void* y8_scales, void* h8, void* h8_scales, float* rstd,
+                    lt_stream_t stream);
+/* n = h rstd, g = dy w:  dx = rstd (g - n mean(g n)) + dh,  dw = column sums of dy n.  h (or h8 / h8_scales: h NULL), rstd:
+ * what the forward left; dh, dx, dw may be NULL.  The same bits every time. */
+int64_t lt_rms_norm_bwd_workspace_bytes(int64_t M, int32_t C);
+int lt_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, int64_t lddh, const void* h, int64_t ldh, const void* h8,
+                    const void* h8_scales, const void* w, const float* rstd, int64_t M, int32_t C, int32_t dt, void* dx, void* dw,
+                    void* ws, int64_t ws_bytes, lt_stream_t stream);
+/* lt_bn_apply / lt_bn_bwd_reduce / lt_bn_bwd_apply with what the backward reads held in 8 bits: values uint8 [V][C] and
+ * scales [V][ceil(C/32)] = x - c in mx8 (c: the mean rounded to a multiple of a quarter of the power of two at or below the
+ * standard deviation), mask uint16 [V][ceil(C/16)] = the ReLU's bits (NULL without a ReLU).  y is bit-equal to lt_bn_apply's;
+ * the gradients are those of xhat = (held + c - mean) / sqrt(var + eps). */
+int lt_bn_apply_mx8(const float* x, const float* mean, const float* var, const float* gamma, const float* beta, float eps,
+                    const float* residual, int32_t relu, float* y, void* values, void* scales, void* mask, int64_t V, int32_t C,
+                    lt_stream_t stream);
+int lt_bn_bwd_reduce_mx8(const float* dy, const void* values, const void* scales, const void* mask, const float* mean,
+                         const float* var, float eps, int64_t V, int32_t C, void* ws, int64_t ws_bytes, float* sum_g,
+                         float* sum_gx, lt_stream_t stream);
+int lt_bn_bwd_apply_mx8(const float* dy, const void* values, const void* scales, const void* mask, const float* mean,
+                        const float* var, const float* gamma, float eps, const float* sum_g, const float* sum_gx, float* dx,
+                        float* dres, int64_t V, int32_t C, lt_stream_t stream);
+/* y[M][N] = act(x w^T + bias) + res with x [M][K] and w [N][K] in mx8; y, bias, res of type dt (LT_DT_BF16 | LT_DT_F16) */
+int64_t lt_linear_mx8_workspace_bytes(int64_t M, int32_t K, int32_t N);
+int lt_linear_mx8_fwd(const void* x, const void* x_scales, const void* w, const void* w_scales, const void* bias, const void* res,
+                      int64_t ldres, int32_t act, int64_t M, int32_t K, int32_t N, int32_t dt, void* y, void* ws, int64_t ws_bytes,
+                      lt_stream_t stream);
+
 /* ------------------------------------------------------------------ ST-voxel aggregation (HR_Block / CR_Block)
  * see latte/models/hr_module.py:135-331 and :344-420; declared in the second half of this header */
 #include "latte_hip_st.h"

@@ -91,6 +91,38 @@ __device__ __forceinline__ void lt_mx8_get2(int word, float s, float& a, float& 
   b = v[1];
 }
 
+// 8 neighbours of a row whose block of 32 the four lanes of an aligned group hold together (all four must call): n = how
+// many of the 8 exist (<= 0: none, nothing is stored), q / sc = where they and the block's scale go
+__device__ __forceinline__ void lt_mx8_put8(const float (&v)[8], int n, int max_exp, uint8_t* q, uint8_t* sc) {
+  float a = 0.f;
+#pragma unroll
+  for (int t = 0; t < 8; ++t) a = fmaxf(a, t < n ? lt_finite_abs(v[t]) : 0.f);
+  a = fmaxf(a, __shfl_xor(a, 1, 64));
+  a = fmaxf(a, __shfl_xor(a, 2, 64));
+  if (n <= 0) return;
+  const int e = lt_mx8_exp(a);
+  const float inv = lt_two_to(-e), lim = lt_mx8_lim(a, max_exp);
+  int w[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+    w[t] = (lt_mx8_pack2(v[4 * t], v[4 * t + 1], inv, lim) & 0xFFFF) | (lt_mx8_pack2(v[4 * t + 2], v[4 * t + 3], inv, lim) << 16);
+  if (n >= 8) __builtin_memcpy(q, w, 8);
+  else
+    for (int t = 0; t < n; ++t) q[t] = (uint8_t)(w[t >> 2] >> (8 * (t & 3)));
+  if ((threadIdx.x & 3) == 0) *sc = (uint8_t)(e + 127);
+}
+__device__ __forceinline__ void lt_mx8_get8(const uint8_t* q, int n, uint8_t sc, float (&v)[8]) {
+  int w[2] = {0, 0};
+  if (n >= 8) __builtin_memcpy(w, q, 8);
+  else
+    for (int t = 0; t < n; ++t) w[t >> 2] |= (int)q[t] << (8 * (t & 3));
+  const float s = __uint_as_float((unsigned)sc << 23);
+  lt_mx8_get2<0>(w[0], s, v[0], v[1]);
+  lt_mx8_get2<1>(w[0], s, v[2], v[3]);
+  lt_mx8_get2<0>(w[1], s, v[4], v[5]);
+  lt_mx8_get2<1>(w[1], s, v[6], v[7]);
+}
+
 // ---- activations and their derivatives
 // act'(z) in a byte: (c - 32) / 192, c = 0..254 (0 and 1 exactly; gelu' and silu' stay inside [-0.13, 1.13]); 255 is NaN.
 __device__ __forceinline__ unsigned lt_deriv_byte(float d) {
@@ -191,6 +223,25 @@ __device__ __forceinline__ void lt_epi4(const LtEpi& e, lt_f32x4 acc, const floa
 #pragma unroll
   for (int i = 0; i < 4; ++i) y[i] += r[i];
   lt_stv<T, 4>((T*)e.out + row * e.ldo + col, n, y);
+}
+
+// out[c] = sum over slabs of part[slab][c]: 16 columns a workgroup, 16 threads a column, fixed order
+template <class T>
+__global__ __launch_bounds__(256) void k_col_join(const float* __restrict__ part, int slabs, int N, T* __restrict__ out) {
+  __shared__ float s_sum[16][17];
+  const int c = threadIdx.x & 15, l = threadIdx.x >> 4;
+  const int col = blockIdx.x * 16 + c;
+  float s = 0.f;
+  if (col < N) {
+#pragma unroll 8
+    for (int i = l; i < slabs; i += 16) s += part[(int64_t)i * N + col];
+  }
+  s_sum[l][c] = s;
+  __syncthreads();
+  if (l == 0 && col < N) {
+    for (int i = 1; i < 16; ++i) s += s_sum[i][c];
+    out[col] = (T)s;
+  }
 }
 
 // ---- host side

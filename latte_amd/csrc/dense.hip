@@ -88,25 +88,6 @@ __global__ __launch_bounds__(256) void k_dz(const T* __restrict__ dy, int64_t ld
   }
 }
 
-// out[c] = sum over slabs of part[slab][c]: 16 columns a workgroup, 16 threads a column, fixed order
-template <class T>
-__global__ __launch_bounds__(256) void k_col_join(const float* __restrict__ part, int slabs, int N, T* __restrict__ out) {
-  __shared__ float s_sum[16][17];
-  const int c = threadIdx.x & 15, l = threadIdx.x >> 4;
-  const int col = blockIdx.x * 16 + c;
-  float s = 0.f;
-  if (col < N) {
-#pragma unroll 8
-    for (int i = l; i < slabs; i += 16) s += part[(int64_t)i * N + col];
-  }
-  s_sum[l][c] = s;
-  __syncthreads();
-  if (l == 0 && col < N) {
-    for (int i = 1; i < 16; ++i) s += s_sum[i][c];
-    out[col] = (T)s;
-  }
-}
-
 struct DzPlan {
   int tx, gx, slabs;
   int64_t rows_per;
@@ -165,23 +146,7 @@ __global__ __launch_bounds__(256) void k_mx8_quantize(const T* __restrict__ x, i
     const int col = l * 8;
     float v[8];
     lt_ldv<T, 8>(x + row * ldx + col, live ? K - col : 0, v);
-    float a = 0.f;
-#pragma unroll
-    for (int t = 0; t < 8; ++t) a = fmaxf(a, lt_finite_abs(v[t]));
-    a = fmaxf(a, __shfl_xor(a, 1, 64));
-    a = fmaxf(a, __shfl_xor(a, 2, 64));
-    if (!live) continue;
-    const int e = lt_mx8_exp(a);
-    const float inv = lt_two_to(-e), lim = lt_mx8_lim(a, LtType<T>::kMaxExp);
-    int w[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-      w[t] = (lt_mx8_pack2(v[4 * t], v[4 * t + 1], inv, lim) & 0xFFFF) | (lt_mx8_pack2(v[4 * t + 2], v[4 * t + 3], inv, lim) << 16);
-    uint8_t* o = q + row * K + col;
-    if (K - col >= 8) __builtin_memcpy(o, w, 8);
-    else
-      for (int t = 0; t < K - col; ++t) o[t] = (uint8_t)(w[t >> 2] >> (8 * (t & 3)));
-    if ((threadIdx.x & 3) == 0) sc[row * nb + (l >> 2)] = (uint8_t)(e + 127);
+    lt_mx8_put8(v, live ? K - col : 0, LtType<T>::kMaxExp, q + row * K + col, sc + row * nb + (l >> 2));
   }
 }
 
@@ -196,17 +161,8 @@ __global__ __launch_bounds__(256) void k_mx8_dequantize(const uint8_t* __restric
     lt_divmod(i, L, row, l);
     const int col = l * 8, m = K - col;
     if (m <= 0) continue;
-    const uint8_t* p = q + row * K + col;
-    int w[2] = {0, 0};
-    if (m >= 8) __builtin_memcpy(w, p, 8);
-    else
-      for (int t = 0; t < m; ++t) w[t >> 2] |= (int)p[t] << (8 * (t & 3));
-    const float s = __uint_as_float((unsigned)sc[row * nb + (l >> 2)] << 23);
     float v[8];
-    lt_mx8_get2<0>(w[0], s, v[0], v[1]);
-    lt_mx8_get2<1>(w[0], s, v[2], v[3]);
-    lt_mx8_get2<0>(w[1], s, v[4], v[5]);
-    lt_mx8_get2<1>(w[1], s, v[6], v[7]);
+    lt_mx8_get8(q + row * K + col, m, sc[row * nb + (l >> 2)], v);
     lt_stv<T, 8>(out + row * K + col, m, v);
   }
 }

@@ -1,0 +1,80 @@
+// lt_linear_mx8_fwd: both operands in mx8 (kernels and reasons: dense8.h).
+#include "dense8.h"
+
+template <> int lt_gemm8_launch<lt_bf16>(const LtTile8Args&, const LtPlan&, int, hipStream_t);
+template <> int lt_gemm8_launch<lt_f16>(const LtTile8Args&, const LtPlan&, int, hipStream_t);
+
+static LtPlan plan8(int64_t M, int K, int N, bool direct) {
+  LtPlan p = {};
+  p.direct = direct;
+  p.splits = 1;
+  p.slice = K;
+  p.few = M <= 64;
+  if (p.few) return p;
+  auto tiles = [&](int b) { return ((M + b - 1) / b) * ((N + b - 1) / b); };
+  int b = 64;
+  p.tile = LT_TILE_64x64;
+  if (direct && N >= 192 && tiles(256) >= 192) p.tile = LT_TILE_256x256, b = 256;
+  else if (direct && tiles(128) >= 128) p.tile = LT_TILE_128x128, b = 128;
+  p.tr = (int)((M + b - 1) / b);
+  p.tc = (N + b - 1) / b;
+  const int64_t t = (int64_t)p.tr * p.tc, steps = (K + 127) / 128;
+  if (b != 256 && t < 256) {   // fewer tiles than the chip runs at once: split k, at least four steps each
+    int64_t s = (512 + t - 1) / t;
+    if (s > steps / 4) s = steps / 4;
+    if (s > 1) {
+      const int64_t per = (steps + s - 1) / s;
+      p.slice = per * 128;
+      p.splits = (int)((steps + per - 1) / per);
+    }
+  }
+  return p;
+}
+static int64_t part8(const LtPlan& p, int64_t M, int N) { return p.splits > 1 ? p.splits * M * N * 4 : 0; }
+
+static int check8(const char* who, int64_t M, int32_t K, int32_t N) {
+  LT_REQUIRE(M >= 0 && M <= (int64_t)1 << 40 && K >= 1 && N >= 1 && K <= INT32_MAX - 1024 && N <= INT32_MAX - 1024, LT_ERR_ARG,
+             "%s: bad sizes M=%lld K=%d N=%d", who, (long long)M, K, N);
+  return LT_OK;
+}
+
+extern "C" int64_t lt_linear_mx8_workspace_bytes(int64_t M, int32_t K, int32_t N) {
+  if (check8("lt_linear_mx8_workspace_bytes", M, K, N)) return -1;
+  if (M == 0) return 0;
+  const int64_t a = part8(plan8(M, K, N, true), M, N), b = part8(plan8(M, K, N, false), M, N);
+  return a > b ? a : b;
+}
+
+extern "C" int lt_linear_mx8_fwd(const void* x, const void* x_scales, const void* w, const void* w_scales, const void* bias,
+                                 const void* res, int64_t ldres, int32_t act, int64_t M, int32_t K, int32_t N, int32_t dt, void* y,
+                                 void* ws, int64_t ws_bytes, hipStream_t stream) {
+  int rc = check8("lt_linear_mx8_fwd", M, K, N);
+  if (rc) return rc;
+  LT_REQUIRE(dt == LT_DT_BF16 || dt == LT_DT_F16, LT_ERR_ARG, "lt_linear_mx8_fwd: type %d: results are bfloat16 or float16", dt);
+  LT_REQUIRE(act >= LT_ACT_NONE && act <= LT_ACT_SILU, LT_ERR_ARG, "lt_linear_mx8_fwd: act=%d is none of LT_ACT_*", act);
+  if (M == 0) return LT_OK;
+  LT_REQUIRE(x && x_scales && w && w_scales && y, LT_ERR_ARG, "lt_linear_mx8_fwd: null pointer");
+  LtOnStream on;
+  if ((rc = on.enter(stream))) return rc;
+  const bool direct = K % 16 == 0 && ((uintptr_t)x & 15) == 0 && ((uintptr_t)w & 15) == 0 && (int64_t)K * 256 < (int64_t)1 << 31;
+  const LtPlan p = plan8(M, K, N, direct);
+  LT_REQUIRE(part8(p, M, N) <= (ws ? ws_bytes : 0), LT_ERR_WORKSPACE, "lt_linear_mx8_fwd: workspace too small");
+  LT_REQUIRE((int64_t)p.tr * p.tc * p.splits < (int64_t)1 << 31, LT_ERR_RANGE, "lt_linear_mx8_fwd: too many tiles");
+  LtTile8Args b = {};
+  b.t.P = (const char*)w;
+  b.t.Q = (const char*)x;
+  b.t.ldp = b.t.ldq = K;
+  b.t.rows = M;
+  b.t.cols = N;
+  b.t.depth = K;
+  b.t.tr = p.tr;
+  b.t.tc = p.tc;
+  b.t.splits = p.splits;
+  b.t.slice = p.slice;
+  b.t.part = (float*)ws;
+  b.t.ps = (const uint8_t*)w_scales;
+  b.t.epi = LtEpi{bias, res, ldres, y, N, nullptr, LT_DERIV_NONE, M, N};
+  b.qs = (const uint8_t*)x_scales;
+  b.nb = (K + 31) / 32;
+  return dt == LT_DT_BF16 ? lt_gemm8_launch<lt_bf16>(b, p, act, stream) : lt_gemm8_launch<lt_f16>(b, p, act, stream);
+}

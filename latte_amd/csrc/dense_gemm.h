@@ -46,6 +46,8 @@ template <> struct LtMma<float> {
   }
 };
 
+template <> struct LtMma<uint8_t> { typedef lt_i32x8 frag; };   // mx8: dense8.h
+
 template <class T, bool KM, int R>   // an operand's tile: R rows (or columns) of the product, 128 bytes' worth of k
 struct LtTile {
   static constexpr int SZ = sizeof(T), CH = 16 / SZ, BK = 128 / SZ;
@@ -199,6 +201,52 @@ __device__ __forceinline__ unsigned lt_xcd_map(unsigned b, unsigned n) {
   return x * per + (x < rem ? x : rem) + (b >> 3);
 }
 
+// a wave's accumulators -> partial sums of its split, or the epilogue; (row0, col0) = the wave's corner
+template <class T, int FR, int FC, int ACT>
+__device__ __forceinline__ void lt_tile_store(const LtTileArgs& a, const lt_f32x4 (&acc)[FR][FC], unsigned split, int64_t row0, int col0,
+                                              int lane) {
+  const int r = lane & 15, g = lane >> 4;
+  if (a.splits > 1) {
+#pragma unroll
+    for (int i = 0; i < FR; ++i)
+#pragma unroll
+      for (int j = 0; j < FC; ++j) {
+        const int64_t row = row0 + 16 * i + r;
+        const int col = col0 + 16 * j + 4 * g;
+        if (row < a.rows && col < a.cols) {
+          const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+          lt_stv<float, 4>(a.part + ((int64_t)split * a.rows + row) * a.cols + col, a.cols - col, v);
+        }
+      }
+    return;
+  }
+  float b[FC][4];
+#pragma unroll
+  for (int j = 0; j < FC; ++j) lt_epi_bias<T>(a.epi, col0 + 16 * j + 4 * g, b[j]);
+#pragma unroll
+  for (int i = 0; i < FR; ++i) {
+    const int64_t row = row0 + 16 * i + r;
+    float res[FC][4];
+#pragma unroll
+    for (int j = 0; j < FC; ++j) lt_epi_res<T>(a.epi, row, col0 + 16 * j + 4 * g, res[j]);
+#pragma unroll
+    for (int j = 0; j < FC; ++j) {
+      const int col = col0 + 16 * j + 4 * g;
+      unsigned nib;
+      lt_epi4<T, ACT>(a.epi, acc[i][j], b[j], res[j], row, col, nib);
+      if constexpr (ACT == LT_ACT_RELU) {
+        if (a.epi.dkind == LT_DERIV_BITS) {   // the four lanes of a row join their bits: 16 columns
+          nib <<= 4 * g;
+          nib |= __shfl_xor(nib, 16, 64);
+          nib |= __shfl_xor(nib, 32, 64);
+          if (g == 0 && row < a.rows && col < a.cols)
+            ((uint16_t*)a.epi.deriv)[row * ((a.cols + 15) >> 4) + (col >> 4)] = (uint16_t)nib;
+        }
+      }
+    }
+  }
+}
+
 template <class T, bool PKM, bool QKM, int BR, int BC, int WR, int WC, bool DIRECT, bool P8, int ACT>
 __global__ __launch_bounds__(64 * WR * WC) void k_dense(LtTileArgs a) {
   typedef LtTile<T, PKM, BC> TP;
@@ -287,46 +335,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_dense(LtTileArgs a) {
     }
   }
 
-  const int r = lane & 15, g = lane >> 4;
-  if (a.splits > 1) {
-#pragma unroll
-    for (int i = 0; i < FR; ++i)
-#pragma unroll
-      for (int j = 0; j < FC; ++j) {
-        const int64_t row = row0 + wr + 16 * i + r;
-        const int col = col0 + wc + 16 * j + 4 * g;
-        if (row < a.rows && col < a.cols) {
-          const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-          lt_stv<float, 4>(a.part + ((int64_t)split * a.rows + row) * a.cols + col, a.cols - col, v);
-        }
-      }
-    return;
-  }
-  float b[FC][4];
-#pragma unroll
-  for (int j = 0; j < FC; ++j) lt_epi_bias<T>(a.epi, col0 + wc + 16 * j + 4 * g, b[j]);
-#pragma unroll
-  for (int i = 0; i < FR; ++i) {
-    const int64_t row = row0 + wr + 16 * i + r;
-    float res[FC][4];
-#pragma unroll
-    for (int j = 0; j < FC; ++j) lt_epi_res<T>(a.epi, row, col0 + wc + 16 * j + 4 * g, res[j]);
-#pragma unroll
-    for (int j = 0; j < FC; ++j) {
-      const int col = col0 + wc + 16 * j + 4 * g;
-      unsigned nib;
-      lt_epi4<T, ACT>(a.epi, acc[i][j], b[j], res[j], row, col, nib);
-      if constexpr (ACT == LT_ACT_RELU) {
-        if (a.epi.dkind == LT_DERIV_BITS) {   // the four lanes of a row join their bits: 16 columns
-          nib <<= 4 * g;
-          nib |= __shfl_xor(nib, 16, 64);
-          nib |= __shfl_xor(nib, 32, 64);
-          if (g == 0 && row < a.rows && col < a.cols)
-            ((uint16_t*)a.epi.deriv)[row * ((a.cols + 15) >> 4) + (col >> 4)] = (uint16_t)nib;
-        }
-      }
-    }
-  }
+  lt_tile_store<T, FR, FC, ACT>(a, acc, split, row0 + wr, col0 + wc, lane);
 }
 
 // out = epilogue(sum over the splits, in a fixed order: the same bits every time).  G threads share four neighbours and take
@@ -381,6 +390,37 @@ __global__ __launch_bounds__(256) void k_dense_join(const float* __restrict__ pa
   }
 }
 
+// the eight waves' sums of 16 columns, added in wave order, and their epilogue
+template <class T, int FR, int ACT>
+__device__ __forceinline__ void lt_few_store(const LtTileArgs& a, const lt_f32x4 (&acc)[FR], lt_f32x4 (*s_acc)[FR][64], int col0, int wave,
+                                             int lane) {
+  const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int f = 0; f < FR; ++f) s_acc[wave][f][lane] = acc[f];
+  __syncthreads();
+  if (wave < FR) {
+    lt_f32x4 s = s_acc[0][wave][lane];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) s += s_acc[w][wave][lane];
+    const int64_t row = wave * 16 + r;
+    const int col = col0 + 4 * g;
+    unsigned nib;
+    float b[4], res[4];
+    lt_epi_bias<T>(a.epi, col, b);
+    lt_epi_res<T>(a.epi, row, col, res);
+    lt_epi4<T, ACT>(a.epi, s, b, res, row, col, nib);
+    if constexpr (ACT == LT_ACT_RELU) {
+      if (a.epi.dkind == LT_DERIV_BITS) {
+        nib <<= 4 * g;
+        nib |= __shfl_xor(nib, 16, 64);
+        nib |= __shfl_xor(nib, 32, 64);
+        if (g == 0 && row < a.rows && col < a.cols)
+          ((uint16_t*)a.epi.deriv)[row * ((a.cols + 15) >> 4) + (col >> 4)] = (uint16_t)nib;
+      }
+    }
+  }
+}
+
 // ---- few rows: y[rows <= 64][cols].  Bound by reading P once: a workgroup takes 16 columns, its 8 waves share k in
 // turns of four fragments (256 bytes of each of the 16 lines of P), operands go from memory straight into the matrix
 // instructions' registers (nothing is used twice but the few rows of Q, which the caches hold), and the waves' sums are
@@ -424,30 +464,7 @@ __global__ __launch_bounds__(512) void k_dense_few(LtTileArgs a) {
 #pragma unroll
       for (int f = 0; f < FR; ++f) acc[f] = LtMma<T>::mma(pf[u], qf[f][u], acc[f]);
   }
-#pragma unroll
-  for (int f = 0; f < FR; ++f) s_acc[wave][f][lane] = acc[f];
-  __syncthreads();
-  if (wave < FR) {
-    lt_f32x4 s = s_acc[0][wave][lane];
-#pragma unroll
-    for (int w = 1; w < 8; ++w) s += s_acc[w][wave][lane];
-    const int64_t row = wave * 16 + r;
-    const int col = col0 + 4 * g;
-    unsigned nib;
-    float b[4], res[4];
-    lt_epi_bias<T>(a.epi, col, b);
-    lt_epi_res<T>(a.epi, row, col, res);
-    lt_epi4<T, ACT>(a.epi, s, b, res, row, col, nib);
-    if constexpr (ACT == LT_ACT_RELU) {
-      if (a.epi.dkind == LT_DERIV_BITS) {
-        nib <<= 4 * g;
-        nib |= __shfl_xor(nib, 16, 64);
-        nib |= __shfl_xor(nib, 32, 64);
-        if (g == 0 && row < a.rows && col < a.cols)
-          ((uint16_t*)a.epi.deriv)[row * ((a.cols + 15) >> 4) + (col >> 4)] = (uint16_t)nib;
-      }
-    }
-  }
+  lt_few_store<T, FR, ACT>(a, acc, s_acc, col0, wave, lane);
 }
 
 // ---- host: which kernel, which tile, how many splits

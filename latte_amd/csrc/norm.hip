@@ -7,7 +7,7 @@
 // HBM-bound.  Column reductions: a block owns a slab of rows, a thread owns one float4 column group (16-B
 // loads, a wave reads whole rows), partial sums per block go to a workspace, the finalising kernel combines
 // them in fp64.  Sums are shifted by row 0 so that var = E[d^2]-E[d]^2 does not cancel when |mean| >> std.
-#include "common.h"
+#include "dense.h"
 #include <mutex>
 #include "../../include/latte_hip.h"
 
@@ -659,6 +659,210 @@ extern "C" int lt_bn_bwd_apply(const float* dy, const float* x, const float* y, 
   else
     hipLaunchKernelGGL((k_bn_bwd_apply<false, false>), grid, dim3(256), 0, stream, dy, x, y, mean, var, gamma, beta, eps,
                        sum_g, sum_gx, dx, dres, n4, C / 4, inv_v);
+  LT_LAUNCH_CHECK();
+  return LT_OK;
+}
+
+// ------------------------------------------------------------------ BatchNorm that keeps its input in 8 bits
+// The forward pass leaves x - c in mx8 (dense.h) and the ReLU's mask in bits, (1 + 1/32 + 1/8) bytes an element, and the
+// backward pass reads those instead of x (and y).  c is the channel's mean rounded to a multiple of a quarter of the power
+// of two at or below its standard deviation: at most sd / 8 away from the mean, so that x - c has no offset that would eat
+// up the 4 bits an element is held with, and few-bit, so that x - c rounds the same way whatever order the mean was summed in.
+__device__ __forceinline__ float bn_shift(float mean, float var, float eps) {
+  const int e = (int)(__float_as_uint(sqrtf(var + eps)) >> 23) & 0xFF;
+  if (e < 4 || e == 255) return mean;   // no spread to speak of, or none that is finite
+  const float unit = __uint_as_float((unsigned)(e - 2) << 23);
+  if (!(fabsf(mean) < unit * 16777216.f)) return mean;   // the mean itself has no more bits
+  return rintf(mean * __uint_as_float((unsigned)(256 - e) << 23)) * unit;   // times 1 / unit
+}
+
+// 8 lanes hold a block of 32 columns of one row, 4 each; a thread keeps its columns over all its rows
+__global__ __launch_bounds__(256) void k_bn_apply_mx8(const float* __restrict__ x, const float* __restrict__ mean,
+                                                      const float* __restrict__ var, const float* __restrict__ gamma,
+                                                      const float* __restrict__ beta, float eps, const float* __restrict__ res,
+                                                      int relu, float* __restrict__ y, uint8_t* __restrict__ q,
+                                                      uint8_t* __restrict__ sc, uint8_t* __restrict__ mask, int64_t V, int C) {
+  const int nb = (C + 31) >> 5, L = nb * 8, rpi = 256 / L, mb = ((C + 15) >> 4) * 2;
+  const int l = threadIdx.x % L, rr = threadIdx.x / L, col = 4 * l;
+  const bool cok = col < C && rr < rpi, post = (relu & 2) != 0;
+  float4 m = make_float4(0.f, 0.f, 0.f, 0.f), vr = m, g = m, b = m, c = m;
+  if (cok) {
+    m = *reinterpret_cast<const float4*>(mean + col);
+    vr = *reinterpret_cast<const float4*>(var + col);
+    g = *reinterpret_cast<const float4*>(gamma + col);
+    b = *reinterpret_cast<const float4*>(beta + col);
+    c = make_float4(bn_shift(m.x, vr.x, eps), bn_shift(m.y, vr.y, eps), bn_shift(m.z, vr.z, eps), bn_shift(m.w, vr.w, eps));
+  }
+  for (int64_t r0 = (int64_t)blockIdx.x * rpi; r0 < V; r0 += (int64_t)gridDim.x * rpi) {
+    const int64_t row = r0 + rr;
+    const bool ok = cok && row < V;
+    float4 v = m, r = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (ok) {
+      v = *reinterpret_cast<const float4*>(x + row * C + col);
+      if (res) r = *reinterpret_cast<const float4*>(res + row * C + col);
+    }
+    float4 o = bn_apply4(v, m, vr, g, b, eps);
+    if (res && !post) { o.x += r.x; o.y += r.y; o.z += r.z; o.w += r.w; }
+    unsigned bits = 0;
+    if (relu & 1) {
+      o.x = fmaxf(o.x, 0.f); o.y = fmaxf(o.y, 0.f); o.z = fmaxf(o.z, 0.f); o.w = fmaxf(o.w, 0.f);
+      bits = (o.x > 0.f ? 1u : 0u) | (o.y > 0.f ? 2u : 0u) | (o.z > 0.f ? 4u : 0u) | (o.w > 0.f ? 8u : 0u);
+    }
+    if (res && post) { o.x += r.x; o.y += r.y; o.z += r.z; o.w += r.w; }
+    const float u[4] = {v.x - c.x, v.y - c.y, v.z - c.z, v.w - c.w};
+    float a = 0.f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) a = fmaxf(a, ok ? lt_finite_abs(u[t]) : 0.f);
+    a = fmaxf(a, __shfl_xor(a, 1, 64));
+    a = fmaxf(a, __shfl_xor(a, 2, 64));
+    a = fmaxf(a, __shfl_xor(a, 4, 64));
+    const int e = lt_mx8_exp(a);
+    const float inv = lt_two_to(-e), lim = lt_mx8_lim(a, 127);
+    bits = ok ? bits : 0u;
+    const unsigned other = __shfl_xor(bits, 1, 64);
+    if (ok) {
+      *reinterpret_cast<float4*>(y + row * C + col) = o;
+      *reinterpret_cast<int*>(q + row * C + col) = (lt_mx8_pack2(u[0], u[1], inv, lim) & 0xFFFF) | (lt_mx8_pack2(u[2], u[3], inv, lim) << 16);
+      if ((l & 7) == 0) sc[row * nb + (l >> 3)] = (uint8_t)(e + 127);
+    }
+    if (mask && (l & 1) == 0 && rr < rpi && row < V && (l >> 1) < mb) mask[row * mb + (l >> 1)] = (uint8_t)(bits | (other << 4));
+  }
+}
+
+// column sums of g and g xhat for k_col_partial, xhat = (held + (c - mean)) rstd
+template <bool MASK>
+struct Bwd8Op {
+  const float* dy;
+  const uint8_t *q, *sc, *mask;
+  const float *mean, *var;
+  float eps;
+  struct Cols { float4 off, rs; };
+  struct Ld { float4 g; int w; unsigned s, m; };
+  static constexpr int kLoads = 4;
+  __device__ __forceinline__ Cols cols(int cg) const {
+    const float4 m = reinterpret_cast<const float4*>(mean)[cg], vr = reinterpret_cast<const float4*>(var)[cg];
+    Cols c;
+    c.off = make_float4(bn_shift(m.x, vr.x, eps) - m.x, bn_shift(m.y, vr.y, eps) - m.y, bn_shift(m.z, vr.z, eps) - m.z,
+                        bn_shift(m.w, vr.w, eps) - m.w);
+    c.rs = make_float4(1.0f / sqrtf(vr.x + eps), 1.0f / sqrtf(vr.y + eps), 1.0f / sqrtf(vr.z + eps), 1.0f / sqrtf(vr.w + eps));
+    return c;
+  }
+  __device__ __forceinline__ Ld load(int64_t row, int cg, int C) const {
+    Ld l;
+    l.g = reinterpret_cast<const float4*>(dy + row * C)[cg];
+    l.w = reinterpret_cast<const int*>(q + row * C)[cg];
+    l.s = sc[row * ((C + 31) >> 5) + (cg >> 3)];
+    l.m = MASK ? (unsigned)mask[row * (((C + 15) >> 4) * 2) + (cg >> 1)] >> (4 * (cg & 1)) : 0xFu;
+    return l;
+  }
+  // g (masked) and xhat of the four columns
+  __device__ __forceinline__ void values(const Ld& l, const Cols& c, float4& g, float4& xh) const {
+    float u[4];
+    const float s = __uint_as_float(l.s << 23);
+    lt_mx8_get2<0>(l.w, s, u[0], u[1]);
+    lt_mx8_get2<1>(l.w, s, u[2], u[3]);
+    g = l.g;
+    if (MASK) {
+      g.x = l.m & 1 ? g.x : 0.f; g.y = l.m & 2 ? g.y : 0.f; g.z = l.m & 4 ? g.z : 0.f; g.w = l.m & 8 ? g.w : 0.f;
+    }
+    xh = make_float4((u[0] + c.off.x) * c.rs.x, (u[1] + c.off.y) * c.rs.y, (u[2] + c.off.z) * c.rs.z, (u[3] + c.off.w) * c.rs.w);
+  }
+  __device__ __forceinline__ void acc(const Ld& l, const Cols& c, float4& a, float4& b) const {
+    float4 g, xh;
+    values(l, c, g, xh);
+    a.x += g.x; a.y += g.y; a.z += g.z; a.w += g.w;
+    b.x += g.x * xh.x; b.y += g.y * xh.y; b.z += g.z * xh.z; b.w += g.w * xh.w;
+  }
+};
+
+// dx = gamma rstd (g - sum_g / V - xhat sum_gx / V), dres = g
+template <bool MASK>
+__global__ __launch_bounds__(256) void k_bn_bwd_apply_mx8(Bwd8Op<MASK> op, const float* __restrict__ gamma,
+                                                          const float* __restrict__ sum_g, const float* __restrict__ sum_gx,
+                                                          float* __restrict__ dx, float* __restrict__ dres, int64_t V, int C) {
+  const int cgn = C / 4, rpi = 256 / cgn;
+  const int cg = threadIdx.x % cgn, rr = threadIdx.x / cgn;
+  if (rr >= rpi) return;
+  const typename Bwd8Op<MASK>::Cols c = op.cols(cg);
+  const float iv = 1.0f / (float)V;
+  const float4 gm = reinterpret_cast<const float4*>(gamma)[cg], sg = reinterpret_cast<const float4*>(sum_g)[cg],
+               sx = reinterpret_cast<const float4*>(sum_gx)[cg];
+  const float4 k = make_float4(gm.x * c.rs.x, gm.y * c.rs.y, gm.z * c.rs.z, gm.w * c.rs.w);
+  auto put = [&](int64_t row, const typename Bwd8Op<MASK>::Ld& l) {
+    float4 g, xh;
+    op.values(l, c, g, xh);
+    if (dres) reinterpret_cast<float4*>(dres + row * C)[cg] = g;
+    if (dx)
+      reinterpret_cast<float4*>(dx + row * C)[cg] =
+          make_float4(k.x * (g.x - sg.x * iv - xh.x * (sx.x * iv)), k.y * (g.y - sg.y * iv - xh.y * (sx.y * iv)),
+                      k.z * (g.z - sg.z * iv - xh.z * (sx.z * iv)), k.w * (g.w - sg.w * iv - xh.w * (sx.w * iv)));
+  };
+  const int64_t step = (int64_t)gridDim.x * rpi;
+  int64_t row = (int64_t)blockIdx.x * rpi + rr;
+  for (; row + 3 * step < V; row += 4 * step) {
+    typename Bwd8Op<MASK>::Ld l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) l[i] = op.load(row + i * step, cg, C);
+    __builtin_amdgcn_sched_barrier(0);  // all loads of the four rows issue before the first use
+#pragma unroll
+    for (int i = 0; i < 4; ++i) put(row + i * step, l[i]);
+  }
+  for (; row < V; row += step) put(row, op.load(row, cg, C));
+}
+
+extern "C" int lt_bn_apply_mx8(const float* x, const float* mean, const float* var, const float* gamma, const float* beta, float eps,
+                               const float* residual, int32_t relu, float* y, void* values, void* scales, void* mask, int64_t V,
+                               int32_t C, hipStream_t stream) {
+  int rc = check_vc("lt_bn_apply_mx8", V, C);
+  if (rc) return rc;
+  LT_REQUIRE(x && mean && var && gamma && beta && y && values && scales, LT_ERR_ARG, "lt_bn_apply_mx8: null pointer");
+  LT_REQUIRE((relu == 0 || relu == 1 || (relu == 3 && residual)) && (!(relu & 1) == !mask), LT_ERR_ARG,
+             "lt_bn_apply_mx8: relu=%d not in {0,1,3} (3 needs a residual), a mask goes with the ReLU", relu);
+  const int rpi = 256 / ((C + 31) / 32 * 8);
+  const int64_t g = (V + rpi * 4 - 1) / (rpi * 4);
+  hipLaunchKernelGGL(k_bn_apply_mx8, dim3((unsigned)(g > 4096 ? 4096 : g)), dim3(256), 0, stream, x, mean, var, gamma, beta, eps,
+                     residual, relu, y, (uint8_t*)values, (uint8_t*)scales, (uint8_t*)mask, V, C);
+  LT_LAUNCH_CHECK();
+  return LT_OK;
+}
+
+extern "C" int lt_bn_bwd_reduce_mx8(const float* dy, const void* values, const void* scales, const void* mask, const float* mean,
+                                    const float* var, float eps, int64_t V, int32_t C, void* ws, int64_t ws_bytes, float* sum_g,
+                                    float* sum_gx, hipStream_t stream) {
+  int rc = check_vc("lt_bn_bwd_reduce_mx8", V, C);
+  if (rc) return rc;
+  LT_REQUIRE(dy && values && scales && mean && var && ws && sum_g && sum_gx, LT_ERR_ARG, "lt_bn_bwd_reduce_mx8: null pointer");
+  LT_REQUIRE(ws_bytes >= lt_bn_workspace_bytes(V, C), LT_ERR_WORKSPACE, "lt_bn_bwd_reduce_mx8: workspace too small");
+  const int nb = bn_blocks(V, C), cg = C / 4, rpi = BN_BLOCK / cg > 0 ? BN_BLOCK / cg : 1;
+  const size_t lds = (size_t)rpi * 2 * C * 4;
+  const uint8_t *q = (const uint8_t*)values, *s = (const uint8_t*)scales, *m = (const uint8_t*)mask;
+  if (m)
+    hipLaunchKernelGGL(k_col_partial<Bwd8Op<true>>, dim3(nb), dim3(BN_BLOCK), lds, stream, Bwd8Op<true>{dy, q, s, m, mean, var, eps}, V, C, (float*)ws);
+  else
+    hipLaunchKernelGGL(k_col_partial<Bwd8Op<false>>, dim3(nb), dim3(BN_BLOCK), lds, stream, Bwd8Op<false>{dy, q, s, m, mean, var, eps}, V, C, (float*)ws);
+  LT_LAUNCH_CHECK();
+  hipLaunchKernelGGL(k_sum_partials, dim3(C), dim3(64), 0, stream, (const float*)ws, nb, C, sum_g, sum_gx);
+  LT_LAUNCH_CHECK();
+  return LT_OK;
+}
+
+extern "C" int lt_bn_bwd_apply_mx8(const float* dy, const void* values, const void* scales, const void* mask, const float* mean,
+                                   const float* var, const float* gamma, float eps, const float* sum_g, const float* sum_gx, float* dx,
+                                   float* dres, int64_t V, int32_t C, hipStream_t stream) {
+  int rc = check_vc("lt_bn_bwd_apply_mx8", V, C);
+  if (rc) return rc;
+  LT_REQUIRE(dy && values && scales && mean && var && gamma && sum_g && sum_gx && (dx || dres), LT_ERR_ARG,
+             "lt_bn_bwd_apply_mx8: null pointer");
+  const uint8_t *q = (const uint8_t*)values, *s = (const uint8_t*)scales, *m = (const uint8_t*)mask;
+  const int rpi = 256 / (C / 4);
+  int64_t g = (V + rpi * 4 - 1) / (rpi * 4);
+  if (g > 4096) g = 4096;
+  if (m)
+    hipLaunchKernelGGL(k_bn_bwd_apply_mx8<true>, dim3((unsigned)g), dim3(256), 0, stream, Bwd8Op<true>{dy, q, s, m, mean, var, eps},
+                       gamma, sum_g, sum_gx, dx, dres, V, C);
+  else
+    hipLaunchKernelGGL(k_bn_bwd_apply_mx8<false>, dim3((unsigned)g), dim3(256), 0, stream, Bwd8Op<false>{dy, q, s, m, mean, var, eps},
+                       gamma, sum_g, sum_gx, dx, dres, V, C);
   LT_LAUNCH_CHECK();
   return LT_OK;
 }

@@ -1,6 +1,6 @@
 """Dense layers on the HIP kernels: linear with its epilogue and its backward, and activations kept in 8 bits ("mx8").
 
-Tensor-level calls and autograd nodes over the `lt_mx8_*` and `lt_linear_*` entry points of include/latte_hip.h; the public
+Tensor-level calls and autograd nodes over the `lt_mx8_*`, `lt_linear_*` and `lt_rms_norm_*` entry points of include/latte_hip.h; the public
 names are re-exported by latte_amd.functional, the modules are latte_amd.sparse_modules.Linear / RMSNorm.  Types: fp32,
 bfloat16, float16 (all operands of a call share one); sums are fp32.  GPU tensors only: there is no CPU fallback."""
 from __future__ import annotations
@@ -14,7 +14,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from .ops import _p, _ws_bytes
 
-__all__ = ["Mx8", "quantize_mx8", "linear"]
+__all__ = ["Mx8", "quantize_mx8", "linear", "rms_norm"]
 
 _DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACT = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
@@ -184,17 +184,52 @@ class _Linear(Function):
         return (dx.view(ctx.x_shape) if dx is not None else None), dw, db, (dy if need[3] else None), None, None
 
 
-def linear(x, weight, bias=None, act: str = "none", residual=None, checkpoint: str | None = None):
+def _linear_mx8(x: Mx8, weight: Mx8, bias, act: str, residual, dtype):
+    M, K = x.shape
+    N = weight.shape[0]
+    given = [t for t in (bias, residual) if t is not None]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
+        raise RuntimeError("linear: mx8 operands carry no gradient; call it under torch.no_grad()")
+    dtype = dtype or (given[0].dtype if given else torch.bfloat16)
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"linear: results of mx8 operands are bfloat16 or float16, not {dtype}")
+    if weight.shape[1] != K or min(M + 1, K, N) < 1:
+        raise ValueError(f"linear: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not go together")
+    if not x.values.is_cuda:
+        raise _lib.LatteHipError("linear: tensor must be on the GPU (no CPU fallback in the product path)")
+    if weight.device != x.device:
+        raise ValueError(f"linear weight: on {weight.device}, the other operands on {x.device}")
+    y = torch.empty((M, N), dtype=dtype, device=x.device)
+    if bias is not None:
+        bias = _like(bias, y, (N,), "linear bias").contiguous()
+    r2, ldr = (None, 0) if residual is None else _rows(_like(residual, y, (M, N), "linear residual"), N)
+    nb = _ws_bytes("lt_linear_mx8_workspace_bytes", M, K, N)
+    ws = _buf(nb, x.device) if nb > 0 else None
+    _lib.call("lt_linear_mx8_fwd", _p(x.values), _p(x.scales), _p(weight.values), _p(weight.scales), _p(bias), _p(r2), ldr, _ACT[act],
+              M, K, N, _DT[dtype], _p(y), _p(ws), nb, _stream_of(y))
+    return y
+
+
+def linear(x, weight, bias=None, act: str = "none", residual=None, checkpoint: str | None = None, dtype: torch.dtype | None = None):
     """act(x @ weight.T + bias) + residual as one kernel; act: "none" | "relu" | "gelu" (exact) | "silu".
 
     x [..., K], weight [N, K], bias [N], residual [..., N] -> [..., N], all of one type (float32, bfloat16, float16), sums in
     fp32.  Differentiable in all four; the backward pass reads x, weight and act'.  checkpoint="mx8" keeps what it reads of x
     in 8 bits (quantize_mx8: relative error at most 2^-4 an element) and act' of GELU / SiLU on a uniform 8-bit grid
-    (error at most 1/384); the ReLU's act' is one bit either way.  The output does not depend on `checkpoint`."""
+    (error at most 1/384); the ReLU's act' is one bit either way.  The output does not depend on `checkpoint`.
+
+    x and weight both Mx8 (serving, no gradient): the product of the held values on the 8-bit matrix instructions; bias,
+    residual and the result are bfloat16 or float16 (`dtype`; bias' or the residual's, else bfloat16)."""
     if act not in _ACT:
         raise ValueError(f"linear: act must be one of {sorted(_ACT)}, got {act!r}")
     if checkpoint not in (None, "mx8"):
         raise ValueError(f"linear: checkpoint must be None or 'mx8', got {checkpoint!r}")
+    if isinstance(x, Mx8) or isinstance(weight, Mx8):
+        if not (isinstance(x, Mx8) and isinstance(weight, Mx8)):
+            raise TypeError("linear: x and weight are both Mx8 or neither is (quantize_mx8, Mx8.dequantize)")
+        return _linear_mx8(x, weight, bias, act, residual, dtype)
+    if dtype is not None and dtype != x.dtype:
+        raise TypeError(f"linear: results have the operands' type {x.dtype}, not {dtype}")
     _dt(x, "linear x")
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or min(weight.shape) < 1:
         raise ValueError(f"linear: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not go together")
@@ -205,3 +240,87 @@ def linear(x, weight, bias=None, act: str = "none", residual=None, checkpoint: s
     if residual is not None:
         _like(residual, x, (*x.shape[:-1], N), "linear residual")
     return _Linear.apply(x, weight, bias, residual, act, checkpoint)
+
+
+# ------------------------------------------------------------------ rms_norm
+def _rms_fwd(x, w, residual, eps, want_h, want_y, want_y8, want_h8, want_rstd):
+    """-> (h, y, y8, h8, rstd), None where not asked for"""
+    C = x.shape[-1]
+    x2, ldx = _rows(x, C)
+    M, dev = x2.shape[0], x.device
+    r2, ldr = (None, 0) if residual is None else _rows(residual, C)
+    h = torch.empty((M, C), dtype=x.dtype, device=dev) if want_h else None
+    y = torch.empty((M, C), dtype=x.dtype, device=dev) if want_y else None
+    y8 = Mx8.empty(M, C, dev) if want_y8 else None
+    h8 = Mx8.empty(M, C, dev) if want_h8 else None
+    rstd = torch.empty((M,), dtype=torch.float32, device=dev) if want_rstd else None
+    p8 = lambda q: (None, None) if q is None else (_p(q.values), _p(q.scales))  # noqa: E731
+    _lib.call("lt_rms_norm_fwd", _p(x2), ldx, _p(r2), ldr, _p(w), float(eps), M, C, _DT[x.dtype], _p(h), _p(y), *p8(y8), *p8(h8),
+              _p(rstd), _stream_of(x2))
+    return h, y, y8, h8, rstd
+
+
+class _RmsNorm(Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps, checkpoint):
+        C = x.shape[-1]
+        w = weight.contiguous()
+        need = any(ctx.needs_input_grad)
+        ck = need and checkpoint == "mx8"
+        h, y, _, h8, rstd = _rms_fwd(x, w, residual, eps, residual is not None, True, False, ck, need)
+        if need:
+            if ck:
+                ctx.save_for_backward(None, h8.values, h8.scales, w, rstd)
+            else:   # without a residual h is x itself
+                ctx.save_for_backward(h if residual is not None else _rows(x, C)[0], None, None, w, rstd)
+        ctx.set_materialize_grads(False)   # a sum that nothing reads costs no zeros
+        ctx.x_shape = x.shape
+        y = y.view(x.shape)
+        return y if residual is None else (y, h.view(x.shape))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, q, sc, w, rstd = ctx.saved_tensors
+        C, M = w.shape[0], rstd.shape[0]
+        need = ctx.needs_input_grad
+        if dy is None and dh is None:
+            return None, None, None, None, None
+        if dy is None:   # only the sum was used: its gradient passes through
+            return (dh if need[0] else None), (torch.zeros_like(w) if need[1] else None), (dh if need[2] else None), None, None
+        dy2, lddy = _rows(dy, C)
+        dh2, lddh = (None, 0) if dh is None else _rows(dh, C)
+        dx = torch.empty((M, C), dtype=w.dtype, device=w.device) if (need[0] or need[2]) else None
+        dw = torch.empty((C,), dtype=w.dtype, device=w.device) if need[1] else None
+        nb = _ws_bytes("lt_rms_norm_bwd_workspace_bytes", M, C) if dw is not None else 0
+        ws = _buf(nb, w.device) if dw is not None else None
+        ldh = 0 if h is None else _rows(h, C)[1]
+        _lib.call("lt_rms_norm_bwd", _p(dy2), lddy, _p(dh2), lddh, _p(h), ldh, _p(q), _p(sc), _p(w), _p(rstd), M, C, _DT[w.dtype],
+                  _p(dx), _p(dw), _p(ws), 0 if ws is None else ws.numel(), _stream_of(dy2))
+        dx = dx.view(ctx.x_shape) if dx is not None else None
+        return (dx if need[0] else None), dw, (dx if need[2] else None), None, None
+
+
+def rms_norm(x, weight, residual=None, eps: float = 1e-6, checkpoint: str | None = None, out: str | None = None):
+    """h = x + residual (h = x without one);  y = h / sqrt(mean over the row of h^2 + eps) * weight.  -> y, or (y, h) with a
+    residual.
+
+    x [..., C], residual the same shape, weight [C], all float32, bfloat16 or float16, C <= 16384; the sum of squares and the
+    row's scale are fp32, h enters the norm unrounded.  Differentiable in all three; checkpoint="mx8": the backward pass
+    reads h from 8 bits.  out="mx8" (serving, no gradient): y comes as Mx8 [rows, C], for linear() with an Mx8 weight."""
+    if checkpoint not in (None, "mx8"):
+        raise ValueError(f"rms_norm: checkpoint must be None or 'mx8', got {checkpoint!r}")
+    if out not in (None, "mx8"):
+        raise ValueError(f"rms_norm: out must be None or 'mx8', got {out!r}")
+    _dt(x, "rms_norm x")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 16384:
+        raise ValueError(f"rms_norm: expected rows of 1 to 16384 elements, got shape {tuple(x.shape)}")
+    _like(weight, x, (x.shape[-1],), "rms_norm weight")
+    if residual is not None:
+        _like(residual, x, x.shape, "rms_norm residual")
+    if out == "mx8":
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+            raise RuntimeError("rms_norm: out='mx8' carries no gradient; call it under torch.no_grad()")
+        h, _, y8, _, _ = _rms_fwd(x, weight.contiguous(), residual, eps, residual is not None, False, True, False, False)
+        return y8 if residual is None else (y8, h.view(x.shape))
+    return _RmsNorm.apply(x, weight, residual, float(eps), checkpoint)

@@ -10,10 +10,10 @@ import torch
 from torch.autograd import Function
 
 from . import ops
-from .dense import Mx8, linear, quantize_mx8
+from .dense import Mx8, linear, quantize_mx8, rms_norm
 
 __all__ = ["KernelMap", "get_kernel_offsets", "sparse_conv", "conv_bn", "batch_norm", "spvoxelize", "spdevoxelize",
-           "invalidate_packed", "bump_pack_epoch", "Mx8", "quantize_mx8", "linear"]
+           "invalidate_packed", "bump_pack_epoch", "Mx8", "quantize_mx8", "linear", "rms_norm"]
 
 _OFFSET_CACHE: dict = {}
 
@@ -212,7 +212,8 @@ class _SparseConv(Function):
         else:
             out = _run_conv(feats, _packed(weight, 0, wcache), kmap, transposed, cout)
         ctx.kmap, ctx.transposed = kmap, transposed
-        ctx.save_for_backward(feats, weight)
+        # the input is read for the kernel's gradient only
+        ctx.save_for_backward(feats if ctx.needs_input_grad[1] else None, weight)
         return out
 
     @staticmethod
@@ -309,7 +310,7 @@ class _BatchNorm(Function):
     a residual): y = relu(bn(x)) + residual, the sum after the activation (the point branch of SPVCNN)."""
 
     @staticmethod
-    def forward(ctx, x, gamma, beta, residual, eps, relu, stats_out, post_add=False):
+    def forward(ctx, x, gamma, beta, residual, eps, relu, stats_out, post_add=False, checkpoint=None):
         if x.shape[0] > 0:
             mean, var = ops.bn_stats(x)
         else:   # cross-rank statistics only (batch_norm refuses otherwise): this rank has no row at this level
@@ -319,12 +320,21 @@ class _BatchNorm(Function):
             mean, var, n_total = sync_batch_stats(mean, var, x.shape[0], SYNC_BN_GROUP)
             ctx.sync = (SYNC_BN_GROUP, n_total, x.shape[0])
         post_add = bool(post_add and relu and residual is not None)
-        if x.shape[0] > 0:
-            y = ops.bn_apply(x, mean, var, gamma, beta, eps, residual=residual, relu=relu, post_add=post_add)
-        else:
+        held = None
+        if x.shape[0] == 0:
             y = torch.empty_like(x)
+        elif checkpoint == "mx8" and any(ctx.needs_input_grad):
+            y, *held = ops.bn_apply_mx8(x, mean, var, gamma, beta, eps, residual=residual, relu=relu, post_add=post_add)
+        else:
+            y = ops.bn_apply(x, mean, var, gamma, beta, eps, residual=residual, relu=relu, post_add=post_add)
         ctx.eps, ctx.relu, ctx.post_add = eps, relu, post_add
         ctx.has_res = residual is not None
+        ctx.held = held is not None
+        if ctx.held:
+            ctx.save_for_backward(*held, mean, var, gamma)
+            if stats_out is not None:
+                stats_out.append((mean, var))
+            return y
         # ReLU mask in the backward: from y when a residual was added before the ReLU, otherwise rebuilt from x (y is not
         # read again; with post_add y is not the activation's output, so it cannot serve as the mask)
         ctx.save_for_backward(x, y if (relu and residual is not None and not post_add) else None, mean, var, gamma, beta)
@@ -334,6 +344,8 @@ class _BatchNorm(Function):
 
     @staticmethod
     def backward(ctx, dy):
+        if ctx.held:
+            return _BatchNorm._backward_held(ctx, dy.contiguous())
         x, y, mean, var, gamma, beta = ctx.saved_tensors
         dy = dy.contiguous()
         need_dx = ctx.needs_input_grad[0]
@@ -347,20 +359,40 @@ class _BatchNorm(Function):
                 C = x.shape[1]
                 e = torch.empty_like(x)
                 return (e if need_dx else None), both[C:].contiguous(), both[:C].contiguous(), (e if need_dres else None), \
-                    None, None, None, None
-
-            def sync(sum_g, sum_gx):
-                both = _allreduce_small(torch.cat([sum_g, sum_gx]), group)
-                C = sum_g.numel()
-                return both[:C].contiguous(), both[C:].contiguous(), (rows / n_total).float()
+                    None, None, None, None, None
+            sync = _BatchNorm._sync_of(ctx)
         if ctx.post_add:
             # the residual bypasses the ReLU: its gradient is dy itself
             dx, dgamma, dbeta, _ = ops.bn_bwd(dy, x, None, mean, var, gamma, ctx.eps, True, need_dx=need_dx,
                                               need_dres=False, beta=beta, sync=sync)
-            return dx, dgamma, dbeta, (dy if need_dres else None), None, None, None, None
+            return dx, dgamma, dbeta, (dy if need_dres else None), None, None, None, None, None
         dx, dgamma, dbeta, dres = ops.bn_bwd(dy, x, y, mean, var, gamma, ctx.eps, ctx.relu, need_dx=need_dx,
                                              need_dres=need_dres, beta=beta, sync=sync)
-        return dx, dgamma, dbeta, dres, None, None, None, None
+        return dx, dgamma, dbeta, dres, None, None, None, None, None
+
+    @staticmethod
+    def _sync_of(ctx):
+        """the cross-rank sum of the backward's column sums (ops.bn_bwd's `sync`), or None"""
+        if ctx.sync is None:
+            return None
+        group, n_total, rows = ctx.sync
+
+        def sync(sum_g, sum_gx):
+            both = _allreduce_small(torch.cat([sum_g, sum_gx]), group)
+            C = sum_g.numel()
+            return both[:C].contiguous(), both[C:].contiguous(), (rows / n_total).float()
+        return sync
+
+    @staticmethod
+    def _backward_held(ctx, dy):
+        """the same gradients from the 8-bit form of x and the ReLU's bits (lt_bn_apply_mx8)"""
+        q, sc, mask, mean, var, gamma = ctx.saved_tensors
+        need_dres = ctx.has_res and ctx.needs_input_grad[3]
+        dx, dgamma, dbeta, dres = ops.bn_bwd_mx8(dy, q, sc, mask, mean, var, gamma, ctx.eps, need_dx=ctx.needs_input_grad[0],
+                                                 need_dres=need_dres and not ctx.post_add, sync=_BatchNorm._sync_of(ctx))
+        if ctx.post_add and need_dres:
+            dres = dy   # the residual bypasses the ReLU
+        return dx, dgamma, dbeta, dres, None, None, None, None, None
 
 
 _DIAG_NO_APPLY = False   # diagnostics (spvcnn._DIAG_SKIP_FIRST_APPLY): composites skip the BatchNorm apply pass, WRONG results
@@ -428,12 +460,18 @@ def conv_bn(feats, weight, gamma, beta, kmap: KernelMap, transposed=False, resid
                          float(eps), wcache)
 
 
-def batch_norm(x, gamma, beta, eps=1e-5, residual=None, relu=False, stats_out=None, post_add=False):
+def batch_norm(x, gamma, beta, eps=1e-5, residual=None, relu=False, stats_out=None, post_add=False, checkpoint=None):
+    """relu?(bn(x) + residual) with batch statistics; post_add: relu(bn(x)) + residual.  checkpoint="mx8": what the backward
+    pass reads of x is held in 8 bits and the ReLU's mask in one (lt_bn_apply_mx8), 1.16 bytes an element instead of 4 (8
+    with a residual); the output stays the same bits, gradients are those of the held values (relative error at most 2^-4
+    an element of x - its channel's mean, give or take an eighth of the channel's standard deviation)."""
+    if checkpoint not in (None, "mx8"):
+        raise ValueError(f"batch_norm: checkpoint must be None or 'mx8', got {checkpoint!r}")
     if x.shape[0] <= 1 and SYNC_BN_GROUP is None:
         # same refusal as torch.nn.functional.batch_norm in training mode; with cross-rank statistics the LOCAL row count
         # says nothing (and every rank must reach the collective), so the call goes through
         raise ValueError(f"Expected more than 1 value per channel when training, got input size {tuple(x.shape)}")
-    return _BatchNorm.apply(x, gamma, beta, residual, float(eps), bool(relu), stats_out, bool(post_add))
+    return _BatchNorm.apply(x, gamma, beta, residual, float(eps), bool(relu), stats_out, bool(post_add), checkpoint)
 
 
 class _GatherRows(Function):

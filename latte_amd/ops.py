@@ -416,6 +416,44 @@ def bn_bwd(dy, x, y, mean, var, gamma, eps: float, relu: bool, need_dx=True, nee
     return dx, sum_gx, sum_g, dres
 
 
+def bn_apply_mx8(x, mean, var, gamma, beta, eps: float, residual=None, relu: bool = False, post_add: bool = False):
+    """bn_apply that also leaves what the backward pass reads in 8 bits -> (y, values, scales, mask | None); see lt_bn_apply_mx8."""
+    x = _chk(x, torch.float32, "bn_apply_mx8 x")
+    V, C = x.shape
+    y = torch.empty_like(x)
+    q = torch.empty((V, C), dtype=torch.float8_e4m3fn, device=x.device)
+    sc = torch.empty((V, (C + 31) // 32), dtype=torch.uint8, device=x.device)
+    mask = torch.empty((V, (C + 15) // 16), dtype=torch.int16, device=x.device) if relu else None
+    if residual is not None:
+        residual = _chk(residual, torch.float32, "bn_apply_mx8 residual")
+        assert residual.shape == x.shape
+    _lib.call("lt_bn_apply_mx8", _p(x), _p(mean), _p(var), _p(_chk(gamma.detach(), torch.float32, "gamma")),
+              _p(_chk(beta.detach(), torch.float32, "beta")), float(eps), _p(residual),
+              3 if (post_add and relu and residual is not None) else int(bool(relu)), _p(y), _p(q), _p(sc), _p(mask), V, C, _stream())
+    return y, q, sc, mask
+
+
+def bn_bwd_mx8(dy, q, sc, mask, mean, var, gamma, eps: float, need_dx=True, need_dres=False, sync=None):
+    """bn_bwd from what bn_apply_mx8 left -> (dx | None, dgamma, dbeta, dres | None); sync as in bn_bwd."""
+    dy = _chk(dy, torch.float32, "bn_bwd_mx8 dy")
+    V, C = dy.shape
+    ws = _scratch(_ws_bytes("lt_bn_workspace_bytes", V, C), dy.device)
+    sums = torch.empty((2, C), dtype=torch.float32, device=dy.device)
+    sum_g, sum_gx = sums[0], sums[1]
+    _lib.call("lt_bn_bwd_reduce_mx8", _p(dy), _p(q), _p(sc), _p(mask), _p(mean), _p(var), float(eps), V, C, _p(ws), ws.numel(),
+              _p(sum_g), _p(sum_gx), _stream())
+    dx = torch.empty_like(dy) if need_dx else None
+    dres = torch.empty_like(dy) if need_dres else None
+    ag, agx = sum_g, sum_gx
+    if sync is not None:
+        sum_g, sum_gx, scale = sync(sum_g, sum_gx)
+        ag, agx = (sum_g * scale).contiguous(), (sum_gx * scale).contiguous()
+    if need_dx or need_dres:
+        _lib.call("lt_bn_bwd_apply_mx8", _p(dy), _p(q), _p(sc), _p(mask), _p(mean), _p(var),
+                  _p(_chk(gamma.detach(), torch.float32, "gamma")), float(eps), _p(ag), _p(agx), _p(dx), _p(dres), V, C, _stream())
+    return dx, sum_gx, sum_g, dres
+
+
 # ------------------------------------------------------------------ point <-> voxel
 def voxelize_fwd(feats, idx, counts):
     feats = _chk(feats, torch.float32, "voxelize feats")

@@ -14,7 +14,7 @@ from . import functional as LF
 from . import ops
 from .tensor import SparseTensor
 
-__all__ = ["Conv3d", "BatchNorm", "ReLU", "conv3d", "conv3d_bn", "build_kernel_map"]
+__all__ = ["Conv3d", "BatchNorm", "ReLU", "Linear", "RMSNorm", "conv3d", "conv3d_bn", "build_kernel_map", "set_activation_checkpoint"]
 
 
 def _n3(v):
@@ -176,7 +176,10 @@ def _wrap(input: SparseTensor, feats) -> SparseTensor:
 
 class BatchNorm(nn.BatchNorm1d):
     """BatchNorm1d over SparseTensor.F.  Batch statistics (training mode or track_running_stats=False, which is what
-    configure_model_norm forces: latte/common/utils/ema_util.py:26-29) run in the HIP kernels."""
+    configure_model_norm forces: latte/common/utils/ema_util.py:26-29) run in the HIP kernels.  `checkpoint` = "mx8": the
+    backward pass reads its input from 8 bits (set_activation_checkpoint, functional.batch_norm)."""
+
+    checkpoint = None
 
     def bn_feats(self, feats, residual=None, relu=False, post_add=False):
         """relu?(bn(feats) + residual); post_add: relu(bn(feats)) + residual (the sum after the activation)."""
@@ -184,7 +187,7 @@ class BatchNorm(nn.BatchNorm1d):
         if use_batch:
             stats = [] if (self.training and self.track_running_stats and self.running_mean is not None) else None
             y = LF.batch_norm(feats, self.weight, self.bias, self.eps, residual=residual, relu=relu, stats_out=stats,
-                              post_add=post_add)
+                              post_add=post_add, checkpoint=self.checkpoint)
             if stats:
                 mean, var = stats[0]
                 n = feats.shape[0]
@@ -217,3 +220,49 @@ class ReLU(nn.ReLU):
         if isinstance(input, SparseTensor):
             return _wrap(input, super().forward(input.feats))
         return super().forward(input)
+
+
+class Linear(nn.Linear):
+    """nn.Linear (same parameters, same state_dict keys) with its activation, a residual and 8-bit checkpoints in one kernel:
+    functional.linear.  Takes and returns plain tensors or SparseTensors."""
+
+    def __init__(self, in_features, out_features, bias=True, act="none", checkpoint=None, **kwargs):
+        super().__init__(in_features, out_features, bias=bias, **kwargs)
+        self.act, self.checkpoint = act, checkpoint
+
+    def extra_repr(self):
+        return super().extra_repr() + f", act={self.act!r}, checkpoint={self.checkpoint!r}"
+
+    def forward(self, input, residual=None):
+        if isinstance(input, SparseTensor):
+            return _wrap(input, self.forward(input.feats, residual.feats if isinstance(residual, SparseTensor) else residual))
+        return LF.linear(input, self.weight, self.bias, act=self.act, residual=residual, checkpoint=self.checkpoint)
+
+
+class RMSNorm(nn.Module):
+    """functional.rms_norm with a learned weight: y, or (y, x + residual) with a residual.  Plain tensors or SparseTensors."""
+
+    def __init__(self, channels, eps=1e-6, checkpoint=None, device=None, dtype=None):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(channels, device=device, dtype=dtype))
+        self.eps, self.checkpoint = eps, checkpoint
+
+    def extra_repr(self):
+        return f"{self.weight.numel()}, eps={self.eps}, checkpoint={self.checkpoint!r}"
+
+    def forward(self, input, residual=None):
+        if isinstance(input, SparseTensor):
+            out = self.forward(input.feats, residual.feats if isinstance(residual, SparseTensor) else residual)
+            return _wrap(input, out) if residual is None else (_wrap(input, out[0]), _wrap(input, out[1]))
+        return LF.rms_norm(input, self.weight, residual=residual, eps=self.eps, checkpoint=self.checkpoint)
+
+
+def set_activation_checkpoint(model: nn.Module, mode: str | None) -> nn.Module:
+    """Every BatchNorm, Linear and RMSNorm of `model` keeps what its backward pass reads of its input in 8 bits ("mx8"), or in
+    full (None).  A SPVCNN with checkpoints walks its module tree (the one-call pass keeps its buffers in full)."""
+    if mode not in (None, "mx8"):
+        raise ValueError(f"set_activation_checkpoint: mode must be None or 'mx8', got {mode!r}")
+    for m in model.modules():
+        if isinstance(m, (BatchNorm, Linear, RMSNorm)):
+            m.checkpoint = mode
+    return model

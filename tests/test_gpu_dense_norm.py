@@ -1,0 +1,351 @@
+"""rms_norm, BatchNorm's 8-bit checkpoints and the product of two mx8 matrices against 64-bit formulas (tests/dense_ref.py).
+Tolerances as in test_gpu_dense.py: u = 2^-24 per fp32 addition of a sum, h = half a step per rounding to a type."""
+import pytest
+import torch
+
+from tests import dense_ref as R
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _close(got, want, tol, what):
+    err = (got.double() - want).abs()
+    bad = ~(err <= tol)
+    assert not bool(bad.any()), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((err - tol).max()):.3e} over its bound"
+
+
+def _rn(seed, dt, *shapes):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return [torch.randn(*s, generator=g, device="cuda").to(dt) for s in shapes]
+
+
+# ------------------------------------------------------------------ rms_norm
+def _check_rms(x, w, r, dy, dh, ckpt, eps=1e-6):
+    from latte_amd import functional as LF
+    dt = x.dtype
+    h_, lo = R.EPS[dt], R.LOW[dt]
+    M, C = x.shape
+    t = [v.detach().clone().requires_grad_(True) if v is not None else None for v in (x, w, r)]
+    out = LF.rms_norm(t[0], t[1], residual=t[2], eps=eps, checkpoint=ckpt)
+    y, hs = out if r is not None else (out, None)
+    live = [v for v in t if v is not None]
+    if r is not None and dh is not None:
+        grads = torch.autograd.grad((y, hs), live, (dy, dh))
+    else:
+        grads = torch.autograd.grad(y, live, dy)
+    gx, gw = grads[0], grads[1]
+    h32 = x.float() + r.float() if r is not None else x.float()       # one fp32 addition: the same bits everywhere
+    H, W = h32.double(), w.double()
+    rstd = 1 / torch.sqrt(H.square().mean(1, keepdim=True) + eps)
+    rel = (C / 2 + 8) * U                                              # of the row's scale and of n
+    Y = H * rstd * W
+    _close(y, Y, rel * Y.abs() + h_ * Y.abs() * (1 + rel) + lo, "y")
+    if r is not None:
+        assert torch.equal(hs, h32.to(dt))
+    if ckpt:
+        N, nerr = R.mx8(h32)[0] * rstd, rel
+    else:
+        N, nerr = H * rstd, rel + h_ + 0.0                             # h was stored in its type
+    low = 0.0 if ckpt else lo
+    NA = N.abs() + low * rstd
+    G = dy.double() * W
+    dot = (G * N).mean(1, keepdim=True)
+    doterr = ((C + 2) * U + nerr) * (G.abs() * NA).mean(1, keepdim=True) + low * (G.abs() * rstd).mean(1, keepdim=True)
+    dX = rstd * (G - N * dot)
+    t_ = rstd * (4 * U * (G.abs() + NA * dot.abs()) + NA * doterr + nerr * NA * dot.abs() + low * rstd * dot.abs()) + rel * dX.abs()
+    if dh is not None and r is not None:
+        dX, t_ = dX + dh.double(), t_ + 2 * U * dh.double().abs()
+    _close(gx, dX, t_ + h_ * (dX.abs() + t_) + lo, "dx")
+    dW = (dy.double() * N).sum(0)
+    mag = (dy.double().abs() * NA).sum(0)
+    t_ = (M * U + nerr + 2 * U) * mag + low * (dy.double().abs() * rstd).sum(0)
+    _close(gw, dW, t_ + h_ * (dW.abs() + t_) + lo, "dw")
+    if r is not None:
+        assert torch.equal(grads[2], gx)
+
+
+RMS_SIZES = [(1, 1), (1, 7), (3, 32), (5, 33), (64, 64), (130, 96), (77, 129), (40, 256), (33, 257), (9, 512), (21, 513), (10, 1000),
+             (6, 2048), (5, 2049), (4, 4096), (3, 5001), (2, 16384), (5000, 96), (20011, 33)]
+
+
+@pytest.mark.parametrize("ckpt", [None, "mx8"])
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("size", RMS_SIZES, ids=str)
+def test_rms_norm_sizes(size, dt, ckpt):
+    M, C = size
+    x, w, r, dy, dh = _rn(1, dt, (M, C), (C,), (M, C), (M, C), (M, C))
+    _check_rms(x, w, r, dy, dh, ckpt)
+    _check_rms(x * 3, w, None, dy, None, ckpt)
+    _check_rms(x, w, r, dy, None, ckpt)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_rms_norm_mx8_output(dt):
+    """the held y is y rounded to mx8; y in 32 bits here is within the row scale's error, so each held value is one of the two
+    neighbours that a y within that error can round to, and reads back within 2^-4 of it"""
+    from latte_amd import functional as LF
+    for M, C in ((1, 40), (50, 96), (300, 1000), (70, 4096)):
+        x, w, r = _rn(2, dt, (M, C), (C,), (M, C))
+        with torch.no_grad():
+            q, hs = LF.rms_norm(x, w, residual=r, out="mx8")
+            alone = LF.rms_norm(x, w, out="mx8")
+        h32 = x.float() + r.float()
+        for got, H in ((q, h32.double()), (alone, x.double())):
+            Y = H / torch.sqrt(H.square().mean(1, keepdim=True) + 1e-6) * w.double()
+            scale = torch.ldexp(torch.ones_like(got.scales, dtype=torch.float64), got.scales.int() - 127).repeat_interleave(32, 1)[:, :C]
+            bound = Y.abs() * 2.0 ** -4 + scale * 2.0 ** -10
+            _close(got.dequantize(), Y, bound * (1 + (C + 20) * U), "y8")
+            # the scale is the smallest that fits: the block's largest value lies in (224, 448] of it, give or take rounding
+            pad = torch.nn.functional.pad(Y.abs() / scale, (0, (-C) % 32)).view(M, -1, 32).amax(2)
+            assert float(pad.max()) <= 448 * 1.001 and float(pad.min()) >= 224 * 0.999
+        assert torch.equal(hs, h32.to(dt))
+
+
+def test_rms_norm_layouts_and_unused_outputs():
+    from latte_amd import functional as LF
+    for dt in TYPES:
+        big, w = _rn(3, dt, (60, 301), (70,))
+        want = LF.rms_norm(big[:, 5:75].contiguous(), w)
+        assert torch.equal(LF.rms_norm(big[:, 5:75], w), want)
+        x3 = big[:, 5:75].reshape(6, 10, 70)
+        assert torch.equal(LF.rms_norm(x3, w), want.view(6, 10, 70))
+        y, h = LF.rms_norm(big[:, 5:75], w, residual=big[:1, 100:170].expand(60, 70))
+        assert torch.equal(h, (big[:, 5:75].float() + big[:1, 100:170].float()).to(dt))
+        assert torch.equal(LF.rms_norm(big[0, 5:75], w), want[0])
+        e = torch.zeros(0, 70, dtype=dt, device="cuda", requires_grad=True)
+        w2 = w.clone().requires_grad_(True)
+        gx, gw = torch.autograd.grad(LF.rms_norm(e, w2), (e, w2), torch.zeros_like(e))
+        assert gx.shape == (0, 70) and float(gw.abs().sum()) == 0
+        x, r = big[:, :70].clone().requires_grad_(True), big[:, 70:140].clone().requires_grad_(True)
+        y, h = LF.rms_norm(x, w2, residual=r)
+        gx, gr = torch.autograd.grad(h, (x, r), torch.ones_like(h))     # only the sum is used
+        assert torch.equal(gx, torch.ones_like(gx)) and torch.equal(gr, gx)
+        zero = torch.zeros(4, 70, dtype=dt, device="cuda")
+        assert float(LF.rms_norm(zero, w).abs().max()) == 0             # a row of zeros stays one
+
+
+def test_rms_norm_gradients_by_differences():
+    from latte_amd import functional as LF
+    x, w, r, dy, dh = _rn(4, torch.float32, (23, 77), (77,), (23, 77), (23, 77), (23, 77))
+    t = [v.clone().requires_grad_(True) for v in (x, w, r)]
+    grads = torch.autograd.grad(LF.rms_norm(t[0], t[1], residual=t[2]), t, (dy, dh))
+    dirs = [d.double() for d in _rn(5, torch.float32, (23, 77), (77,), (23, 77))]
+
+    def f(e):
+        X, W, Rr = (v.double() + e * d for v, d in zip((x, w, r), dirs))
+        H = X + Rr
+        Y = H / torch.sqrt(H.square().mean(1, keepdim=True) + 1e-6) * W
+        return float((Y * dy.double()).sum() + (H * dh.double()).sum())
+    num = (f(1e-5) - f(-1e-5)) / 2e-5
+    ana = sum(float((g.double() * d).sum()) for g, d in zip(grads, dirs))
+    assert abs(num - ana) < 1e-5 * sum(float((g.double() * d).abs().sum()) for g, d in zip(grads, dirs))
+
+
+# ------------------------------------------------------------------ batch_norm, 8-bit checkpoint
+def _held_bn(x, mean, var, eps):
+    """c and what x - c reads back as, from the fp32 statistics"""
+    ex = torch.frexp(torch.sqrt(var + eps))[1].to(torch.int32)
+    unit = ((ex - 3 + 127) << 23).view(torch.float32)
+    c = torch.round(mean / unit) * unit
+    return c, R.mx8(x - c)[0]
+
+
+@pytest.mark.parametrize("mode", ["plain", "relu", "res", "res_relu", "post"])
+@pytest.mark.parametrize("size", [(2, 4), (5, 16), (100, 20), (333, 32), (1000, 96), (4097, 256), (70, 1024), (30001, 64)], ids=str)
+def test_bn_checkpoint(size, mode):
+    from latte_amd import functional as LF
+    from latte_amd import ops
+    V, C = size
+    eps = 1e-5
+    x, gamma, beta, r, dy = _rn(6, torch.float32, (V, C), (C,), (C,), (V, C), (V, C))
+    x = x * torch.linspace(0.1, 30.0, C, device="cuda") + torch.linspace(-40.0, 40.0, C, device="cuda")
+    kw = dict(residual=r if "res" in mode or mode == "post" else None, relu=mode in ("relu", "res_relu", "post"), post_add=mode == "post")
+    def run(ck):
+        t = [v.clone().requires_grad_(True) for v in (x, gamma, beta)] + ([r.clone().requires_grad_(True)] if kw["residual"] is not None else [])
+        k = dict(kw, residual=t[3] if len(t) == 4 else None)
+        y = LF.batch_norm(t[0], t[1], t[2], eps, checkpoint=ck, **k)
+        return y, torch.autograd.grad(y, t, dy)
+    y0, g0 = run(None)
+    y1, g1 = run("mx8")
+    assert torch.equal(y0, y1)
+    mean, var = ops.bn_stats(x)
+    c, held = _held_bn(x, mean, var, eps)
+    q = ops.bn_apply_mx8(x, mean, var, gamma, beta, eps, **kw)
+    got = LF.Mx8(q[1], q[2]).dequantize().double()
+    assert torch.equal(got, held)
+    # 64-bit formula over the held values; the mask is the forward's own
+    rstd = 1 / torch.sqrt(var.double() + eps)
+    XH = (held + (c.double() - mean.double())) * rstd
+    on = torch.ones_like(y0, dtype=torch.bool)
+    if kw["relu"]:
+        on = (y0 > 0) if mode != "post" else (ops.bn_apply(x, mean, var, gamma, beta, eps, relu=True) > 0)
+    G = dy.double() * on
+    SG, SX = G.sum(0), (G * XH).sum(0)
+    xa = (held.abs() + (c.double() - mean.double()).abs() + 2 * U * mean.double().abs()) * rstd
+    tg, tx = (V + 4) * U * G.abs().sum(0), (V + 8) * U * (G.abs() * xa).sum(0)
+    _close(g1[2], SG, tg + U * SG.abs(), "dbeta")
+    _close(g1[1], SX, tx + U * SX.abs(), "dgamma")
+    K = gamma.double() * rstd
+    dX = K * (G - SG / V - XH * SX / V)
+    t = K.abs() * (tg / V + xa * tx / V + 8 * U * (G.abs() + SG.abs() / V + xa * SX.abs() / V))
+    _close(g1[0], dX, t + 4 * U * dX.abs(), "dx")
+    if kw["residual"] is not None:
+        assert torch.equal(g1[3].double(), dy.double() if mode == "post" else G)
+
+
+def test_bn_checkpoint_statistics_corner_cases():
+    """a constant channel, a channel far from zero, a NaN that stays in its channel"""
+    from latte_amd import functional as LF
+    x, gamma, beta, dy = _rn(7, torch.float32, (500, 36), (36,), (36,), (500, 36))
+    x[:, 3] = 7.0
+    x[:, 5] += 4096.0
+    for bad in (False, True):
+        if bad:
+            x[17, 9] = float("nan")
+        t = [v.clone().requires_grad_(True) for v in (x, gamma, beta)]
+        g8 = torch.autograd.grad(LF.batch_norm(*t, checkpoint="mx8"), t, dy)
+        g = torch.autograd.grad(LF.batch_norm(*t), t, dy)
+        cols = [c for c in range(36) if not (bad and c == 9)]
+        assert bool(torch.isfinite(g8[0][:, cols]).all()) and bool(torch.isfinite(g8[1][cols]).all())
+        # x - c is within sd / 8 + |x - mean|; its held form is 2^-4 of that off: so is xhat, whatever the channel's offset
+        xm = (x.double() - x.double().mean(0)).abs()
+        sd = torch.sqrt(x.double().var(0, unbiased=False) + 1e-5)
+        off = ((xm + sd / 8) / sd * 2.0 ** -4 + 2.0 ** -10 + 4096 * U / sd)
+        lim = (dy.double().abs() * off).sum(0) + 500 * U * (dy.double().abs() * xm / sd).sum(0)
+        err = (g8[1].double() - g[1].double()).abs()
+        assert bool((err <= lim * 1.01 + 1e-6)[[c for c in cols if c != 3]].all())
+
+
+def test_spvcnn_with_checkpoints_runs_and_keeps_its_forward():
+    """the backbone with every BatchNorm checkpointed: the module path's forward, gradients for every norm parameter, and the
+    last layer's dbeta, which no held value enters"""
+    from latte_amd import sparse_modules as spnn
+    from latte_amd import netprog, synth
+    from latte_amd.spvcnn import Net3DSeg
+    from latte_amd.tta_step import configure_model_norm
+    from latte_amd.workload import build_batch
+    w = synth.workload("tiny")
+    torch.manual_seed(3)
+    net, _ = configure_model_norm(Net3DSeg(w["C"], True, "SPVCNN", {"cr": 0.5}).cuda(), reset_dropout=True)
+    batch = build_batch(w, device="cuda:0")
+    params = [p for p in net.parameters() if p.requires_grad]
+    last = net.net_3d.point_transforms[2][1].bias
+    was, out = netprog.ENABLED, []
+    try:
+        netprog.ENABLED = False
+        for mode in (None, "mx8"):
+            spnn.set_activation_checkpoint(net, mode)
+            y = net(batch)["seg_logit"]
+            out.append((y.detach(), torch.autograd.grad(y.square().mean(), params), ))
+        netprog.ENABLED = True      # the switch alone must lead to the module path
+        y2 = net(batch)["seg_logit"].detach()
+    finally:
+        netprog.ENABLED = was
+    (ya, ga), (yb, gb) = out
+    assert float((ya - yb).norm() / ya.norm()) < 1e-4 and torch.equal(yb, y2)
+    i = [k for k, p in enumerate(params) if p is last][0]
+    assert float((ga[i] - gb[i]).norm() / ga[i].norm()) < 1e-3
+    assert all(bool(torch.isfinite(g).all()) for g in gb) and len(gb) == len(params)
+
+
+# ------------------------------------------------------------------ mx8 x mx8
+def _mx8_sum_err(X, W):
+    """The 8-bit matrix instructions add 8 neighbouring products in fixed point before the sum goes on in fp32: each product
+    is cut (towards zero) to a multiple of 2^-13 times the power of two of the group's largest -- seen directly: next to
+    +-2^12, 2^-1 (2^-13 of it) arrives and 2^-2 does not, 1.875 * 2^-1 arrives as 2^-1.  The largest loses nothing, so a
+    group is off by less than 7 * 2^-13 times its largest product, itself at most the product of the largest |x| and |w|."""
+    K = X.shape[1]
+    grp = lambda t: torch.nn.functional.pad(t.abs(), (0, (-K) % 8)).view(t.shape[0], -1, 8).amax(2)  # noqa: E731
+    return 7 * 2.0 ** -13 * (grp(X) @ grp(W).t())
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size", [(1, 1, 1), (1, 32, 16), (3, 100, 40), (13, 2048, 64), (16, 129, 17), (33, 256, 100), (64, 1000, 33),
+                                  (65, 128, 64), (200, 416, 130), (300, 77, 90), (1000, 512, 512), (2500, 640, 300)], ids=str)
+def test_linear_mx8(size, dt):
+    from latte_amd import functional as LF
+    M, K, N = size
+    x, w, b, r = _rn(8, torch.float32, (M, K), (N, K), (N,), (M, N))
+    x = x * torch.ldexp(torch.ones(M, 1, device="cuda"), torch.arange(M, device="cuda").view(-1, 1) % 7 - 3)   # rows of unlike size
+    b, r = b.to(dt), r.to(dt)
+    xq, wq = LF.quantize_mx8(x), LF.quantize_mx8(w * K ** -0.5)
+    X, W = R.mx8(x)[0], R.mx8(w * K ** -0.5)[0]
+    h, lo = R.EPS[dt], R.LOW[dt]
+    for act in ("none", "relu", "gelu", "silu"):
+        with torch.no_grad():
+            y = LF.linear(xq, wq, b, act=act, residual=r if act != "none" else None)
+        Z = X @ W.t() + b.double()
+        zerr = (K + 1) * U * (X.abs() @ W.abs().t() + b.double().abs()) + _mx8_sum_err(X, W)
+        Y = R.act(Z, act)[0] + (r.double() if act != "none" else 0)
+        tol = 1.13 * zerr + (3e-6 * (1 + Z.abs()) if act in ("gelu", "silu") else 0) + 2 * U * Y.abs()
+        assert y.dtype == dt
+        _close(y, Y, tol + h * (Y.abs() + tol) + lo, f"y {act}")
+
+
+def test_linear_mx8_large_tiles_and_nan():
+    from latte_amd import functional as LF
+    M, K, N = 4100, 1040, 3400
+    x, w = _rn(9, torch.float32, (M, K), (N, K))
+    xq, wq = LF.quantize_mx8(x), LF.quantize_mx8(w)
+    with torch.no_grad():
+        y = LF.linear(xq, wq)
+    X, W = R.mx8(x)[0], R.mx8(w)[0]
+    Y = X @ W.t()
+    tol = K * U * (X.abs() @ W.abs().t()) + _mx8_sum_err(X, W)
+    assert y.dtype == torch.bfloat16
+    _close(y, Y, tol + R.EPS[y.dtype] * (Y.abs() + tol), "y")
+    x[7, 3] = float("nan")
+    with torch.no_grad():
+        y2 = LF.linear(LF.quantize_mx8(x), wq)
+    keep = [i for i in range(M) if i != 7]
+    assert torch.equal(y2[keep], y[keep]) and bool(torch.isnan(y2[7]).all())
+
+
+def test_serving_block_together():
+    """norm -> 8-bit product -> residual, as a serving layer calls them, against the same in 64 bits from the held values"""
+    from latte_amd import functional as LF
+    for M in (1, 5, 300):
+        x, r, nw, w, b = _rn(10, torch.bfloat16, (M, 256), (M, 256), (256,), (192, 256), (192,))
+        w8 = LF.quantize_mx8(w)
+        with torch.no_grad():
+            q, h = LF.rms_norm(x, nw, residual=r, out="mx8")
+            y = LF.linear(q, w8, b, act="gelu")
+        Z = q.dequantize().double() @ w8.dequantize().double().t() + b.double()
+        zerr = 258 * U * (q.dequantize().double().abs() @ w8.dequantize().double().abs().t() + b.double().abs())
+        zerr = zerr + _mx8_sum_err(q.dequantize().double(), w8.dequantize().double())
+        tol = 1.13 * zerr + 3e-6 * (1 + Z.abs())
+        Y = R.act(Z, "gelu")[0]
+        _close(y, Y, tol + R.EPS[y.dtype] * (Y.abs() + tol), "y")
+
+
+def test_training_block_together_in_a_graph():
+    """RMSNorm -> Linear(GELU) -> Linear + skip, trained with checkpoints: captured once, replayed over new inputs, equal to
+    the eager step every time"""
+    from latte_amd import sparse_modules as spnn
+    torch.manual_seed(0)
+    net = torch.nn.ModuleList([spnn.RMSNorm(64, checkpoint="mx8"), spnn.Linear(64, 128, act="gelu", checkpoint="mx8"),
+                               spnn.Linear(128, 64, checkpoint="mx8")]).cuda()
+    params = list(net.parameters())
+
+    def step(x, d):
+        y = net[2](net[1](net[0](x)), residual=x)
+        return (y.detach(),) + torch.autograd.grad(y, params, d)
+    x, d = _rn(11, torch.float32, (3001, 64), (3001, 64))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(x, d)
+    torch.cuda.current_stream().wait_stream(s)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = step(x, d)
+    for k in range(4):
+        nx, nd = _rn(12 + k, torch.float32, (3001, 64), (3001, 64))
+        x.copy_(nx)
+        d.copy_(nd)
+        want = [v.clone() for v in step(nx, nd)]
+        gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
