@@ -324,7 +324,8 @@ int lt_devoxelize_cell_bwd(const float* gout, const int32_t* cells, const int32_
 #define LT_ACT_GELU 2 /* z Phi(z) */
 #define LT_ACT_SILU 3 /* z / (1 + exp(-z)) */
 /* what the forward keeps of act'(z): nothing (act none, or no backward will come); bits uint16 [M][ceil(N/16)] (ReLU);
- * bytes [M][N], (c - 32) / 192 (GELU, SiLU); values [M][N] of type dt (GELU, SiLU) */
+ * bytes [M][N], (c - 32) / 192, 255 = NaN (GELU, SiLU); in full [M][N]: fp32 values, or for 16-bit dt uint16 (c - 8192) / 49152,
+ * 65535 = NaN (GELU, SiLU) */
 #define LT_DERIV_NONE 0
 #define LT_DERIV_BITS 1
 #define LT_DERIV_BYTE 2
@@ -340,7 +341,7 @@ int lt_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const 
                   int64_t ws_bytes, lt_stream_t stream);
 /* dz = dy * deriv;  dx[M][K] = dz w;  dw[N][K] = dz^T x;  db[N] = column sums of dz; dx, dw, db may be NULL.  x_scales not
  * NULL: x is mx8 (ldx == K).  Sums are split and joined in a fixed order: the same bits every time. */
-int64_t lt_linear_bwd_workspace_bytes(int64_t M, int32_t K, int32_t N, int32_t dt);
+int64_t lt_linear_bwd_workspace_bytes(int64_t M, int32_t K, int32_t N, int32_t dt, int32_t x_mx8);
 int lt_linear_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* x_scales, const void* w, int64_t ldw,
                   const void* deriv, int32_t deriv_kind, int64_t M, int32_t K, int32_t N, int32_t dt, void* dx, void* dw,
                   void* db, void* ws, int64_t ws_bytes, lt_stream_t stream);

@@ -89,7 +89,7 @@ SIGNATURES = {
     "lt_mx8_dequantize": (ctypes.c_int, [P, P, I64, I32, I32, P, P]),
     "lt_linear_workspace_bytes": (I64, [I64, I32, I32, I32]),
     "lt_linear_fwd": (ctypes.c_int, [P, I64, P, I64, P, P, I64, I32, I64, I32, I32, I32, P, P, I32, P, I64, P]),
-    "lt_linear_bwd_workspace_bytes": (I64, [I64, I32, I32, I32]),
+    "lt_linear_bwd_workspace_bytes": (I64, [I64, I32, I32, I32, I32]),
     "lt_linear_bwd": (ctypes.c_int, [P, I64, P, I64, P, P, I64, P, I32, I64, I32, I32, I32, P, P, P, P, I64, P]),
     "lt_rms_norm_fwd": (ctypes.c_int, [P, I64, P, I64, P, F32, I64, I32, I32, P, P, P, P, P, P, P, P]),
     "lt_rms_norm_bwd_workspace_bytes": (I64, [I64, I32]),

@@ -132,6 +132,15 @@ __device__ __forceinline__ unsigned lt_deriv_byte(float d) {
 __device__ __forceinline__ float lt_deriv_value(unsigned c) {
   return c == 255u ? __builtin_nanf("") : ((float)(int)c - 32.f) * (1.f / 192.f);
 }
+// act'(z) beside 16-bit results, no checkpoint: the same grid in 16 bits, (c - 8192) / 49152, |error| <= 1e-5.  A 16-bit
+// float would be off by up to 2^-9 of act' and, with dz rounded to the type as well, double the variance of every gradient.
+__device__ __forceinline__ unsigned lt_deriv_word(float d) {
+  const float c = rintf(__builtin_amdgcn_fmed3f(__fmaf_rn(d, 49152.f, 8192.f), 0.f, 65534.f));
+  return d == d ? (unsigned)c : 65535u;
+}
+__device__ __forceinline__ float lt_deriv_word_value(unsigned c) {
+  return c == 65535u ? __builtin_nanf("") : ((float)(int)c - 8192.f) * (1.f / 49152.f);
+}
 // y = act(z), d = act'(z).  FAST (16-bit results): erfc by Abramowitz & Stegun 7.1.26 (|error| <= 1.5e-7) and the
 // hardware's exp2 and reciprocal; otherwise the library's functions.
 template <int ACT, bool FAST>
@@ -177,7 +186,8 @@ struct LtEpi {
   int64_t ldres;
   void* out;            // [rows][ldo]
   int64_t ldo;
-  void* deriv;          // LT_DERIV_BITS: uint16 [rows][ceil(cols/16)]; _BYTE: uint8 [rows][cols]; _FULL: type of y
+  void* deriv;          // LT_DERIV_BITS: uint16 [rows][ceil(cols/16)]; _BYTE: uint8 [rows][cols]; _FULL: fp32, or
+                        // uint16 beside 16-bit results, [rows][cols]
   int dkind;
   int64_t rows;
   int cols;
@@ -217,7 +227,16 @@ __device__ __forceinline__ void lt_epi4(const LtEpi& e, lt_f32x4 acc, const floa
       else
         for (int i = 0; i < n; ++i) p[i] = c[i];
     } else if (e.dkind == LT_DERIV_FULL) {
-      lt_stv<T, 4>((T*)e.deriv + row * e.cols + col, n, d);
+      if constexpr (sizeof(T) == 4) lt_stv<float, 4>((float*)e.deriv + row * e.cols + col, n, d);
+      else {
+        uint16_t* p = (uint16_t*)e.deriv + row * e.cols + col;
+        uint16_t c[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] = (uint16_t)lt_deriv_word(d[i]);
+        if (n >= 4) __builtin_memcpy(p, c, 8);
+        else
+          for (int i = 0; i < n; ++i) p[i] = c[i];
+      }
     }
   }
 #pragma unroll

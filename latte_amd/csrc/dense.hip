@@ -2,8 +2,8 @@
 //
 //   forward    z = x W^T + b (fp32 sums);  y = act(z) + r;  kept: x (or mx8(x)), W, act'(z)
 //   backward   dz = dy act'(z);  dx = dz W;  dW = dz^T x;  db = sum_rows dz;  dr = dy
-// act' is kept instead of z: the ReLU's is one bit, the others fit a uniform 8-bit grid (|error| <= 1/384), and the
-// backward pass needs no exponential.  dz is rounded to the operands' type, as the matrix instructions take it.
+// act' is kept instead of z: the ReLU's is one bit, the others fit a uniform grid (8 bits with a checkpoint, |error| <=
+// 1/384; 16 bits beside 16-bit types, 1e-5), and the backward pass needs no exponential.  dz is rounded to the operands' type, as the matrix instructions take it.
 //
 // Replaces the library products of nn.Linear (point branches and heads: latte/models/spvcnn.py:95-111,
 // latte/models/xmuda_arch.py:326-335) where a layer trains or keeps its activations in 8 bits.
@@ -69,7 +69,16 @@ __global__ __launch_bounds__(256) void k_dz(const T* __restrict__ dy, int64_t ld
 #pragma unroll
         for (int i = 0; i < 4; ++i) g[i] *= lt_deriv_value(c[i]);
       } else if constexpr (DK == LT_DERIV_FULL) {
-        lt_ldv<T, 4>((const T*)deriv + row * N + col, n, d);
+        if constexpr (sizeof(T) == 4) lt_ldv<float, 4>((const float*)deriv + row * N + col, n, d);
+        else {
+          const uint16_t* p = (const uint16_t*)deriv + row * N + col;
+          uint16_t c[4] = {0, 0, 0, 0};
+          if (n >= 4) __builtin_memcpy(c, p, 8);
+          else
+            for (int i = 0; i < n; ++i) c[i] = p[i];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d[i] = lt_deriv_word_value(c[i]);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) g[i] *= d[i];
       }
@@ -238,16 +247,23 @@ extern "C" int lt_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t 
   return gemm_run(g, ws, ws ? ws_bytes : 0, stream);
 }
 
+// dW = dz^T x with x in mx8: up to 256 output columns the product widens x while it stages it (x is read once or twice);
+// wider layers would do that once per column tile and without direct staging, so x is widened into the workspace first.
+// 16384 x 1024 -> 4096, bf16: @WIDE@
+static bool widen_first(int64_t M, int K, int N) { return N > 256 && M > 0; }
+
 struct BwdWs {
-  int64_t dz, part, gemm, bytes;
+  int64_t dz, part, wide, gemm, bytes;
 };
-static BwdWs bwd_ws(int64_t M, int K, int N, int dt) {
+static BwdWs bwd_ws(int64_t M, int K, int N, int dt, bool x8) {
   BwdWs w;
   int64_t off = 0;
   w.dz = off;
   off += lt_align_up(M * N * lt_dt_size(dt), 256);
   w.part = off;
   off += lt_align_up((int64_t)dz_plan(M, N).slabs * N * 4, 256);
+  w.wide = off;
+  if (x8 && widen_first(M, K, N)) off += lt_align_up(M * K * lt_dt_size(dt), 256);
   w.gemm = off;
   const int64_t a = gemm_ws_bytes(M, K, N, dt, false), b = gemm_ws_bytes(N, K, M, dt, false);
   off += a > b ? a : b;
@@ -255,9 +271,9 @@ static BwdWs bwd_ws(int64_t M, int K, int N, int dt) {
   return w;
 }
 
-extern "C" int64_t lt_linear_bwd_workspace_bytes(int64_t M, int32_t K, int32_t N, int32_t dt) {
+extern "C" int64_t lt_linear_bwd_workspace_bytes(int64_t M, int32_t K, int32_t N, int32_t dt, int32_t x_mx8) {
   if (check_dense("lt_linear_bwd_workspace_bytes", M, K, N, dt)) return -1;
-  return bwd_ws(M, K, N, dt).bytes;
+  return bwd_ws(M, K, N, dt, x_mx8 != 0).bytes;
 }
 
 extern "C" int lt_linear_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* x_scales, const void* w,
@@ -267,7 +283,7 @@ extern "C" int lt_linear_bwd(const void* dy, int64_t lddy, const void* x, int64_
   if (rc) return rc;
   LT_REQUIRE(deriv_kind >= LT_DERIV_NONE && deriv_kind <= LT_DERIV_FULL, LT_ERR_ARG, "lt_linear_bwd: deriv_kind=%d", deriv_kind);
   LT_REQUIRE(!x_scales || ldx == K, LT_ERR_ARG, "lt_linear_bwd: an mx8 x has rows of K values, not ldx=%lld", (long long)ldx);
-  const BwdWs o = bwd_ws(M, K, N, dt);
+  const BwdWs o = bwd_ws(M, K, N, dt, x_scales != nullptr);
   LT_REQUIRE(ws_bytes >= o.bytes && (ws || o.bytes == 0), LT_ERR_WORKSPACE, "lt_linear_bwd: workspace too small");
   if (M > 0)
     LT_REQUIRE(dy && (deriv_kind == LT_DERIV_NONE || deriv) && (!dx || w) && (!dw || x), LT_ERR_ARG, "lt_linear_bwd: null pointer");
@@ -302,6 +318,12 @@ extern "C" int lt_linear_bwd(const void* dy, int64_t lddy, const void* x, int64_
     g.ldp = ldx;
     g.p_kmajor = true;
     g.p_scales = (const uint8_t*)x_scales;
+    if (x_scales && widen_first(M, K, N)) {
+      if ((rc = lt_mx8_dequantize(x, x_scales, M, K, dt, wsb + o.wide, stream))) return rc;
+      g.P = wsb + o.wide;
+      g.ldp = K;
+      g.p_scales = nullptr;
+    }
     g.Q = dz;
     g.ldq = lddz;
     g.q_kmajor = true;

@@ -127,7 +127,7 @@ def _linear_fwd(x2, ldx, w, ldw, bias, res, act: str, deriv_kind: int):
     elif deriv_kind == _BYTE:
         deriv = torch.empty((M, N), dtype=torch.uint8, device=dev)
     elif deriv_kind == _FULL:
-        deriv = torch.empty((M, N), dtype=x2.dtype, device=dev)
+        deriv = torch.empty((M, N), dtype=torch.float32 if dt == 0 else torch.int16, device=dev)
     nb = _ws_bytes("lt_linear_workspace_bytes", M, K, N, dt)
     ws = _buf(nb, dev) if nb > 0 else None
     r2, ldr = _rows(res, N) if res is not None else (None, 0)
@@ -175,7 +175,7 @@ class _Linear(Function):
         db = torch.empty((N,), dtype=dtype, device=dev) if need[2] else None
         if dx is not None or dw is not None or db is not None:
             dt = _DT[dtype]
-            nb = _ws_bytes("lt_linear_bwd_workspace_bytes", M, K, N, dt)
+            nb = _ws_bytes("lt_linear_bwd_workspace_bytes", M, K, N, dt, int(xs is not None))
             ws = _buf(nb, dev)
             ldx = 0 if x2 is None else (K if xs is not None else _rows(x2, K)[1])
             ldw = 0 if w2 is None else _rows(w2, K)[1]
