@@ -193,55 +193,57 @@ struct LtEpi {
   int cols;
 };
 
+// eight neighbours (row, col..col+7) of the product, n of which exist (<= 0: nothing to do), with their residual (loaded
+// ahead: the stores in between would hold the loads back)
 template <class T>
-__device__ __forceinline__ void lt_epi_bias(const LtEpi& e, int col, float (&b)[4]) {
-  b[0] = b[1] = b[2] = b[3] = 0.f;
-  if (e.bias) lt_ldv<T, 4>((const T*)e.bias + col, e.cols - col, b);
+__device__ __forceinline__ void lt_epi_res(const LtEpi& e, int64_t row, int col, int n, float (&r)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = 0.f;
+  if (e.res && n > 0) lt_ldv<T, 8>((const T*)e.res + row * e.ldres + col, n, r);
 }
-template <class T>
-__device__ __forceinline__ void lt_epi_res(const LtEpi& e, int64_t row, int col, float (&r)[4]) {
-  r[0] = r[1] = r[2] = r[3] = 0.f;
-  if (e.res && row < e.rows) lt_ldv<T, 4>((const T*)e.res + row * e.ldres + col, e.cols - col, r);
-}
-// four neighbours (row, col..col+3) of the product with their bias and residual (loaded ahead: the stores in between
-// would hold the loads back); nib = their ReLU bits (the caller joins four lanes into 16 bits)
 template <class T, int ACT>
-__device__ __forceinline__ void lt_epi4(const LtEpi& e, lt_f32x4 acc, const float (&b)[4], const float (&r)[4], int64_t row, int col,
-                                        unsigned& nib) {
-  nib = 0;
-  const int n = row < e.rows ? e.cols - col : 0;
+__device__ __forceinline__ void lt_epi8(const LtEpi& e, const float (&z)[8], const float (&b)[8], const float (&r)[8], int64_t row,
+                                        int col, int n) {
   if (n <= 0) return;
-  float y[4], d[4];
+  float y[8], d[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) lt_act<ACT, sizeof(T) == 2>(acc[i] + b[i], y[i], d[i]);
-  if constexpr (ACT != LT_ACT_NONE) {
+  for (int i = 0; i < 8; ++i) lt_act<ACT, sizeof(T) == 2>(z[i] + b[i], y[i], d[i]);
+  if constexpr (ACT == LT_ACT_RELU) {
     if (e.dkind == LT_DERIV_BITS) {
+      unsigned m = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) nib |= (d[i] != 0.f && i < n) ? 1u << i : 0u;
-    } else if (e.dkind == LT_DERIV_BYTE) {
+      for (int i = 0; i < 8; ++i) m |= d[i] != 0.f ? 1u << i : 0u;
+      ((uint8_t*)e.deriv)[row * (((e.cols + 15) >> 4) * 2) + (col >> 3)] = (uint8_t)m;
+    }
+  } else if constexpr (ACT != LT_ACT_NONE) {
+    if (e.dkind == LT_DERIV_BYTE) {
       uint8_t* p = (uint8_t*)e.deriv + row * e.cols + col;
-      uint8_t c[4];
+      uint8_t c[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) c[i] = (uint8_t)lt_deriv_byte(d[i]);
-      if (n >= 4) __builtin_memcpy(p, c, 4);
+      for (int i = 0; i < 8; ++i) c[i] = (uint8_t)lt_deriv_byte(d[i]);
+      if (n >= 8) __builtin_memcpy(p, c, 8);
       else
-        for (int i = 0; i < n; ++i) p[i] = c[i];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < n) p[i] = c[i];
     } else if (e.dkind == LT_DERIV_FULL) {
-      if constexpr (sizeof(T) == 4) lt_stv<float, 4>((float*)e.deriv + row * e.cols + col, n, d);
+      if constexpr (sizeof(T) == 4) lt_stv<float, 8>((float*)e.deriv + row * e.cols + col, n, d);
       else {
         uint16_t* p = (uint16_t*)e.deriv + row * e.cols + col;
-        uint16_t c[4];
+        uint16_t c[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] = (uint16_t)lt_deriv_word(d[i]);
-        if (n >= 4) __builtin_memcpy(p, c, 8);
+        for (int i = 0; i < 8; ++i) c[i] = (uint16_t)lt_deriv_word(d[i]);
+        if (n >= 8) __builtin_memcpy(p, c, 16);
         else
-          for (int i = 0; i < n; ++i) p[i] = c[i];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = c[i];
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) y[i] += r[i];
-  lt_stv<T, 4>((T*)e.out + row * e.ldo + col, n, y);
+  for (int i = 0; i < 8; ++i) y[i] += r[i];
+  lt_stv<T, 8>((T*)e.out + row * e.ldo + col, n, y);
 }
 
 // out[c] = sum over slabs of part[slab][c]: 16 columns a workgroup, 16 threads a column, fixed order

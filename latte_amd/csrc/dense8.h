@@ -124,7 +124,10 @@ __global__ __launch_bounds__(64 * WR * WC) void k_dense8(LtTile8Args b) {
       compute(cur);
     }
   }
-  lt_tile_store<T, FR, FC, ACT>(a, acc, split, row0 + wr, col0 + wc, lane);
+  static_assert(NW * LtTurn<FC>::BYTES <= 2 * BUF, "the turned rows do not fit the tiles' LDS");
+  __syncthreads();
+  lt_tile_store<T, FR, FC, ACT>(a, acc, split, row0 + wr, col0 + wc, lane,
+                                reinterpret_cast<float*>(s_tile + wave * LtTurn<FC>::BYTES));
 }
 
 // few rows: as k_dense_few, 128 k an instruction straight from memory

@@ -201,47 +201,51 @@ __device__ __forceinline__ unsigned lt_xcd_map(unsigned b, unsigned n) {
   return x * per + (x < rem ? x : rem) + (b >> 3);
 }
 
-// a wave's accumulators -> partial sums of its split, or the epilogue; (row0, col0) = the wave's corner
+// A wave's accumulators -> partial sums of its split, or the epilogue; (row0, col0) = the wave's corner, s = its piece of
+// LDS (the tiles are no longer read).  A lane's four columns of one row would make stores of 16 bytes a row and line, so 16
+// rows at a time turn through LDS and leave eight columns a lane: whole 128-byte lines of 16-bit results.
+template <int FC> struct LtTurn { static constexpr int LD = 16 * FC + 4, BYTES = 16 * LD * 4; };
 template <class T, int FR, int FC, int ACT>
 __device__ __forceinline__ void lt_tile_store(const LtTileArgs& a, const lt_f32x4 (&acc)[FR][FC], unsigned split, int64_t row0, int col0,
-                                              int lane) {
+                                              int lane, float* s) {
+  constexpr int LD = LtTurn<FC>::LD, LPR = FC * 2, RPP = 64 / LPR < 16 ? 64 / LPR : 16, PASS = 16 / RPP;   // lanes a row, rows a pass
   const int r = lane & 15, g = lane >> 4;
-  if (a.splits > 1) {
+  const int pr = lane / LPR, col = col0 + (lane % LPR) * 8;
+  const bool use = lane < LPR * RPP;
+  const int64_t nc = use ? a.cols - col : 0;
+  float b[8];
 #pragma unroll
-    for (int i = 0; i < FR; ++i)
-#pragma unroll
-      for (int j = 0; j < FC; ++j) {
-        const int64_t row = row0 + 16 * i + r;
-        const int col = col0 + 16 * j + 4 * g;
-        if (row < a.rows && col < a.cols) {
-          const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-          lt_stv<float, 4>(a.part + ((int64_t)split * a.rows + row) * a.cols + col, a.cols - col, v);
-        }
-      }
-    return;
-  }
-  float b[FC][4];
-#pragma unroll
-  for (int j = 0; j < FC; ++j) lt_epi_bias<T>(a.epi, col0 + 16 * j + 4 * g, b[j]);
+  for (int i = 0; i < 8; ++i) b[i] = 0.f;
+  if (a.splits == 1 && a.epi.bias) lt_ldv<T, 8>((const T*)a.epi.bias + col, nc, b);
 #pragma unroll
   for (int i = 0; i < FR; ++i) {
-    const int64_t row = row0 + 16 * i + r;
-    float res[FC][4];
+    float res[PASS][8];
+    if (a.splits == 1) {
 #pragma unroll
-    for (int j = 0; j < FC; ++j) lt_epi_res<T>(a.epi, row, col0 + 16 * j + 4 * g, res[j]);
+      for (int p = 0; p < PASS; ++p) {
+        const int64_t row = row0 + 16 * i + p * RPP + pr;
+        lt_epi_res<T>(a.epi, row, col, row < a.rows ? (int)nc : 0, res[p]);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the rows before have been read
 #pragma unroll
-    for (int j = 0; j < FC; ++j) {
-      const int col = col0 + 16 * j + 4 * g;
-      unsigned nib;
-      lt_epi4<T, ACT>(a.epi, acc[i][j], b[j], res[j], row, col, nib);
-      if constexpr (ACT == LT_ACT_RELU) {
-        if (a.epi.dkind == LT_DERIV_BITS) {   // the four lanes of a row join their bits: 16 columns
-          nib <<= 4 * g;
-          nib |= __shfl_xor(nib, 16, 64);
-          nib |= __shfl_xor(nib, 32, 64);
-          if (g == 0 && row < a.rows && col < a.cols)
-            ((uint16_t*)a.epi.deriv)[row * ((a.cols + 15) >> 4) + (col >> 4)] = (uint16_t)nib;
-        }
+    for (int j = 0; j < FC; ++j) *reinterpret_cast<lt_f32x4*>(s + r * LD + 16 * j + 4 * g) = acc[i][j];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int p = 0; p < PASS; ++p) {
+      const int64_t row = row0 + 16 * i + p * RPP + pr;
+      const int n = row < a.rows ? (int)nc : 0;
+      float z[8];
+      if (use) {
+        const float* src = s + (p * RPP + pr) * LD + (lane % LPR) * 8;
+        const lt_f32x4 u = *reinterpret_cast<const lt_f32x4*>(src), v = *reinterpret_cast<const lt_f32x4*>(src + 4);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) z[t] = u[t], z[4 + t] = v[t];
+      }
+      if (a.splits > 1) {
+        if (n > 0) lt_stv<float, 8>(a.part + ((int64_t)split * a.rows + row) * a.cols + col, n, z);
+      } else {
+        lt_epi8<T, ACT>(a.epi, z, b, res[p], row, col, n);
       }
     }
   }
@@ -335,7 +339,10 @@ __global__ __launch_bounds__(64 * WR * WC) void k_dense(LtTileArgs a) {
     }
   }
 
-  lt_tile_store<T, FR, FC, ACT>(a, acc, split, row0 + wr, col0 + wc, lane);
+  static_assert(NW * LtTurn<FC>::BYTES <= 2 * BUF, "the turned rows do not fit the tiles' LDS");
+  __syncthreads();
+  lt_tile_store<T, FR, FC, ACT>(a, acc, split, row0 + wr, col0 + wc, lane,
+                                reinterpret_cast<float*>(s_tile + wave * LtTurn<FC>::BYTES));
 }
 
 // out = epilogue(sum over the splits, in a fixed order: the same bits every time).  G threads share four neighbours and take
@@ -343,50 +350,48 @@ __global__ __launch_bounds__(64 * WR * WC) void k_dense(LtTileArgs a) {
 template <class T, int ACT, int G>
 __global__ __launch_bounds__(256) void k_dense_join(const float* __restrict__ part, int splits, LtEpi e) {
   constexpr int EL = 256 / G;
-  __shared__ lt_f32x4 s_sum[G][EL];
+  __shared__ float s_sum[G > 1 ? G : 1][8][EL];
   const int el = threadIdx.x % EL, sl = threadIdx.x / EL;
-  const int c4 = ((e.cols + 15) >> 4) * 4;   // four lanes to 16 columns
-  const int64_t n = e.rows * c4, stride = (int64_t)gridDim.x * EL;
+  const int c8 = (e.cols + 7) >> 3;
+  const int64_t n = e.rows * c8, stride = (int64_t)gridDim.x * EL;
   const int64_t plane = e.rows * e.cols;
   for (int64_t b = blockIdx.x * (int64_t)EL; b < n; b += stride) {
     const int64_t i = b + el;
-    int64_t row = e.rows;
-    int col = 0;
-    if (i < n) lt_divmod(i, c4, row, col);
-    col *= 4;
-    lt_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    if (row < e.rows && col < e.cols) {
+    int64_t row = 0;
+    int col = e.cols;
+    if (i < n) {
+      lt_divmod(i, c8, row, col);
+      col *= 8;
+    }
+    const int m = e.cols - col;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (m > 0) {
       const float* p = part + row * e.cols + col;
-#pragma unroll 8
+#pragma unroll 4
       for (int s = sl; s < splits; s += G) {
-        float v[4];
-        lt_ldv<float, 4>(p + s * plane, e.cols - col, v);
+        float v[8];
+        lt_ldv<float, 8>(p + s * plane, m, v);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) acc[t] += v[t];
+        for (int t = 0; t < 8; ++t) acc[t] += v[t];
       }
     }
     if constexpr (G > 1) {
       __syncthreads();   // the previous turn's sums have been read
-      s_sum[sl][el] = acc;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) s_sum[sl][t][el] = acc[t];
       __syncthreads();
       if (sl != 0) continue;
 #pragma unroll
-      for (int s = 1; s < G; ++s) acc += s_sum[s][el];
+      for (int s = 1; s < G; ++s)
+#pragma unroll
+        for (int t = 0; t < 8; ++t) acc[t] += s_sum[s][t][el];
     }
-    unsigned nib;
-    float bias[4], res[4];
-    lt_epi_bias<T>(e, col, bias);
-    lt_epi_res<T>(e, row, col, res);
-    lt_epi4<T, ACT>(e, acc, bias, res, row, col, nib);
-    if constexpr (ACT == LT_ACT_RELU) {
-      if (e.dkind == LT_DERIV_BITS) {
-        nib <<= 4 * (threadIdx.x & 3);
-        nib |= __shfl_xor(nib, 1, 64);
-        nib |= __shfl_xor(nib, 2, 64);
-        if ((threadIdx.x & 3) == 0 && row < e.rows && col < e.cols)
-          ((uint16_t*)e.deriv)[row * ((e.cols + 15) >> 4) + (col >> 4)] = (uint16_t)nib;
-      }
-    }
+    float bias[8], res[8];
+#pragma unroll
+    for (int t = 0; t < 8; ++t) bias[t] = 0.f;
+    if (e.bias) lt_ldv<T, 8>((const T*)e.bias + col, m, bias);
+    lt_epi_res<T>(e, row, col, m, res);
+    lt_epi8<T, ACT>(e, acc, bias, res, row, col, m);
   }
 }
 
@@ -394,31 +399,31 @@ __global__ __launch_bounds__(256) void k_dense_join(const float* __restrict__ pa
 template <class T, int FR, int ACT>
 __device__ __forceinline__ void lt_few_store(const LtTileArgs& a, const lt_f32x4 (&acc)[FR], lt_f32x4 (*s_acc)[FR][64], int col0, int wave,
                                              int lane) {
-  const int r = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int f = 0; f < FR; ++f) s_acc[wave][f][lane] = acc[f];
   __syncthreads();
+  lt_f32x4 s = {0.f, 0.f, 0.f, 0.f};
   if (wave < FR) {
-    lt_f32x4 s = s_acc[0][wave][lane];
+    s = s_acc[0][wave][lane];
 #pragma unroll
     for (int w = 1; w < 8; ++w) s += s_acc[w][wave][lane];
-    const int64_t row = wave * 16 + r;
-    const int col = col0 + 4 * g;
-    unsigned nib;
-    float b[4], res[4];
-    lt_epi_bias<T>(a.epi, col, b);
-    lt_epi_res<T>(a.epi, row, col, res);
-    lt_epi4<T, ACT>(a.epi, s, b, res, row, col, nib);
-    if constexpr (ACT == LT_ACT_RELU) {
-      if (a.epi.dkind == LT_DERIV_BITS) {
-        nib <<= 4 * g;
-        nib |= __shfl_xor(nib, 16, 64);
-        nib |= __shfl_xor(nib, 32, 64);
-        if (g == 0 && row < a.rows && col < a.cols)
-          ((uint16_t*)a.epi.deriv)[row * ((a.cols + 15) >> 4) + (col >> 4)] = (uint16_t)nib;
-      }
-    }
   }
+  // lane 16 g + r holds columns 4 g .. 4 g + 3 of row r; two lanes' columns make one lane's eight
+  lt_f32x4 t;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t[i] = __shfl_xor(s[i], 16, 64);
+  const int g = lane >> 4;
+  if (wave >= FR || (g & 1)) return;
+  const int64_t row = wave * 16 + (lane & 15);
+  const int col = col0 + 4 * g, n = row < a.rows ? a.cols - col : 0;
+  if (n <= 0) return;
+  const float z[8] = {s[0], s[1], s[2], s[3], t[0], t[1], t[2], t[3]};
+  float b[8], res[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) b[i] = 0.f;
+  if (a.epi.bias) lt_ldv<T, 8>((const T*)a.epi.bias + col, n, b);
+  lt_epi_res<T>(a.epi, row, col, n, res);
+  lt_epi8<T, ACT>(a.epi, z, b, res, row, col, n);
 }
 
 // ---- few rows: y[rows <= 64][cols].  Bound by reading P once: a workgroup takes 16 columns, its 8 waves share k in
@@ -561,7 +566,7 @@ static int lt_launch_few(const LtTileArgs& a, hipStream_t stream) {
 
 template <class T, int ACT>
 static int lt_launch_join(const LtEpi& e, const float* part, int splits, hipStream_t stream) {
-  const int64_t n = e.rows * (int64_t)(((e.cols + 15) >> 4) * 4);
+  const int64_t n = e.rows * (int64_t)((e.cols + 7) >> 3);
   if (splits >= 64) hipLaunchKernelGGL((k_dense_join<T, ACT, 16>), dim3(lt_grid(n, 16)), dim3(256), 0, stream, part, splits, e);
   else if (splits >= 8) hipLaunchKernelGGL((k_dense_join<T, ACT, 4>), dim3(lt_grid(n, 64)), dim3(256), 0, stream, part, splits, e);
   else hipLaunchKernelGGL((k_dense_join<T, ACT, 1>), dim3(lt_grid(n, 256)), dim3(256), 0, stream, part, splits, e);
