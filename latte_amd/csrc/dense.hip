@@ -249,7 +249,7 @@ extern "C" int lt_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t 
 
 // dW = dz^T x with x in mx8: up to 256 output columns the product widens x while it stages it (x is read once or twice);
 // wider layers would do that once per column tile and without direct staging, so x is widened into the workspace first.
-// 16384 x 1024 -> 4096, bf16: @WIDE@
+// 16384 x 1024 -> 4096, bf16: a training step 1130 us with the widening in the staging, 696 us with it first
 static bool widen_first(int64_t M, int K, int N) { return N > 256 && M > 0; }
 
 struct BwdWs {

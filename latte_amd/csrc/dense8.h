@@ -17,6 +17,8 @@ struct LtTile8Args {
   int nb;               // scales a row
 };
 
+template <int V> struct LtInt { static constexpr int value = V; };
+
 // scale byte of k-block kb of a row; blocks past the end hold zeros, whose scale must only be finite
 __device__ __forceinline__ int lt_scale8(const uint8_t* row, int kb, int nb) { return kb < nb ? row[kb] : 127; }
 
@@ -32,10 +34,10 @@ __device__ __forceinline__ lt_i32x8 lt_frag8(const char* t, int i0, int lane) {
 template <class T, int BR, int BC, int WR, int WC, bool DIRECT, int ACT>
 __global__ __launch_bounds__(64 * WR * WC) void k_dense8(LtTile8Args b) {
   const LtTileArgs& a = b.t;
-  typedef LtTile<uint8_t, false, BC> TP;
-  typedef LtTile<uint8_t, false, BR> TQ;
+  typedef LtTile<uint8_t, false, BC, 128> TP;
+  typedef LtTile<uint8_t, false, BR, 128> TQ;
   constexpr int NW = WR * WC, NT = 64 * NW, FR = BR / WR / 16, FC = BC / WC / 16;
-  constexpr int BUF = TP::BYTES + TQ::BYTES;
+  constexpr int BUF = TP::BYTES + TQ::BYTES, NBUF = 2;
   extern __shared__ __attribute__((aligned(1024))) char s_tile[];
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -54,11 +56,38 @@ __global__ __launch_bounds__(64 * WR * WC) void k_dense8(LtTile8Args b) {
   const int64_t pn = a.cols - col0, qn = a.rows - row0;
   const int wr = (wave / WC) * (BR / WR), wc = (wave % WC) * (BC / WC);
 
-  const uint8_t *ps[FC], *qs[FR];   // scale rows of this lane's fragments (rows that do not exist: any row's)
+  // Scales: four steps' worth, 16 bytes a row, go through LDS at a time.  They are turned there so that a lane's four bytes
+  // (block g of each of the four steps) are one word, of which the instruction picks byte t & 3 itself.  Loading each
+  // fragment's byte from memory instead took more address cycles than the tiles' own loads (8192^3: 956 us, this: 521 us).
+  char* s_sc = s_tile + 2 * BUF;                 // [2][BC + BR][16]
+  const bool srow_ok = tid < BC ? tid < pn : (tid < BC + BR && tid - BC < qn);
+  const uint8_t* srow = tid < BC ? a.ps + (int64_t)(srow_ok ? col0 + tid : 0) * b.nb : b.qs + (srow_ok ? row0 + tid - BC : 0) * (int64_t)b.nb;
+  unsigned sw[4];
+  auto sc_load = [&](int kb) {                   // blocks past the end hold zeros, whose scale must only be finite
+    const int n = srow_ok ? b.nb - kb : 0;
+    if (n >= 16) __builtin_memcpy(sw, srow + kb, 16);
+    else {
 #pragma unroll
-  for (int j = 0; j < FC; ++j) ps[j] = a.ps + (int64_t)(wc + 16 * j + r < pn ? col0 + wc + 16 * j + r : 0) * b.nb;
+      for (int w = 0; w < 4; ++w) {
+        sw[w] = 0x7F7F7F7Fu;
 #pragma unroll
-  for (int i = 0; i < FR; ++i) qs[i] = b.qs + (wr + 16 * i + r < qn ? row0 + wr + 16 * i + r : 0) * b.nb;
+        for (int t = 0; t < 4; ++t)
+          if (4 * w + t < n) sw[w] = (sw[w] & ~(0xFFu << (8 * t))) | ((unsigned)srow[kb + 4 * w + t] << (8 * t));
+      }
+    }
+  };
+  auto sc_store = [&](int buf) {
+    if (tid < BC + BR) {
+      const unsigned l01 = __builtin_amdgcn_perm(sw[1], sw[0], 0x05010400u), h01 = __builtin_amdgcn_perm(sw[1], sw[0], 0x07030602u);
+      const unsigned l23 = __builtin_amdgcn_perm(sw[3], sw[2], 0x05010400u), h23 = __builtin_amdgcn_perm(sw[3], sw[2], 0x07030602u);
+      lt_i32x4 o;
+      o[0] = (int)__builtin_amdgcn_perm(l23, l01, 0x05040100u);   // block 0 of steps 0 .. 3
+      o[1] = (int)__builtin_amdgcn_perm(l23, l01, 0x07060302u);
+      o[2] = (int)__builtin_amdgcn_perm(h23, h01, 0x05040100u);
+      o[3] = (int)__builtin_amdgcn_perm(h23, h01, 0x07060302u);
+      *reinterpret_cast<lt_i32x4*>(s_sc + buf * (BC + BR) * 16 + tid * 16) = o;
+    }
+  };
   lt_f32x4 acc[FR][FC];
 #pragma unroll
   for (int i = 0; i < FR; ++i)
@@ -66,65 +95,91 @@ __global__ __launch_bounds__(64 * WR * WC) void k_dense8(LtTile8Args b) {
     for (int j = 0; j < FC; ++j) acc[i][j] = (lt_f32x4){0.f, 0.f, 0.f, 0.f};
 
   int sp_[FC], sq_[FR];
-  auto scales = [&](int kb) {
+  auto sc_read = [&](int buf) {
+    const char* p = s_sc + buf * (BC + BR) * 16 + 4 * g;
 #pragma unroll
-    for (int j = 0; j < FC; ++j) sp_[j] = lt_scale8(ps[j], kb + g, b.nb);
+    for (int j = 0; j < FC; ++j) sp_[j] = *reinterpret_cast<const int*>(p + (wc + 16 * j + r) * 16);
 #pragma unroll
-    for (int i = 0; i < FR; ++i) sq_[i] = lt_scale8(qs[i], kb + g, b.nb);
+    for (int i = 0; i < FR; ++i) sq_[i] = *reinterpret_cast<const int*>(p + (BC + wr + 16 * i + r) * 16);
   };
-  auto compute = [&](const char* buf) {
+  auto mma = [&](const char* buf, auto sel, auto ahead) {
+    constexpr int S = decltype(sel)::value;
     lt_i32x8 p[FC];
 #pragma unroll
     for (int j = 0; j < FC; ++j) p[j] = lt_frag8<BC>(buf, wc + 16 * j, lane);
+    ahead();
 #pragma unroll
     for (int i = 0; i < FR; ++i) {
       const lt_i32x8 q = lt_frag8<BR>(buf + TP::BYTES, wr + 16 * i, lane);
 #pragma unroll
       for (int j = 0; j < FC; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(p[j], q, acc[i][j], 0, 0, 0, sp_[j], 0, sq_[i]);
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(p[j], q, acc[i][j], 0, 0, S, sp_[j], S, sq_[i]);
     }
   };
   const int kb0 = (int)(k0 >> 5);
+  const int64_t len = kend - k0;
+  sc_load(kb0);
   if constexpr (DIRECT) {
     LtDirect<TP, false, NW> sp;
     LtDirect<TQ, false, NW> sq;
     sp.init(a.ldp, pn, wave, lane);
     sq.init(a.ldq, qn, wave, lane);
-    sp.load(pb, s_tile, kend - k0, wave, lane);
-    sq.load(qb, s_tile + TP::BYTES, kend - k0, wave, lane);
-    for (int t = 0; t < nk; ++t) {
-      char* cur = s_tile + (t & 1) * BUF;
-      char* nxt = s_tile + ((t + 1) & 1) * BUF;
-      scales(kb0 + 4 * t);
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      if (t + 1 < nk) {
-        const int64_t left = kend - k0 - (int64_t)(t + 1) * 128;
-        sp.load(pb + (t + 1) * 128, nxt, left, wave, lane);
-        sq.load(qb + (t + 1) * 128, nxt + TP::BYTES, left, wave, lane);
+    auto issue = [&](int t) {
+      char* buf = s_tile + (t & 1) * BUF;
+      sp.load(pb + (int64_t)t * 128, buf, len - (int64_t)t * 128, wave, lane);
+      sq.load(qb + (int64_t)t * 128, buf + TP::BYTES, len - (int64_t)t * 128, wave, lane);
+    };
+    auto step = [&](int t, auto sel) {
+      constexpr int S = decltype(sel)::value;
+      if (t >= nk) return;
+      if (S == 0) sc_store((t >> 2) & 1);        // its last readers are two barriers back
+      lt_wait_barrier();                         // this step's tiles (and scales) are there, nobody reads the other buffer
+      if (S == 0) {
+        sc_read((t >> 2) & 1);
+        if (t + 4 < nk) sc_load(kb0 + 4 * (t + 4));
       }
-      compute(cur);
+      mma(s_tile + (t & 1) * BUF, sel, [&]() {
+        if (t + 1 < nk) issue(t + 1);
+      });
+    };
+    issue(0);
+    for (int t = 0; t < nk; t += 4) {
+      step(t, LtInt<0>());
+      step(t + 1, LtInt<1>());
+      step(t + 2, LtInt<2>());
+      step(t + 3, LtInt<3>());
     }
   } else {
     LtStaged<uint8_t, TP, false, false, NT> sp;
     LtStaged<uint8_t, TQ, false, false, NT> sq;
-    sp.load(pb, a.ldp, pn, kend - k0, nullptr, 0, 0, tid);
-    sq.load(qb, a.ldq, qn, kend - k0, nullptr, 0, 0, tid);
-    for (int t = 0; t < nk; ++t) {
+    auto get = [&](int t) {
+      sp.load(pb + (int64_t)t * 128, a.ldp, pn, len - (int64_t)t * 128, nullptr, 0, 0, tid);
+      sq.load(qb + (int64_t)t * 128, a.ldq, qn, len - (int64_t)t * 128, nullptr, 0, 0, tid);
+    };
+    auto step = [&](int t, auto sel) {
+      constexpr int S = decltype(sel)::value;
+      if (t >= nk) return;
       char* cur = s_tile + (t & 1) * BUF;
       sp.store(cur, tid);
       sq.store(cur + TP::BYTES, tid);
-      scales(kb0 + 4 * t);
+      if (S == 0) sc_store((t >> 2) & 1);
       __syncthreads();
-      if (t + 1 < nk) {
-        const int64_t left = kend - k0 - (int64_t)(t + 1) * 128;
-        sp.load(pb + (t + 1) * 128, a.ldp, pn, left, nullptr, 0, 0, tid);
-        sq.load(qb + (t + 1) * 128, a.ldq, qn, left, nullptr, 0, 0, tid);
+      if (S == 0) {
+        sc_read((t >> 2) & 1);
+        if (t + 4 < nk) sc_load(kb0 + 4 * (t + 4));
       }
-      compute(cur);
+      if (t + 1 < nk) get(t + 1);
+      mma(cur, sel, [] {});
+    };
+    get(0);
+    for (int t = 0; t < nk; t += 4) {
+      step(t, LtInt<0>());
+      step(t + 1, LtInt<1>());
+      step(t + 2, LtInt<2>());
+      step(t + 3, LtInt<3>());
     }
   }
-  static_assert(NW * LtTurn<FC>::BYTES <= 2 * BUF, "the turned rows do not fit the tiles' LDS");
+  static_assert(NW * LtTurn<FC>::BYTES <= NBUF * BUF, "the turned rows do not fit the tiles' LDS");
   __syncthreads();
   lt_tile_store<T, FR, FC, ACT>(a, acc, split, row0 + wr, col0 + wc, lane,
                                 reinterpret_cast<float*>(s_tile + wave * LtTurn<FC>::BYTES));
@@ -188,7 +243,7 @@ template <class T> int lt_gemm8_launch(const LtTile8Args& b, const LtPlan& p, in
 
 template <class T, int BR, int BC, int WR, int WC, bool DIRECT, int ACT>
 static int lt_launch_tile8(const LtTile8Args& b, hipStream_t stream) {
-  const int smem = 2 * (BR + BC) * 128;
+  const int smem = 2 * (BR + BC) * 128 + 2 * (BR + BC) * 16;
   if (smem > 65536)
     LT_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_dense8<T, BR, BC, WR, WC, DIRECT, ACT>),
                                      hipFuncAttributeMaxDynamicSharedMemorySize, smem));

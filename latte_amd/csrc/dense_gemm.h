@@ -1,15 +1,18 @@
 // The tiled product of the dense operators, and its joins.  out[i][j] = sum_k Q(i,k) P(j,k).
 //
 // The matrix instructions compute D = A B with A = P (output columns) and B = Q (output rows): a lane then holds four
-// neighbouring COLUMNS of one output row, so bias, residual and result move 8 or 16 bytes at a time.  A workgroup owns a
-// BR x BC tile of the output and walks k in steps of 128 bytes (64 16-bit or 32 fp32 values) through two LDS buffers, one
-// barrier a step: while the step's matrix instructions run, the next step's tiles are on the way.
+// neighbouring COLUMNS of one output row.  A workgroup owns a BR x BC tile of the output and walks k.
+// k in steps of 128 bytes (64 16-bit or 32 fp32 values) through two LDS buffers, one barrier a step: while the step's
+// matrix instructions run, the next step's tiles are on the way.  Tiles go from memory straight into LDS where lines are
+// 16-byte aligned, through registers elsewhere (and where mx8 is widened on the way).
+//   8192 x 4096 -> 4096, bf16: 220 us, 1250 TFLOP/s (243 us with a residual); steps of 64 bytes through four buffers, three
+//   steps ahead: 253 us -- the barriers and the 64-byte requests cost more than the distance gives.
 //
 // LDS images, 16-byte chunks:
-//   operand [i][k]  (k runs along memory)  : tile [R][128 B], chunk c of row i at position c ^ (i & 7)
-//   operand [k][i]  (i runs along memory)  : tile [BK][R], chunk c of line k at position c ^ f(k), see kswz(); 16-bit
-//                                            fragments are read with the transposing LDS read (4 lines x 16 columns)
-// Both keep every fragment read free of bank conflicts between the lanes that are served together.
+//   operand [i][k]  (k runs along memory)  : tile [R][BKB], chunk c of row i at position c ^ rswz(i)
+//   operand [k][i]  (i runs along memory)  : tile [BK][R], chunk c of line k at position c ^ kswz(k); 16-bit fragments are
+//                                            read with the transposing LDS read (4 lines x 16 columns)
+// Both spread the lanes that are served together over all banks (conflicts: 2 % of the LDS cycles).
 #pragma once
 #include "dense.h"
 
@@ -48,11 +51,13 @@ template <> struct LtMma<float> {
 
 template <> struct LtMma<uint8_t> { typedef lt_i32x8 frag; };   // mx8: dense8.h
 
-template <class T, bool KM, int R>   // an operand's tile: R rows (or columns) of the product, 128 bytes' worth of k
+template <class T, bool KM, int R, int BKB>   // an operand's tile: R rows (or columns) of the product, BKB bytes' worth of k
 struct LtTile {
-  static constexpr int SZ = sizeof(T), CH = 16 / SZ, BK = 128 / SZ;
-  static constexpr int BYTES = R * 128, SEGS = BYTES / 1024;
-  static constexpr int CPL = KM ? R / CH : 8;   // chunks per line
+  static constexpr int SZ = sizeof(T), CH = 16 / SZ, BK = BKB / SZ;
+  static constexpr int BYTES = R * BKB, SEGS = BYTES / 1024;
+  static constexpr int CPL = KM ? R / CH : BKB / 16;   // chunks per line
+  // rows of 128 (64) bytes meet in a bank every 2 (4) rows
+  static __device__ __forceinline__ int rswz(int i) { return BKB == 128 ? i & 7 : (i >> 2) & 3; }
   // k-major lines of one fragment read must not meet in a bank: 16-bit reads take 32 bytes of lines k0 + {0..3} per 16
   // lanes, fp32 reads 64 bytes of lines k0 + {0, 4, 8, 12}
   static __device__ __forceinline__ int kswz(int k) {
@@ -62,14 +67,14 @@ struct LtTile {
   // chunk L (linear position in the image) -> its line and its chunk within the line in memory
   static __device__ __forceinline__ void where(int L, int& line, int& c) {
     line = L / CPL;
-    c = (L % CPL) ^ (KM ? kswz(line) : (line & 7));
+    c = (L % CPL) ^ (KM ? kswz(line) : rswz(line));
   }
   // fragment kk of the 16 rows from i0: k = kk * KF + ..., KF = 32 (16-bit) or 16 (fp32)
   static __device__ __forceinline__ typename LtMma<T>::frag frag(const char* t, int i0, int kk, int lane) {
     const int r = lane & 15, g = lane >> 4;
     if constexpr (!KM) {
       const int i = i0 + r, c = kk * 4 + g;
-      return *reinterpret_cast<const typename LtMma<T>::frag*>(t + i * 128 + ((c ^ (i & 7)) << 4));
+      return *reinterpret_cast<const typename LtMma<T>::frag*>(t + i * BKB + ((c ^ rswz(i)) << 4));
     } else if constexpr (SZ == 2) {
       const int k = kk * 32 + 8 * g + (r >> 2), col = i0 + 4 * (r & 3);
       const char* p = t + k * (R * 2) + (((col >> 3) ^ kswz(k)) << 4) + (col & 7) * 2;   // kswz(k + 4) == kswz(k)
@@ -102,13 +107,16 @@ __device__ __forceinline__ void lt_load_lds16(const char* base, char* lds, unsig
 // loads zeros.  Needs 16-byte aligned lines, k (or the columns, k-major) in whole chunks, and tiles below 2 GiB.
 template <class TL, bool KM, int NW>
 struct LtDirect {
-  static constexpr int N = TL::SEGS / NW;
+  // where there are fewer 1024-byte pieces than waves, several waves load the same piece
+  static constexpr int N = TL::SEGS >= NW ? TL::SEGS / NW : 1;
+  static_assert(TL::SEGS % NW == 0 || NW % TL::SEGS == 0, "pieces and waves");
+  static __device__ __forceinline__ int seg(int wave, int i) { return TL::SEGS >= NW ? wave + i * NW : wave % TL::SEGS; }
   unsigned off[N];
   __device__ __forceinline__ void init(int64_t ld, int64_t n_lines_or_cols, int wave, int lane) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       int line, c;
-      TL::where((wave + i * NW) * 64 + lane, line, c);
+      TL::where(seg(wave, i) * 64 + lane, line, c);
       const bool ok = KM ? c * TL::CH < n_lines_or_cols : line < n_lines_or_cols;
       off[i] = ok ? (unsigned)(line * ld + c * 16) : 0x80000000u;
     }
@@ -118,14 +126,14 @@ struct LtDirect {
     if (kleft >= TL::BK) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        lt_load_lds16(base, lds + (wave + i * NW) * 1024, off[i]);
+        lt_load_lds16(base, lds + seg(wave, i) * 1024, off[i]);
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         int line, c;
-        TL::where((wave + i * NW) * 64 + lane, line, c);
+        TL::where(seg(wave, i) * 64 + lane, line, c);
         const bool ok = KM ? line < kleft : c * TL::CH < kleft;
-        lt_load_lds16(base, lds + (wave + i * NW) * 1024, ok ? off[i] : 0x80000000u);
+        lt_load_lds16(base, lds + seg(wave, i) * 1024, ok ? off[i] : 0x80000000u);
       }
     }
   }
@@ -251,10 +259,15 @@ __device__ __forceinline__ void lt_tile_store(const LtTileArgs& a, const lt_f32x
   }
 }
 
+// wait for the wave's own loads and LDS reads, then for the other waves
+__device__ __forceinline__ void lt_wait_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+
 template <class T, bool PKM, bool QKM, int BR, int BC, int WR, int WC, bool DIRECT, bool P8, int ACT>
 __global__ __launch_bounds__(64 * WR * WC) void k_dense(LtTileArgs a) {
-  typedef LtTile<T, PKM, BC> TP;
-  typedef LtTile<T, QKM, BR> TQ;
+  constexpr int BKB = 128, NBUF = 2;
+  typedef LtTile<T, PKM, BC, BKB> TP;
+  typedef LtTile<T, QKM, BR, BKB> TQ;
   constexpr int NW = WR * WC, NT = 64 * NW, FR = BR / WR / 16, FC = BC / WC / 16;
   constexpr int BUF = TP::BYTES + TQ::BYTES;
   extern __shared__ __attribute__((aligned(1024))) char s_tile[];
@@ -274,7 +287,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_dense(LtTileArgs a) {
   constexpr int PS = P8 ? 1 : (int)sizeof(T);
   const char* pb = a.P + (PKM ? k0 * a.ldp + (int64_t)col0 * PS : col0 * a.ldp + k0 * PS);
   const char* qb = a.Q + (QKM ? k0 * a.ldq + row0 * (int64_t)sizeof(T) : row0 * a.ldq + k0 * (int64_t)sizeof(T));
-  const int64_t pstep = PKM ? TP::BK * a.ldp : TP::BK * PS, qstep = QKM ? TQ::BK * a.ldq : 128;
+  const int64_t pstep = PKM ? TP::BK * a.ldp : TP::BK * PS, qstep = QKM ? TQ::BK * a.ldq : BKB;
   const int64_t pn = a.cols - col0, qn = a.rows - row0;
   const uint8_t* psc = P8 ? a.ps + k0 * a.ldps : nullptr;
 
@@ -285,19 +298,26 @@ __global__ __launch_bounds__(64 * WR * WC) void k_dense(LtTileArgs a) {
     for (int j = 0; j < FC; ++j) acc[i][j] = (lt_f32x4){0.f, 0.f, 0.f, 0.f};
   const int wr = (wave / WC) * (BR / WR), wc = (wave % WC) * (BC / WC);
 
-  auto compute = [&](const char* buf) {
+  // all of the step's fragments are asked for first, the matrix instructions start with the first that arrive; ahead() =
+  // what else to set going in between
+  auto compute = [&](const char* buf, auto ahead) {
+    constexpr int KK = BKB / 64;
+    typename LtMma<T>::frag p[KK][FC], q[KK][FR];
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      typename LtMma<T>::frag p[FC], q[FR];
+    for (int kk = 0; kk < KK; ++kk) {
 #pragma unroll
-      for (int j = 0; j < FC; ++j) p[j] = TP::frag(buf, wc + 16 * j, kk, lane);
+      for (int j = 0; j < FC; ++j) p[kk][j] = TP::frag(buf, wc + 16 * j, kk, lane);
 #pragma unroll
-      for (int i = 0; i < FR; ++i) q[i] = TQ::frag(buf + TP::BYTES, wr + 16 * i, kk, lane);
+      for (int i = 0; i < FR; ++i) q[kk][i] = TQ::frag(buf + TP::BYTES, wr + 16 * i, kk, lane);
+    }
+    ahead();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
       for (int i = 0; i < FR; ++i)
 #pragma unroll
-        for (int j = 0; j < FC; ++j) acc[i][j] = LtMma<T>::mma(p[j], q[i], acc[i][j]);
-    }
+        for (int j = 0; j < FC; ++j) acc[i][j] = LtMma<T>::mma(p[kk][j], q[kk][i], acc[i][j]);
   };
 
   if constexpr (DIRECT) {
@@ -305,19 +325,19 @@ __global__ __launch_bounds__(64 * WR * WC) void k_dense(LtTileArgs a) {
     LtDirect<TQ, QKM, NW> sq;
     sp.init(a.ldp, pn, wave, lane);
     sq.init(a.ldq, qn, wave, lane);
-    sp.load(pb, s_tile, kend - k0, wave, lane);
-    sq.load(qb, s_tile + TP::BYTES, kend - k0, wave, lane);
+    auto issue = [&](int t) {
+      const int64_t left = kend - k0 - (int64_t)t * TP::BK;
+      char* buf = s_tile + (t % NBUF) * BUF;
+      sp.load(pb + t * pstep, buf, left, wave, lane);
+      sq.load(qb + t * qstep, buf + TP::BYTES, left, wave, lane);
+    };
+    issue(0);
     for (int t = 0; t < nk; ++t) {
-      char* cur = s_tile + (t & 1) * BUF;
-      char* nxt = s_tile + ((t + 1) & 1) * BUF;
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();   // this step's tiles have landed, and nobody reads the other buffer any more
-      if (t + 1 < nk) {
-        const int64_t left = kend - k0 - (int64_t)(t + 1) * TP::BK;
-        sp.load(pb + (t + 1) * pstep, nxt, left, wave, lane);
-        sq.load(qb + (t + 1) * qstep, nxt + TP::BYTES, left, wave, lane);
-      }
-      compute(cur);
+      // this step's tiles have landed, and nobody reads the buffer of step t - 1 any more
+      lt_wait_barrier();
+      compute(s_tile + (t % NBUF) * BUF, [&]() {
+        if (t + 1 < nk) issue(t + 1);
+      });
     }
   } else {
     LtStaged<T, TP, PKM, P8, NT> sp;
@@ -335,11 +355,11 @@ __global__ __launch_bounds__(64 * WR * WC) void k_dense(LtTileArgs a) {
         sp.load(pb + (t + 1) * pstep, a.ldp, pn, left, psc, a.ldps, col0, tid);
         sq.load(qb + (t + 1) * qstep, a.ldq, qn, left, nullptr, 0, 0, tid);
       }
-      compute(cur);
+      compute(cur, [] {});
     }
   }
 
-  static_assert(NW * LtTurn<FC>::BYTES <= 2 * BUF, "the turned rows do not fit the tiles' LDS");
+  static_assert(NW * LtTurn<FC>::BYTES <= NBUF * BUF, "the turned rows do not fit the tiles' LDS");
   __syncthreads();
   lt_tile_store<T, FR, FC, ACT>(a, acc, split, row0 + wr, col0 + wc, lane,
                                 reinterpret_cast<float*>(s_tile + wave * LtTurn<FC>::BYTES));
@@ -493,7 +513,12 @@ static inline LtPlan lt_gemm_plan(int64_t rows, int cols, int64_t depth, int dt,
   const int bk = dt == LT_DT_F32 ? 32 : 64;
   auto tiles = [&](int br, int bc) { return ((rows + br - 1) / br) * ((cols + bc - 1) / bc); };
   int br, bc;
-  if (direct && dt != LT_DT_F32 && cols >= 192 && tiles(256, 256) >= 192) p.tile = LT_TILE_256x256, br = 256, bc = 256;
+  // the widest tile needs the fewest operand bytes a product, and one workgroup a CU: 192 of them, or fewer whose k is long
+  // enough to be split into at least 32 steps each (training 16384 x 1024 -> 4096, bf16:
+  // its dW on 128 x 128 tiles 618 us a step, on 256 x 256 tiles split four ways 554 us)
+  const int64_t t256 = tiles(256, 256);
+  const bool wide = direct && dt != LT_DT_F32 && cols >= 192 && rows >= 192;
+  if (wide && (t256 >= 192 || (t256 >= 16 && depth >= 64 * 32 * (256 / t256)))) p.tile = LT_TILE_256x256, br = 256, bc = 256;
   else if (cols <= 32 && direct) p.tile = LT_TILE_256x32, br = 256, bc = 32;
   else if (cols <= 64 && direct) p.tile = LT_TILE_128x64, br = 128, bc = 64;
   else if (tiles(128, 128) >= 128 || rows * (int64_t)cols >= 128 * 128 * 32) p.tile = LT_TILE_128x128, br = 128, bc = 128;
@@ -502,8 +527,8 @@ static inline LtPlan lt_gemm_plan(int64_t rows, int cols, int64_t depth, int dt,
   p.tc = (cols + bc - 1) / bc;
   // fewer tiles than the chip runs at once: split k, at least four steps each
   const int64_t t = (int64_t)p.tr * p.tc, steps = (depth + bk - 1) / bk;
-  if (p.tile != LT_TILE_256x256 && t < 256) {
-    int64_t s = (512 + t - 1) / t;
+  if (t < (p.tile == LT_TILE_256x256 ? 192 : 256)) {
+    int64_t s = p.tile == LT_TILE_256x256 ? 256 / t : (512 + t - 1) / t;
     if (s > steps / 4) s = steps / 4;
     if (s > 256) s = 256;
     if (s > 1) {
@@ -520,7 +545,11 @@ template <class T> int lt_gemm_launch(const LtGemm& g, const LtPlan& p, float* p
 
 template <class T, bool PKM, bool QKM, int BR, int BC, int WR, int WC, bool DIRECT, bool P8, int ACT>
 static int lt_launch_tile(const LtTileArgs& a, hipStream_t stream) {
-  const int smem = 2 * (BR + BC) * 128;
+  // a single step needs one buffer: more workgroups a CU (310017 x 32 -> 256 fp32: 196 -> 178 us)
+  const bool one = a.slice <= 128 / (int64_t)sizeof(T);
+  const int need = WR * WC * LtTurn<BC / WC / 16>::BYTES;
+  int smem = (one ? 1 : 2) * (BR + BC) * 128;
+  if (smem < need) smem = need;
   if (smem > 65536)
     LT_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_dense<T, PKM, QKM, BR, BC, WR, WC, DIRECT, P8, ACT>),
                                      hipFuncAttributeMaxDynamicSharedMemorySize, smem));
