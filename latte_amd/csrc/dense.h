@@ -195,16 +195,18 @@ struct LtEpi {
 
 // eight neighbours (row, col..col+7) of the product, n of which exist (<= 0: nothing to do), with their residual (loaded
 // ahead: the stores in between would hold the loads back)
-template <class T>
+// EVEN: n is 8 or more, or 0 and less -- straight-line code, no element by element ends
+template <class T, bool EVEN>
 __device__ __forceinline__ void lt_epi_res(const LtEpi& e, int64_t row, int col, int n, float (&r)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) r[i] = 0.f;
-  if (e.res && n > 0) lt_ldv<T, 8>((const T*)e.res + row * e.ldres + col, n, r);
+  if (e.res && n > 0) lt_ldv<T, 8>((const T*)e.res + row * e.ldres + col, EVEN ? 8 : n, r);
 }
-template <class T, int ACT>
+template <class T, int ACT, bool EVEN>
 __device__ __forceinline__ void lt_epi8(const LtEpi& e, const float (&z)[8], const float (&b)[8], const float (&r)[8], int64_t row,
-                                        int col, int n) {
-  if (n <= 0) return;
+                                        int col, int n_) {
+  if (n_ <= 0) return;
+  const int n = EVEN ? 8 : n_;
   float y[8], d[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) lt_act<ACT, sizeof(T) == 2>(z[i] + b[i], y[i], d[i]);

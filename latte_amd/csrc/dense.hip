@@ -7,11 +7,14 @@
 //
 // Replaces the library products of nn.Linear (point branches and heads: latte/models/spvcnn.py:95-111,
 // latte/models/xmuda_arch.py:326-335) where a layer trains or keeps its activations in 8 bits.
-#include "dense_gemm.h"
+#include "dense_plan.h"
 
 template <> int lt_gemm_launch<float>(const LtGemm&, const LtPlan&, float*, hipStream_t);
 template <> int lt_gemm_launch<lt_bf16>(const LtGemm&, const LtPlan&, float*, hipStream_t);
 template <> int lt_gemm_launch<lt_f16>(const LtGemm&, const LtPlan&, float*, hipStream_t);
+template <> int lt_rows_bwd_launch<float>(const LtRowsBwdArgs&, const LtRowsBwdPlan&, hipStream_t);
+template <> int lt_rows_bwd_launch<lt_bf16>(const LtRowsBwdArgs&, const LtRowsBwdPlan&, hipStream_t);
+template <> int lt_rows_bwd_launch<lt_f16>(const LtRowsBwdArgs&, const LtRowsBwdPlan&, hipStream_t);
 
 static int64_t part_bytes(const LtPlan& p, int64_t rows, int cols) {
   return p.splits > 1 ? lt_align_up(p.splits * rows * cols * 4, 256) : 0;
@@ -255,6 +258,7 @@ static bool widen_first(int64_t M, int K, int N) { return N > 256 && M > 0; }
 struct BwdWs {
   int64_t dz, part, wide, gemm, bytes;
 };
+// the larger of the two routes: one pass over the rows, or dz and two products
 static BwdWs bwd_ws(int64_t M, int K, int N, int dt, bool x8) {
   BwdWs w;
   int64_t off = 0;
@@ -267,7 +271,9 @@ static BwdWs bwd_ws(int64_t M, int K, int N, int dt, bool x8) {
   w.gemm = off;
   const int64_t a = gemm_ws_bytes(M, K, N, dt, false), b = gemm_ws_bytes(N, K, M, dt, false);
   off += a > b ? a : b;
-  w.bytes = off;
+  const LtRowsBwdPlan p = lt_rows_bwd_plan(M, K, N, dt);
+  const int64_t rows = p.ok ? lt_align_up((int64_t)p.grid * N * K * 4, 256) + (int64_t)p.grid * N * 4 : 0;
+  w.bytes = off > rows ? off : rows;
   return w;
 }
 
@@ -290,6 +296,25 @@ extern "C" int lt_linear_bwd(const void* dy, int64_t lddy, const void* x, int64_
   LtOnStream on;
   if ((rc = on.enter(stream))) return rc;
   char* wsb = (char*)ws;
+  const LtRowsBwdPlan rp = lt_rows_bwd_plan(M, K, N, dt);
+  if (rp.ok) {   // whichever gradients are asked for: each has the same bits alone as with the others
+    float* part_w = (float*)wsb;
+    float* part_b = (float*)(wsb + lt_align_up((int64_t)rp.grid * N * K * 4, 256));
+    const LtRowsBwdArgs a = {dy, x, (const uint8_t*)x_scales, w, deriv, lddy, ldx, ldw, deriv_kind, M, N, K, dx, dw ? part_w : nullptr,
+                             db ? part_b : nullptr, rp.tiles};
+    LT_DENSE_TYPES(dt, rc = lt_rows_bwd_launch<T>(a, rp, stream));
+    if (rc) return rc;
+    if (dw) {
+      const LtEpi e = {nullptr, nullptr, 0, dw, K, nullptr, LT_DERIV_NONE, N, K};
+      LT_DENSE_TYPES(dt, rc = lt_launch_join<T, LT_ACT_NONE>(e, part_w, rp.grid, stream));
+      if (rc) return rc;
+    }
+    if (db) {
+      LT_DENSE_TYPES(dt, hipLaunchKernelGGL((k_col_join<T>), dim3((N + 15) / 16), dim3(256), 0, stream, part_b, rp.grid, N, (T*)db));
+      LT_LAUNCH_CHECK();
+    }
+    return LT_OK;
+  }
   const void* dz = dy;
   int64_t lddz = lddy;
   if (deriv_kind != LT_DERIV_NONE) {

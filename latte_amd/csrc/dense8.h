@@ -9,7 +9,7 @@
 // of the group's largest (measured), and goes on in fp32.  That is the price of the 8-bit rate (twice the 16-bit one); the
 // operands were rounded to within 2^-4, and widening them to bf16 instead would keep every product whole at half the rate.
 #pragma once
-#include "dense_gemm.h"
+#include "dense_plan.h"
 
 struct LtTile8Args {
   LtTileArgs t;

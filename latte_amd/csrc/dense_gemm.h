@@ -213,9 +213,9 @@ __device__ __forceinline__ unsigned lt_xcd_map(unsigned b, unsigned n) {
 // LDS (the tiles are no longer read).  A lane's four columns of one row would make stores of 16 bytes a row and line, so 16
 // rows at a time turn through LDS and leave eight columns a lane: whole 128-byte lines of 16-bit results.
 template <int FC> struct LtTurn { static constexpr int LD = 16 * FC + 4, BYTES = 16 * LD * 4; };
-template <class T, int FR, int FC, int ACT>
-__device__ __forceinline__ void lt_tile_store(const LtTileArgs& a, const lt_f32x4 (&acc)[FR][FC], unsigned split, int64_t row0, int col0,
-                                              int lane, float* s) {
+template <class T, int FR, int FC, int ACT, bool EVEN>
+__device__ __forceinline__ void lt_tile_store_(const LtTileArgs& a, const lt_f32x4 (&acc)[FR][FC], unsigned split, int64_t row0, int col0,
+                                               int lane, float* s) {
   constexpr int LD = LtTurn<FC>::LD, LPR = FC * 2, RPP = 64 / LPR < 16 ? 64 / LPR : 16, PASS = 16 / RPP;   // lanes a row, rows a pass
   const int r = lane & 15, g = lane >> 4;
   const int pr = lane / LPR, col = col0 + (lane % LPR) * 8;
@@ -224,7 +224,7 @@ __device__ __forceinline__ void lt_tile_store(const LtTileArgs& a, const lt_f32x
   float b[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) b[i] = 0.f;
-  if (a.splits == 1 && a.epi.bias) lt_ldv<T, 8>((const T*)a.epi.bias + col, nc, b);
+  if (a.splits == 1 && a.epi.bias && nc > 0) lt_ldv<T, 8>((const T*)a.epi.bias + col, EVEN ? 8 : nc, b);
 #pragma unroll
   for (int i = 0; i < FR; ++i) {
     float res[PASS][8];
@@ -232,7 +232,7 @@ __device__ __forceinline__ void lt_tile_store(const LtTileArgs& a, const lt_f32x
 #pragma unroll
       for (int p = 0; p < PASS; ++p) {
         const int64_t row = row0 + 16 * i + p * RPP + pr;
-        lt_epi_res<T>(a.epi, row, col, row < a.rows ? (int)nc : 0, res[p]);
+        lt_epi_res<T, EVEN>(a.epi, row, col, row < a.rows ? (int)nc : 0, res[p]);
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the rows before have been read
@@ -251,9 +251,9 @@ __device__ __forceinline__ void lt_tile_store(const LtTileArgs& a, const lt_f32x
         for (int t = 0; t < 4; ++t) z[t] = u[t], z[4 + t] = v[t];
       }
       if (a.splits > 1) {
-        if (n > 0) lt_stv<float, 8>(a.part + ((int64_t)split * a.rows + row) * a.cols + col, n, z);
+        if (n > 0) lt_stv<float, 8>(a.part + ((int64_t)split * a.rows + row) * a.cols + col, EVEN ? 8 : n, z);
       } else {
-        lt_epi8<T, ACT>(a.epi, z, b, res[p], row, col, n);
+        lt_epi8<T, ACT, EVEN>(a.epi, z, b, res[p], row, col, n);
       }
     }
   }
@@ -262,6 +262,13 @@ __device__ __forceinline__ void lt_tile_store(const LtTileArgs& a, const lt_f32x
 // wait for the wave's own loads and LDS reads, then for the other waves
 __device__ __forceinline__ void lt_wait_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+
+template <class T, int FR, int FC, int ACT>
+__device__ __forceinline__ void lt_tile_store(const LtTileArgs& a, const lt_f32x4 (&acc)[FR][FC], unsigned split, int64_t row0, int col0,
+                                              int lane, float* s) {
+  if (a.cols % 8 == 0) lt_tile_store_<T, FR, FC, ACT, true>(a, acc, split, row0, col0, lane, s);
+  else lt_tile_store_<T, FR, FC, ACT, false>(a, acc, split, row0, col0, lane, s);
+}
 
 template <class T, bool PKM, bool QKM, int BR, int BC, int WR, int WC, bool DIRECT, bool P8, int ACT>
 __global__ __launch_bounds__(64 * WR * WC) void k_dense(LtTileArgs a) {
@@ -410,8 +417,8 @@ __global__ __launch_bounds__(256) void k_dense_join(const float* __restrict__ pa
 #pragma unroll
     for (int t = 0; t < 8; ++t) bias[t] = 0.f;
     if (e.bias) lt_ldv<T, 8>((const T*)e.bias + col, m, bias);
-    lt_epi_res<T>(e, row, col, m, res);
-    lt_epi8<T, ACT>(e, acc, bias, res, row, col, m);
+    lt_epi_res<T, false>(e, row, col, m, res);
+    lt_epi8<T, ACT, false>(e, acc, bias, res, row, col, m);
   }
 }
 
@@ -442,8 +449,8 @@ __device__ __forceinline__ void lt_few_store(const LtTileArgs& a, const lt_f32x4
 #pragma unroll
   for (int i = 0; i < 8; ++i) b[i] = 0.f;
   if (a.epi.bias) lt_ldv<T, 8>((const T*)a.epi.bias + col, n, b);
-  lt_epi_res<T>(a.epi, row, col, n, res);
-  lt_epi8<T, ACT>(a.epi, z, b, res, row, col, n);
+  lt_epi_res<T, false>(a.epi, row, col, n, res);
+  lt_epi8<T, ACT, false>(a.epi, z, b, res, row, col, n);
 }
 
 // ---- few rows: y[rows <= 64][cols].  Bound by reading P once: a workgroup takes 16 columns, its 8 waves share k in
@@ -490,157 +497,4 @@ __global__ __launch_bounds__(512) void k_dense_few(LtTileArgs a) {
       for (int f = 0; f < FR; ++f) acc[f] = LtMma<T>::mma(pf[u], qf[f][u], acc[f]);
   }
   lt_few_store<T, FR, ACT>(a, acc, s_acc, col0, wave, lane);
-}
-
-// ---- host: which kernel, which tile, how many splits
-// tile shapes (rows x columns of the output)
-enum { LT_TILE_256x256, LT_TILE_128x128, LT_TILE_128x64, LT_TILE_256x32, LT_TILE_64x64 };
-
-struct LtPlan {
-  int tile, tr, tc, splits;
-  int64_t slice;
-  bool few, direct;
-};
-
-static inline LtPlan lt_gemm_plan(int64_t rows, int cols, int64_t depth, int dt, bool nn, bool direct, bool few_ok) {
-  LtPlan p = {};
-  p.direct = direct;
-  p.splits = 1;
-  p.slice = depth;
-  // up to 64 rows the tile kernels would leave most of a tile idle; both operands must run along k
-  p.few = few_ok && nn && rows <= 64;
-  if (p.few || rows <= 0 || depth <= 0) return p;
-  const int bk = dt == LT_DT_F32 ? 32 : 64;
-  auto tiles = [&](int br, int bc) { return ((rows + br - 1) / br) * ((cols + bc - 1) / bc); };
-  int br, bc;
-  // the widest tile needs the fewest operand bytes a product, and one workgroup a CU: 192 of them, or fewer whose k is long
-  // enough to be split into at least 32 steps each (training 16384 x 1024 -> 4096, bf16:
-  // its dW on 128 x 128 tiles 618 us a step, on 256 x 256 tiles split four ways 554 us)
-  const int64_t t256 = tiles(256, 256);
-  const bool wide = direct && dt != LT_DT_F32 && cols >= 192 && rows >= 192;
-  if (wide && (t256 >= 192 || (t256 >= 16 && depth >= 64 * 32 * (256 / t256)))) p.tile = LT_TILE_256x256, br = 256, bc = 256;
-  else if (cols <= 32 && direct) p.tile = LT_TILE_256x32, br = 256, bc = 32;
-  else if (cols <= 64 && direct) p.tile = LT_TILE_128x64, br = 128, bc = 64;
-  else if (tiles(128, 128) >= 128 || rows * (int64_t)cols >= 128 * 128 * 32) p.tile = LT_TILE_128x128, br = 128, bc = 128;
-  else p.tile = LT_TILE_64x64, br = 64, bc = 64;
-  p.tr = (int)((rows + br - 1) / br);
-  p.tc = (cols + bc - 1) / bc;
-  // fewer tiles than the chip runs at once: split k, at least four steps each
-  const int64_t t = (int64_t)p.tr * p.tc, steps = (depth + bk - 1) / bk;
-  if (t < (p.tile == LT_TILE_256x256 ? 192 : 256)) {
-    int64_t s = p.tile == LT_TILE_256x256 ? 256 / t : (512 + t - 1) / t;
-    if (s > steps / 4) s = steps / 4;
-    if (s > 256) s = 256;
-    if (s > 1) {
-      const int64_t per = (steps + s - 1) / s;
-      p.slice = per * bk;
-      p.splits = (int)((steps + per - 1) / per);
-    }
-  }
-  return p;
-}
-
-// the launches for one value type (dense_f32.hip, dense_bf16.hip, dense_f16.hip)
-template <class T> int lt_gemm_launch(const LtGemm& g, const LtPlan& p, float* part, hipStream_t stream);
-
-template <class T, bool PKM, bool QKM, int BR, int BC, int WR, int WC, bool DIRECT, bool P8, int ACT>
-static int lt_launch_tile(const LtTileArgs& a, hipStream_t stream) {
-  // a single step needs one buffer: more workgroups a CU (310017 x 32 -> 256 fp32: 196 -> 178 us)
-  const bool one = a.slice <= 128 / (int64_t)sizeof(T);
-  const int need = WR * WC * LtTurn<BC / WC / 16>::BYTES;
-  int smem = (one ? 1 : 2) * (BR + BC) * 128;
-  if (smem < need) smem = need;
-  if (smem > 65536)
-    LT_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_dense<T, PKM, QKM, BR, BC, WR, WC, DIRECT, P8, ACT>),
-                                     hipFuncAttributeMaxDynamicSharedMemorySize, smem));
-  hipLaunchKernelGGL((k_dense<T, PKM, QKM, BR, BC, WR, WC, DIRECT, P8, ACT>), dim3((unsigned)a.tr * a.tc * a.splits),
-                     dim3(64 * WR * WC), smem, stream, a);
-  LT_LAUNCH_CHECK();
-  return LT_OK;
-}
-
-template <class T, bool PKM, bool QKM, int ACT>
-static int lt_launch_shape(const LtPlan& p, const LtTileArgs& a, bool p8, hipStream_t stream) {
-  if constexpr (PKM && QKM) {
-    if (p8) {
-      if (p.tile == LT_TILE_128x128) return lt_launch_tile<T, true, true, 128, 128, 2, 2, false, true, LT_ACT_NONE>(a, stream);
-      return lt_launch_tile<T, true, true, 64, 64, 2, 2, false, true, LT_ACT_NONE>(a, stream);
-    }
-  }
-  if (p.direct) {
-    switch (p.tile) {
-      case LT_TILE_256x256:
-        if constexpr (sizeof(T) == 2) return lt_launch_tile<T, PKM, QKM, 256, 256, 2, 4, true, false, ACT>(a, stream);
-        break;
-      case LT_TILE_128x128: return lt_launch_tile<T, PKM, QKM, 128, 128, 2, 2, true, false, ACT>(a, stream);
-      case LT_TILE_128x64: return lt_launch_tile<T, PKM, QKM, 128, 64, 2, 2, true, false, ACT>(a, stream);
-      case LT_TILE_256x32: return lt_launch_tile<T, PKM, QKM, 256, 32, 4, 1, true, false, ACT>(a, stream);
-      default: return lt_launch_tile<T, PKM, QKM, 64, 64, 2, 2, true, false, ACT>(a, stream);
-    }
-  }
-  if (p.tile == LT_TILE_128x128) return lt_launch_tile<T, PKM, QKM, 128, 128, 2, 2, false, false, ACT>(a, stream);
-  return lt_launch_tile<T, PKM, QKM, 64, 64, 2, 2, false, false, ACT>(a, stream);
-}
-
-template <class T, int ACT>
-static int lt_launch_few(const LtTileArgs& a, hipStream_t stream) {
-  const dim3 grid((a.cols + 15) / 16), block(512);
-  const int fr = (int)((a.rows + 15) / 16);
-  if (fr == 1) hipLaunchKernelGGL((k_dense_few<T, 1, ACT>), grid, block, 0, stream, a);
-  else if (fr == 2) hipLaunchKernelGGL((k_dense_few<T, 2, ACT>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((k_dense_few<T, 4, ACT>), grid, block, 0, stream, a);
-  LT_LAUNCH_CHECK();
-  return LT_OK;
-}
-
-template <class T, int ACT>
-static int lt_launch_join(const LtEpi& e, const float* part, int splits, hipStream_t stream) {
-  const int64_t n = e.rows * (int64_t)((e.cols + 7) >> 3);
-  if (splits >= 64) hipLaunchKernelGGL((k_dense_join<T, ACT, 16>), dim3(lt_grid(n, 16)), dim3(256), 0, stream, part, splits, e);
-  else if (splits >= 8) hipLaunchKernelGGL((k_dense_join<T, ACT, 4>), dim3(lt_grid(n, 64)), dim3(256), 0, stream, part, splits, e);
-  else hipLaunchKernelGGL((k_dense_join<T, ACT, 1>), dim3(lt_grid(n, 256)), dim3(256), 0, stream, part, splits, e);
-  LT_LAUNCH_CHECK();
-  return LT_OK;
-}
-
-template <class T, int ACT>
-static int lt_gemm_launch_act(const LtGemm& g, const LtPlan& p, const LtTileArgs& a, float* part, hipStream_t stream) {
-  int rc = LT_OK;
-  if (g.depth > 0) {
-    if (p.few) return lt_launch_few<T, ACT>(a, stream);
-    if (!g.p_kmajor) rc = lt_launch_shape<T, false, false, ACT>(p, a, false, stream);
-    else if constexpr (ACT == LT_ACT_NONE) {
-      if (!g.q_kmajor) rc = lt_launch_shape<T, true, false, ACT>(p, a, false, stream);
-      else rc = lt_launch_shape<T, true, true, ACT>(p, a, g.p_scales != nullptr, stream);
-    }
-    if (rc) return rc;
-    if (p.splits == 1) return LT_OK;
-  }
-  return lt_launch_join<T, ACT>(g.epi, part, g.depth > 0 ? p.splits : 0, stream);   // no k at all: the sum is zero
-}
-
-template <class T>
-static int lt_gemm_launch_impl(const LtGemm& g, const LtPlan& p, float* part, hipStream_t stream) {
-  LtTileArgs a = {};
-  a.P = (const char*)g.P;
-  a.Q = (const char*)g.Q;
-  a.ldp = g.ldp * (g.p_scales ? 1 : (int64_t)sizeof(T));
-  a.ldq = g.ldq * (int64_t)sizeof(T);
-  a.rows = g.rows;
-  a.depth = g.depth;
-  a.cols = g.cols;
-  a.tr = p.tr;
-  a.tc = p.tc;
-  a.splits = p.splits;
-  a.slice = p.slice;
-  a.part = part;
-  a.ps = g.p_scales;
-  a.ldps = (g.cols + 31) / 32;
-  a.epi = g.epi;
-  switch (g.act) {
-    case LT_ACT_RELU: return lt_gemm_launch_act<T, LT_ACT_RELU>(g, p, a, part, stream);
-    case LT_ACT_GELU: return lt_gemm_launch_act<T, LT_ACT_GELU>(g, p, a, part, stream);
-    case LT_ACT_SILU: return lt_gemm_launch_act<T, LT_ACT_SILU>(g, p, a, part, stream);
-    default: return lt_gemm_launch_act<T, LT_ACT_NONE>(g, p, a, part, stream);
-  }
 }

@@ -293,3 +293,19 @@ def test_linear_on_another_stream_matches():
         got = LF.linear(x, w, b, act="gelu", residual=r)
     torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(got, want)
+
+
+ROWS = [(8192, 32, 256), (8200, 128, 96), (9001, 96, 20), (8193, 256, 64), (2048, 64, 64), (2049, 33, 65), (3000, 130, 100), (2500, 256, 128),
+        (2100, 100, 256), (20000, 17, 5), (8197, 250, 31)]
+
+
+@pytest.mark.parametrize("ckpt", [None, "mx8"])
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("size", ROWS, ids=str)
+def test_linear_long_and_narrow(size, dt, ckpt):
+    """the one-pass kernels over many rows, with odd widths and a cut last tile"""
+    x, w, b, r, dy = _inputs(*size, dt, seed=11, exact=True)
+    _check_linear(x, w, b, r, dy, "relu", ckpt)
+    x, w, b, r, dy = _inputs(*size, dt, seed=12)
+    _check_linear(x, w, b, None, dy, "silu", ckpt)
+    _check_linear(x[:, 1:], w[:, 1:], None, r, dy, "none", ckpt) if size[1] > 1 else None
