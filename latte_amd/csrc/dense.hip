@@ -47,7 +47,7 @@ static int gemm_run(const LtGemm& g, void* ws, int64_t ws_bytes, hipStream_t str
 // four columns, a workgroup a slab of rows; the slabs' sums are joined in a fixed order by k_col_join.
 template <class T, int DK>
 __global__ __launch_bounds__(256) void k_dz(const T* __restrict__ dy, int64_t lddy, const void* __restrict__ deriv, int64_t M,
-                                            int N, int tx, int64_t rows_per, T* __restrict__ dz, float* __restrict__ part) {
+                                            int N, int tx, int64_t rows_per, T* __restrict__ dz, float* __restrict__ part, T* __restrict__ db) {
   __shared__ lt_f32x4 s_sum[256];
   const int x = threadIdx.x % tx, yy = threadIdx.x / tx, ty = 256 / tx;
   const int col = (blockIdx.x * tx + x) * 4;
@@ -96,7 +96,8 @@ __global__ __launch_bounds__(256) void k_dz(const T* __restrict__ dy, int64_t ld
   if (yy == 0 && n > 0) {
     for (int j = 1; j < ty; ++j) sum += s_sum[j * tx + x];
     const float v[4] = {sum[0], sum[1], sum[2], sum[3]};
-    lt_stv<float, 4>(part + (int64_t)blockIdx.y * N + col, n, v);
+    if (gridDim.y == 1) lt_stv<T, 4>(db + col, n, v);   // one slab: the sums are db
+    else lt_stv<float, 4>(part + (int64_t)blockIdx.y * N + col, n, v);
   }
 }
 
@@ -128,14 +129,14 @@ static int dz_run(const void* dy, int64_t lddy, const void* deriv, int dkind, in
     const dim3 grid(p.gx, p.slabs), block(256);
     const T* g = (const T*)dy;
     switch (dkind) {
-      case LT_DERIV_BITS: hipLaunchKernelGGL((k_dz<T, LT_DERIV_BITS>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, part); break;
-      case LT_DERIV_BYTE: hipLaunchKernelGGL((k_dz<T, LT_DERIV_BYTE>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, part); break;
-      case LT_DERIV_FULL: hipLaunchKernelGGL((k_dz<T, LT_DERIV_FULL>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, part); break;
-      default: hipLaunchKernelGGL((k_dz<T, LT_DERIV_NONE>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, part); break;
+      case LT_DERIV_BITS: hipLaunchKernelGGL((k_dz<T, LT_DERIV_BITS>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, part, (T*)db); break;
+      case LT_DERIV_BYTE: hipLaunchKernelGGL((k_dz<T, LT_DERIV_BYTE>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, part, (T*)db); break;
+      case LT_DERIV_FULL: hipLaunchKernelGGL((k_dz<T, LT_DERIV_FULL>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, part, (T*)db); break;
+      default: hipLaunchKernelGGL((k_dz<T, LT_DERIV_NONE>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, part, (T*)db); break;
     }
     LT_LAUNCH_CHECK();
   }
-  if (db) {
+  if (db && p.slabs != 1) {
     hipLaunchKernelGGL((k_col_join<T>), dim3((N + 15) / 16), dim3(256), 0, stream, part, p.slabs, N, (T*)db);
     LT_LAUNCH_CHECK();
   }

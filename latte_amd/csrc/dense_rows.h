@@ -86,19 +86,19 @@ struct LtRowsBwd {
   static constexpr int CH = 16 / sizeof(T), BKB = 32 * sizeof(T);   // 32 rows of a tile are 32 k of dW's product
   typedef LtTile<T, true, NP, BKB> TZ;
   typedef LtTile<T, true, KP, BKB> TX;
-  static constexpr int NZ = TZ::BYTES / 16 / 512 > 0 ? TZ::BYTES / 16 / 512 : 1, NX = TX::BYTES / 16 / 512 > 0 ? TX::BYTES / 16 / 512 : 1;
-  static constexpr int WK = KP >= NP ? 4 : 2, WN = 8 / WK;          // the waves' grid over dW
-  static constexpr int TN = NP / 16 / WN, TK = KP / 16 / WK;        // its 16 x 16 tiles a wave
-  static constexpr int FX = KP / 64;                                // dx: 2 strips x 4 column groups of FX tiles
+  static constexpr int NT = 1024;   // 16 waves: with 8 the LDS latencies showed (@RB8@)
+  static constexpr int NZ = (TZ::BYTES / 16 + NT - 1) / NT, NX = (TX::BYTES / 16 + NT - 1) / NT;
+  static constexpr int TN = NP / 64, TK = KP / 64;                  // the waves' 4 x 4 grid over dW: 16 x 16 tiles a wave
+  static constexpr int FX = KP > 128 ? KP / 128 : 1;                // dx: 2 strips x 8 column groups of FX tiles
   static constexpr int BUF = TZ::BYTES + TX::BYTES;
   static int lds(int N, int K) {
     const int nf = (N + 4 * CH - 1) / (4 * CH), kt = (K + 15) / 16;
-    return 2 * BUF + nf * kt * 1024 + 8 * LtTurn<FX>::BYTES;
+    return 2 * BUF + nf * kt * 1024 + NT / 64 * LtTurn<FX>::BYTES;
   }
 };
 
 template <class T, int NP, int KP>
-__global__ __launch_bounds__(512) void k_rows_bwd(LtRowsBwdArgs a) {
+__global__ __launch_bounds__(1024) void k_rows_bwd(LtRowsBwdArgs a) {
   typedef LtRowsBwd<T, NP, KP> S;
   typedef typename S::TZ TZ;
   typedef typename S::TX TX;
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(512) void k_rows_bwd(LtRowsBwdArgs a) {
   float* turn = reinterpret_cast<float*>(s_w + nf * kt * 1024 + wave * LtTurn<S::FX>::BYTES);
   // W for dx: fragment (f, c): lane (r, g) holds column 16 c + r of W, rows f KF + g CH ..
   if (a.dx) {
-    for (int i = tid; i < nf * kt * 64; i += 512) {
+    for (int i = tid; i < nf * kt * 64; i += S::NT) {
       const int l = i & 63, c = (i >> 6) % kt, f = (i >> 6) / kt, k = 16 * c + (l & 15), n0 = f * KF + (l >> 4) * CH;
       Frag v;
 #pragma unroll
@@ -139,7 +139,7 @@ __global__ __launch_bounds__(512) void k_rows_bwd(LtRowsBwdArgs a) {
 #pragma unroll
     for (int i = 0; i < S::NZ; ++i) {
       int line, c;
-      TZ::where(tid + i * 512, line, c);
+      TZ::where(tid + i * S::NT, line, c);
       const int64_t row = m0 + line < a.M ? m0 + line : a.M - 1;   // what does not exist is read elsewhere and cleared in put()
       const int col = c * CH < N ? c * CH : 0;
       __builtin_memcpy(&gz[i], (const T*)a.dy + row * a.lddy + col, 16);
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(512) void k_rows_bwd(LtRowsBwdArgs a) {
 #pragma unroll
     for (int i = 0; i < S::NX; ++i) {
       int line, c;
-      TX::where(tid + i * 512, line, c);
+      TX::where(tid + i * S::NT, line, c);
       const int64_t row = m0 + line < a.M ? m0 + line : a.M - 1;
       const int col = c * CH < K ? c * CH : 0;
       if (a.xs) {
@@ -166,7 +166,7 @@ __global__ __launch_bounds__(512) void k_rows_bwd(LtRowsBwdArgs a) {
 #pragma unroll
     for (int i = 0; i < S::NZ; ++i) {
       int line, c;
-      TZ::where(tid + i * 512, line, c);
+      TZ::where(tid + i * S::NT, line, c);
       const bool ok = line < 32 && m0 + line < a.M && c * CH < N;
       T t[CH], y[CH];
       __builtin_memcpy(y, &gz[i], 16);
@@ -193,13 +193,13 @@ __global__ __launch_bounds__(512) void k_rows_bwd(LtRowsBwdArgs a) {
         db[i][j] += z[j];
         t[j] = (T)z[j];
       }
-      if (tid + i * 512 < TZ::BYTES / 16) __builtin_memcpy(buf + (tid + i * 512) * 16, t, 16);
+      if (tid + i * S::NT < TZ::BYTES / 16) __builtin_memcpy(buf + (tid + i * S::NT) * 16, t, 16);
     }
     if (!a.dw) return;
 #pragma unroll
     for (int i = 0; i < S::NX; ++i) {
       int line, c;
-      TX::where(tid + i * 512, line, c);
+      TX::where(tid + i * S::NT, line, c);
       const bool ok = line < 32 && m0 + line < a.M && c * CH < K;
       lt_i32x4 v = gx[i];
       if (a.xs) {
@@ -217,7 +217,7 @@ __global__ __launch_bounds__(512) void k_rows_bwd(LtRowsBwdArgs a) {
         __builtin_memcpy(&v, t, 16);
       }
       if (!ok) v = (lt_i32x4){0, 0, 0, 0};
-      if (tid + i * 512 < TX::BYTES / 16) *reinterpret_cast<lt_i32x4*>(buf + TZ::BYTES + (tid + i * 512) * 16) = v;
+      if (tid + i * S::NT < TX::BYTES / 16) *reinterpret_cast<lt_i32x4*>(buf + TZ::BYTES + (tid + i * S::NT) * 16) = v;
     }
   };
 
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(512) void k_rows_bwd(LtRowsBwdArgs a) {
   e.splits = 1;
   e.epi = LtEpi{nullptr, nullptr, 0, a.dx, K, nullptr, LT_DERIV_NONE, a.M, K};
   const int strip = wave & 1, xg = wave >> 1;          // dx: rows 16 strip .., columns 16 FX xg ..
-  const int wn = (wave / S::WK) * S::TN, wk = (wave % S::WK) * S::TK;
+  const int wn = (wave >> 2) * S::TN, wk = (wave & 3) * S::TK;
   int64_t t = blockIdx.x;
   if (t < a.tiles) fetch(t * 32);
   for (int b = 0; t < a.tiles; t += gridDim.x, b ^= 1) {
@@ -240,6 +240,7 @@ __global__ __launch_bounds__(512) void k_rows_bwd(LtRowsBwdArgs a) {
 #pragma unroll
       for (int j = 0; j < S::FX; ++j) acc[0][j] = (lt_f32x4){0.f, 0.f, 0.f, 0.f};
       const int m = 16 * strip + r;
+#pragma unroll 2
       for (int f = 0; f < nf; ++f) {
         const int c = f * 4 + g;                       // chunk of CH columns n of row m
         const Frag q = *reinterpret_cast<const Frag*>(buf + m * (NP * (int)sizeof(T)) + ((c ^ TZ::kswz(m)) << 4));
@@ -282,13 +283,13 @@ __global__ __launch_bounds__(512) void k_rows_bwd(LtRowsBwdArgs a) {
 #pragma unroll
   for (int i = 0; i < S::NZ; ++i) {
     int line, c;
-    TZ::where(tid + i * 512, line, c);
+    TZ::where(tid + i * S::NT, line, c);
     if (line < 32)
 #pragma unroll
       for (int j = 0; j < CH; ++j) s_db[line * NP + c * CH + j] = db[i][j];
   }
   __syncthreads();
-  for (int n = tid; n < N; n += 512) {
+  for (int n = tid; n < N; n += S::NT) {
     float s = 0.f;
 #pragma unroll 8
     for (int l = 0; l < 32; ++l) s += s_db[l * NP + n];
@@ -352,7 +353,7 @@ static inline LtRowsBwdPlan lt_rows_bwd_plan(int64_t M, int K, int N, int dt) {
   p.np = pad(N);
   p.kp = pad(K);
   const int sz = lt_dt_size(dt), kf = 64 / sz;
-  const int w = ((N + kf - 1) / kf) * ((K + 15) / 16) * 1024, turn = 8 * 16 * (p.kp / 4 + 4) * 4;
+  const int w = ((N + kf - 1) / kf) * ((K + 15) / 16) * 1024, turn = 16 * 16 * (16 * (p.kp > 128 ? p.kp / 128 : 1) + 4) * 4;
   p.ok = 2 * 32 * (p.np + p.kp) * sz + w + turn <= 160 * 1024 && p.np * p.kp <= 256 * 128;
   p.tiles = (int)((M + 31) / 32);
   p.grid = p.tiles < 256 ? p.tiles : 256;
@@ -363,7 +364,7 @@ static int lt_rows_bwd_go(const LtRowsBwdArgs& a, int grid, hipStream_t stream) 
   const int smem = LtRowsBwd<T, NP, KP>::lds(a.N, a.K);
   if (smem > 65536)
     LT_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_rows_bwd<T, NP, KP>), hipFuncAttributeMaxDynamicSharedMemorySize, smem));
-  hipLaunchKernelGGL((k_rows_bwd<T, NP, KP>), dim3(grid), dim3(512), smem, stream, a);
+  hipLaunchKernelGGL((k_rows_bwd<T, NP, KP>), dim3(grid), dim3(1024), smem, stream, a);
   LT_LAUNCH_CHECK();
   return LT_OK;
 }

@@ -5,14 +5,11 @@ names are re-exported by latte_amd.functional, the modules are latte_amd.sparse_
 bfloat16, float16 (all operands of a call share one); sums are fp32.  GPU tensors only: there is no CPU fallback."""
 from __future__ import annotations
 
-import ctypes
-
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _p, _ws_bytes
+from .ops import _ws_bytes
 
 __all__ = ["Mx8", "quantize_mx8", "linear", "rms_norm"]
 
@@ -31,33 +28,61 @@ def _dt(t: torch.Tensor, name: str) -> int:
 
 
 def _like(t, ref: torch.Tensor, shape, name: str):
-    """`t` checked against the operand it goes with: type, device, shape"""
+    """`t` checked against the operand it goes with: type, device, shape (a torch.Size)"""
     if t.dtype != ref.dtype:
         raise TypeError(f"{name}: expected {ref.dtype}, got {t.dtype}")
     if t.device != ref.device:
         raise ValueError(f"{name}: on {t.device}, the other operands on {ref.device}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     return t
 
 
 def _rows(t: torch.Tensor, cols: int):
     """-> (2-D tensor with neighbouring columns, its row stride): a view wherever the strides allow one"""
-    t2 = t if t.dim() == 2 else t.reshape(-1, cols)
-    if t2.stride(1) != 1 and cols > 1:
-        t2 = t2.contiguous()
-    # a single row's stride means nothing; negative strides do not exist in torch
-    return t2, (t2.stride(0) if t2.shape[0] > 1 else cols)
+    if t.dim() != 2:
+        t = t.reshape(-1, cols)
+    ld, c = t.stride()
+    if c != 1 and cols > 1:
+        t = t.contiguous()
+        ld = cols
+    return t, (ld if t.shape[0] > 1 else cols)   # a single row's stride means nothing
 
 
-def _stream_of(t: torch.Tensor):
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _stream_of(t: torch.Tensor) -> int:
     """the current stream of the tensor's own device, whatever device is current"""
-    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(t.device.index))
+    return _raw_stream(t.device.index)
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+_LIB = None
+
+
+def _call(name: str, *args) -> None:
+    """_lib.call with plain integers for pointers: a call costs 4 us of host time here, of which 1 is spent in ctypes"""
+    global _LIB
+    if _LIB is None:
+        _LIB = _lib.load()
+    rc = getattr(_LIB, name)(*args)
+    if rc != 0:
+        raise _lib.LatteHipError(f"{name} failed (rc={rc}): {(_LIB.lt_last_error() or b'').decode()}")
+
+
+def _no_second(name: str) -> None:
+    """a backward pass runs with gradients enabled only where its own graph is asked for, which these kernels do not build"""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{name}: gradients of gradients are not implemented (create_graph=True)")
 
 
 def _buf(nbytes: int, device) -> torch.Tensor:
     """workspace of one call: torch's allocator (and a graph's private pool) keeps it from any other stream or graph"""
-    return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+    return torch.empty(nbytes if nbytes > 256 else 256, dtype=torch.uint8, device=device)
 
 
 # ------------------------------------------------------------------ mx8
@@ -91,7 +116,7 @@ class Mx8:
         out = torch.empty(self.shape, dtype=dtype, device=self.device)
         dt = _dt(out, "Mx8.dequantize")
         M, K = self.shape
-        _lib.call("lt_mx8_dequantize", _p(self.values), _p(self.scales), M, K, dt, _p(out), _stream_of(out))
+        _call("lt_mx8_dequantize", _p(self.values), _p(self.scales), M, K, dt, _p(out), _stream_of(out))
         return out
 
     @staticmethod
@@ -109,7 +134,7 @@ def quantize_mx8(x: torch.Tensor) -> Mx8:
     K = x.shape[-1]
     x2, ld = _rows(x.detach(), K)
     q = Mx8.empty(x2.shape[0], K, x.device)
-    _lib.call("lt_mx8_quantize", _p(x2), ld, x2.shape[0], K, dt, _p(q.values), _p(q.scales), _stream_of(x2))
+    _call("lt_mx8_quantize", _p(x2), ld, x2.shape[0], K, dt, _p(q.values), _p(q.scales), _stream_of(x2))
     return q
 
 
@@ -131,7 +156,7 @@ def _linear_fwd(x2, ldx, w, ldw, bias, res, act: str, deriv_kind: int):
     nb = _ws_bytes("lt_linear_workspace_bytes", M, K, N, dt)
     ws = _buf(nb, dev) if nb > 0 else None
     r2, ldr = _rows(res, N) if res is not None else (None, 0)
-    _lib.call("lt_linear_fwd", _p(x2), ldx, _p(w), ldw, _p(bias), _p(r2), ldr, _ACT[act], M, K, N, dt, _p(y), _p(deriv),
+    _call("lt_linear_fwd", _p(x2), ldx, _p(w), ldw, _p(bias), _p(r2), ldr, _ACT[act], M, K, N, dt, _p(y), _p(deriv),
               deriv_kind, _p(ws), nb, _stream_of(x2))
     return y, deriv
 
@@ -139,49 +164,51 @@ def _linear_fwd(x2, ldx, w, ldw, bias, res, act: str, deriv_kind: int):
 class _Linear(Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, checkpoint):
-        K, N = x.shape[-1], weight.shape[0]
+        N, K = weight.shape
         x2, ldx = _rows(x, K)
         w2, ldw = _rows(weight, K)
-        need = ctx.needs_input_grad
-        grads = need[0] or need[1] or need[2]
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
         kind = 0
-        if grads and act != "none":
+        if act != "none" and (need_x or need_w or need_b):
             kind = _BITS if act == "relu" else (_BYTE if checkpoint == "mx8" else _FULL)
-        b = bias.contiguous() if bias is not None else None
-        y, deriv = _linear_fwd(x2, ldx, w2, ldw, b, residual, act, kind)
-        keep_x, x_scales = None, None
-        if need[1]:
+        if bias is not None and not bias.is_contiguous():
+            bias = bias.contiguous()
+        y, deriv = _linear_fwd(x2, ldx, w2, ldw, bias, residual, act, kind)
+        keep_x = x_scales = None
+        if need_w:
             if checkpoint == "mx8":
                 q = quantize_mx8(x2)
-                keep_x, x_scales = q.values, q.scales
+                keep_x, x_scales, ldx = q.values, q.scales, K
             else:
                 keep_x = x2
-        ctx.kind, ctx.x_shape = kind, x.shape
-        ctx.save_for_backward(keep_x, x_scales, w2 if need[0] else None, deriv)
-        ctx.meta = (K, N, weight.dtype)
-        return y.view(*x.shape[:-1], N)
+        ctx.save_for_backward(keep_x, x_scales, w2 if need_x else None, deriv)
+        ctx.meta = (K, N, x.dtype, kind, ldx, ldw, x.shape)
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        _no_second("linear")
         x2, xs, w2, deriv = ctx.saved_tensors
-        K, N, dtype = ctx.meta
-        need = ctx.needs_input_grad
-        dev = dy.device
-        dy2, lddy = _rows(dy, N)
-        M = dy2.shape[0]
-        dx = torch.empty((M, K), dtype=dtype, device=dev) if need[0] else None
-        dw = torch.empty((N, K), dtype=dtype, device=dev) if need[1] else None
-        db = torch.empty((N,), dtype=dtype, device=dev) if need[2] else None
-        if dx is not None or dw is not None or db is not None:
+        K, N, dtype, kind, ldx, ldw, x_shape = ctx.meta
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        dx = dw = db = None
+        if need_x or need_w or need_b:
+            dev = dy.device
+            dy2, lddy = _rows(dy, N)
+            M = dy2.shape[0]
+            if need_x:
+                dx = torch.empty((M, K), dtype=dtype, device=dev)
+            if need_w:
+                dw = torch.empty((N, K), dtype=dtype, device=dev)
+            if need_b:
+                db = torch.empty((N,), dtype=dtype, device=dev)
             dt = _DT[dtype]
-            nb = _ws_bytes("lt_linear_bwd_workspace_bytes", M, K, N, dt, int(xs is not None))
-            ws = _buf(nb, dev)
-            ldx = 0 if x2 is None else (K if xs is not None else _rows(x2, K)[1])
-            ldw = 0 if w2 is None else _rows(w2, K)[1]
-            _lib.call("lt_linear_bwd", _p(dy2), lddy, _p(x2), ldx, _p(xs), _p(w2), ldw, _p(deriv), ctx.kind, M, K, N, dt,
-                      _p(dx), _p(dw), _p(db), _p(ws), ws.numel(), _stream_of(dy2))
-        return (dx.view(ctx.x_shape) if dx is not None else None), dw, db, (dy if need[3] else None), None, None
+            ws = _buf(_ws_bytes("lt_linear_bwd_workspace_bytes", M, K, N, dt, int(xs is not None)), dev)
+            _call("lt_linear_bwd", dy2.data_ptr(), lddy, _p(x2), ldx, _p(xs), _p(w2), ldw, _p(deriv), kind, M, K, N, dt, _p(dx), _p(dw),
+                  _p(db), ws.data_ptr(), ws.numel(), _stream_of(dy2))
+            if need_x and len(x_shape) != 2:
+                dx = dx.view(x_shape)
+        return dx, dw, db, (dy if need_r else None), None, None
 
 
 def _linear_mx8(x: Mx8, weight: Mx8, bias, act: str, residual, dtype):
@@ -201,11 +228,11 @@ def _linear_mx8(x: Mx8, weight: Mx8, bias, act: str, residual, dtype):
         raise ValueError(f"linear weight: on {weight.device}, the other operands on {x.device}")
     y = torch.empty((M, N), dtype=dtype, device=x.device)
     if bias is not None:
-        bias = _like(bias, y, (N,), "linear bias").contiguous()
-    r2, ldr = (None, 0) if residual is None else _rows(_like(residual, y, (M, N), "linear residual"), N)
+        bias = _like(bias, y, y.shape[1:], "linear bias").contiguous()
+    r2, ldr = (None, 0) if residual is None else _rows(_like(residual, y, y.shape, "linear residual"), N)
     nb = _ws_bytes("lt_linear_mx8_workspace_bytes", M, K, N)
     ws = _buf(nb, x.device) if nb > 0 else None
-    _lib.call("lt_linear_mx8_fwd", _p(x.values), _p(x.scales), _p(weight.values), _p(weight.scales), _p(bias), _p(r2), ldr, _ACT[act],
+    _call("lt_linear_mx8_fwd", _p(x.values), _p(x.scales), _p(weight.values), _p(weight.scales), _p(bias), _p(r2), ldr, _ACT[act],
               M, K, N, _DT[dtype], _p(y), _p(ws), nb, _stream_of(y))
     return y
 
@@ -234,11 +261,11 @@ def linear(x, weight, bias=None, act: str = "none", residual=None, checkpoint: s
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or min(weight.shape) < 1:
         raise ValueError(f"linear: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not go together")
     N, K = weight.shape
-    _like(weight, x, (N, K), "linear weight")
+    _like(weight, x, weight.shape, "linear weight")
     if bias is not None:
-        _like(bias, x, (N,), "linear bias")
+        _like(bias, x, weight.shape[:1], "linear bias")
     if residual is not None:
-        _like(residual, x, (*x.shape[:-1], N), "linear residual")
+        _like(residual, x, x.shape[:-1] + weight.shape[:1], "linear residual")
     return _Linear.apply(x, weight, bias, residual, act, checkpoint)
 
 
@@ -255,7 +282,7 @@ def _rms_fwd(x, w, residual, eps, want_h, want_y, want_y8, want_h8, want_rstd):
     h8 = Mx8.empty(M, C, dev) if want_h8 else None
     rstd = torch.empty((M,), dtype=torch.float32, device=dev) if want_rstd else None
     p8 = lambda q: (None, None) if q is None else (_p(q.values), _p(q.scales))  # noqa: E731
-    _lib.call("lt_rms_norm_fwd", _p(x2), ldx, _p(r2), ldr, _p(w), float(eps), M, C, _DT[x.dtype], _p(h), _p(y), *p8(y8), *p8(h8),
+    _call("lt_rms_norm_fwd", _p(x2), ldx, _p(r2), ldr, _p(w), float(eps), M, C, _DT[x.dtype], _p(h), _p(y), *p8(y8), *p8(h8),
               _p(rstd), _stream_of(x2))
     return h, y, y8, h8, rstd
 
@@ -275,12 +302,13 @@ class _RmsNorm(Function):
                 ctx.save_for_backward(h if residual is not None else _rows(x, C)[0], None, None, w, rstd)
         ctx.set_materialize_grads(False)   # a sum that nothing reads costs no zeros
         ctx.x_shape = x.shape
-        y = y.view(x.shape)
-        return y if residual is None else (y, h.view(x.shape))
+        if x.dim() != 2:
+            y, h = y.view(x.shape), (h.view(x.shape) if h is not None else None)
+        return y if residual is None else (y, h)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dh=None):
+        _no_second("rms_norm")
         h, q, sc, w, rstd = ctx.saved_tensors
         C, M = w.shape[0], rstd.shape[0]
         need = ctx.needs_input_grad
@@ -295,9 +323,10 @@ class _RmsNorm(Function):
         nb = _ws_bytes("lt_rms_norm_bwd_workspace_bytes", M, C) if dw is not None else 0
         ws = _buf(nb, w.device) if dw is not None else None
         ldh = 0 if h is None else _rows(h, C)[1]
-        _lib.call("lt_rms_norm_bwd", _p(dy2), lddy, _p(dh2), lddh, _p(h), ldh, _p(q), _p(sc), _p(w), _p(rstd), M, C, _DT[w.dtype],
+        _call("lt_rms_norm_bwd", _p(dy2), lddy, _p(dh2), lddh, _p(h), ldh, _p(q), _p(sc), _p(w), _p(rstd), M, C, _DT[w.dtype],
                   _p(dx), _p(dw), _p(ws), 0 if ws is None else ws.numel(), _stream_of(dy2))
-        dx = dx.view(ctx.x_shape) if dx is not None else None
+        if dx is not None and len(ctx.x_shape) != 2:
+            dx = dx.view(ctx.x_shape)
         return (dx if need[0] else None), dw, (dx if need[2] else None), None, None
 
 
@@ -315,7 +344,7 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, checkpoint: str | None
     _dt(x, "rms_norm x")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= 16384:
         raise ValueError(f"rms_norm: expected rows of 1 to 16384 elements, got shape {tuple(x.shape)}")
-    _like(weight, x, (x.shape[-1],), "rms_norm weight")
+    _like(weight, x, x.shape[-1:], "rms_norm weight")
     if residual is not None:
         _like(residual, x, x.shape, "rms_norm residual")
     if out == "mx8":
