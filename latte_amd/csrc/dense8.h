@@ -260,8 +260,7 @@ static int lt_gemm8_launch_act(const LtTile8Args& b, const LtPlan& p, hipStream_
     const dim3 grid((b.t.cols + 15) / 16), block(512);
     const int fr = (int)((b.t.rows + 15) / 16);
     if (fr == 1) hipLaunchKernelGGL((k_dense8_few<T, 1, ACT>), grid, block, 0, stream, b);
-    else if (fr == 2) hipLaunchKernelGGL((k_dense8_few<T, 2, ACT>), grid, block, 0, stream, b);
-    else hipLaunchKernelGGL((k_dense8_few<T, 4, ACT>), grid, block, 0, stream, b);
+    else hipLaunchKernelGGL((k_dense8_few<T, 2, ACT>), grid, block, 0, stream, b);
     LT_LAUNCH_CHECK();
     return LT_OK;
   }

@@ -9,7 +9,7 @@ static LtPlan plan8(int64_t M, int K, int N, bool direct) {
   p.direct = direct;
   p.splits = 1;
   p.slice = K;
-  p.few = M <= 64;
+  p.few = M <= 32;
   if (p.few) return p;
   auto tiles = [&](int b) { return ((M + b - 1) / b) * ((N + b - 1) / b); };
   int b = 64;

@@ -453,7 +453,7 @@ __device__ __forceinline__ void lt_few_store(const LtTileArgs& a, const lt_f32x4
   lt_epi8<T, ACT, false>(a.epi, z, b, res, row, col, n);
 }
 
-// ---- few rows: y[rows <= 64][cols].  Bound by reading P once: a workgroup takes 16 columns, its 8 waves share k in
+// ---- few rows: y[rows <= 32][cols].  Bound by reading P once: a workgroup takes 16 columns, its 8 waves share k in
 // turns of four fragments (256 bytes of each of the 16 lines of P), operands go from memory straight into the matrix
 // instructions' registers (nothing is used twice but the few rows of Q, which the caches hold), and the waves' sums are
 // added through LDS in wave order.
