@@ -352,11 +352,11 @@ int lt_linear_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, cons
 int lt_rms_norm_fwd(const void* x, int64_t ldx, const void* res, int64_t ldres, const void* w, float eps, int64_t M, int32_t C,
                     int32_t dt, void* h, void* y, void* y8, void* y8_scales, void* h8, void* h8_scales, float* rstd,
                     lt_stream_t stream);
-/* n = h rstd, g = dy w:  dx = rstd (g - n mean(g n)) + dh,  dw = column sums of dy n.  h (or h8 / h8_scales: h NULL), rstd:
- * what the forward left; dh, dx, dw may be NULL.  The same bits every time. */
+/* n = h rstd, g = dy w:  dx = rstd (g - n mean(g n)) + dh,  dw = column sums of dy n.  h (h + h2 where h2 is not NULL; or
+ * h8 / h8_scales with h NULL), rstd: what the forward left or was given; dh, dx, dw may be NULL.  The same bits every time. */
 int64_t lt_rms_norm_bwd_workspace_bytes(int64_t M, int32_t C);
-int lt_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, int64_t lddh, const void* h, int64_t ldh, const void* h8,
-                    const void* h8_scales, const void* w, const float* rstd, int64_t M, int32_t C, int32_t dt, void* dx, void* dw,
+int lt_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, int64_t lddh, const void* h, int64_t ldh, const void* h2,
+                    int64_t ldh2, const void* h8, const void* h8_scales, const void* w, const float* rstd, int64_t M, int32_t C, int32_t dt, void* dx, void* dw,
                     void* ws, int64_t ws_bytes, lt_stream_t stream);
 /* lt_bn_apply / lt_bn_bwd_reduce / lt_bn_bwd_apply with what the backward reads held in 8 bits: values uint8 [V][C] and
  * scales [V][ceil(C/32)] = x - c in mx8 (c: the mean rounded to a multiple of a quarter of the power of two at or below the

@@ -93,7 +93,7 @@ SIGNATURES = {
     "lt_linear_bwd": (ctypes.c_int, [P, I64, P, I64, P, P, I64, P, I32, I64, I32, I32, I32, P, P, P, P, I64, P]),
     "lt_rms_norm_fwd": (ctypes.c_int, [P, I64, P, I64, P, F32, I64, I32, I32, P, P, P, P, P, P, P, P]),
     "lt_rms_norm_bwd_workspace_bytes": (I64, [I64, I32]),
-    "lt_rms_norm_bwd": (ctypes.c_int, [P, I64, P, I64, P, I64, P, P, P, P, I64, I32, I32, P, P, P, I64, P]),
+    "lt_rms_norm_bwd": (ctypes.c_int, [P, I64, P, I64, P, I64, P, I64, P, P, P, P, I64, I32, I32, P, P, P, I64, P]),
     "lt_bn_apply_mx8": (ctypes.c_int, [P, P, P, P, P, F32, P, I32, P, P, P, P, I64, I32, P]),
     "lt_bn_bwd_reduce_mx8": (ctypes.c_int, [P, P, P, P, P, P, F32, I64, I32, P, I64, P, P, P]),
     "lt_bn_bwd_apply_mx8": (ctypes.c_int, [P, P, P, P, P, P, P, F32, P, P, P, P, I64, I32, P]),

@@ -301,6 +301,7 @@ struct LtOnStream {
 struct LtGemm {
   const void* P;
   const void* Q;
+  const void* Q2;            // or NULL: a second term of Q, laid out like it
   int64_t ldp, ldq;
   int64_t rows, depth;
   int cols;

@@ -47,7 +47,8 @@ static int gemm_run(const LtGemm& g, void* ws, int64_t ws_bytes, hipStream_t str
 // four columns, a workgroup a slab of rows; the slabs' sums are joined in a fixed order by k_col_join.
 template <class T, int DK>
 __global__ __launch_bounds__(256) void k_dz(const T* __restrict__ dy, int64_t lddy, const void* __restrict__ deriv, int64_t M,
-                                            int N, int tx, int64_t rows_per, T* __restrict__ dz, float* __restrict__ part, T* __restrict__ db) {
+                                            int N, int tx, int64_t rows_per, T* __restrict__ dz, T* __restrict__ dz2, float* __restrict__ part,
+                                            T* __restrict__ db) {
   __shared__ lt_f32x4 s_sum[256];
   const int x = threadIdx.x % tx, yy = threadIdx.x / tx, ty = 256 / tx;
   const int col = (blockIdx.x * tx + x) * 4;
@@ -86,6 +87,13 @@ __global__ __launch_bounds__(256) void k_dz(const T* __restrict__ dy, int64_t ld
         for (int i = 0; i < 4; ++i) g[i] *= d[i];
       }
       if constexpr (DK != LT_DERIV_NONE) lt_stv<T, 4>(dz + row * N + col, n, g);
+      if constexpr (sizeof(T) == 2 && (DK == LT_DERIV_BYTE || DK == LT_DERIV_FULL)) {
+        if (dz2) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d[i] = g[i] - (float)(T)g[i];
+          lt_stv<T, 4>(dz2 + row * N + col, n, d);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[i] += i < n ? g[i] : 0.f;
     }
@@ -122,17 +130,17 @@ static DzPlan dz_plan(int64_t M, int N) {
 }
 
 template <class T>
-static int dz_run(const void* dy, int64_t lddy, const void* deriv, int dkind, int64_t M, int N, void* dz, float* part, void* db,
+static int dz_run(const void* dy, int64_t lddy, const void* deriv, int dkind, int64_t M, int N, void* dz, void* dz2, float* part, void* db,
                   hipStream_t stream) {
   const DzPlan p = dz_plan(M, N);
   if (p.slabs > 0 && (part || dkind != LT_DERIV_NONE)) {
     const dim3 grid(p.gx, p.slabs), block(256);
     const T* g = (const T*)dy;
     switch (dkind) {
-      case LT_DERIV_BITS: hipLaunchKernelGGL((k_dz<T, LT_DERIV_BITS>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, part, (T*)db); break;
-      case LT_DERIV_BYTE: hipLaunchKernelGGL((k_dz<T, LT_DERIV_BYTE>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, part, (T*)db); break;
-      case LT_DERIV_FULL: hipLaunchKernelGGL((k_dz<T, LT_DERIV_FULL>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, part, (T*)db); break;
-      default: hipLaunchKernelGGL((k_dz<T, LT_DERIV_NONE>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, part, (T*)db); break;
+      case LT_DERIV_BITS: hipLaunchKernelGGL((k_dz<T, LT_DERIV_BITS>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, (T*)dz2, part, (T*)db); break;
+      case LT_DERIV_BYTE: hipLaunchKernelGGL((k_dz<T, LT_DERIV_BYTE>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, (T*)dz2, part, (T*)db); break;
+      case LT_DERIV_FULL: hipLaunchKernelGGL((k_dz<T, LT_DERIV_FULL>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, (T*)dz2, part, (T*)db); break;
+      default: hipLaunchKernelGGL((k_dz<T, LT_DERIV_NONE>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, (T*)dz2, part, (T*)db); break;
     }
     LT_LAUNCH_CHECK();
   }
@@ -256,8 +264,13 @@ extern "C" int lt_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t 
 // 16384 x 1024 -> 4096, bf16: a training step 1130 us with the widening in the staging, 696 us with it first
 static bool widen_first(int64_t M, int K, int N) { return N > 256 && M > 0; }
 
+// dz beside 16-bit types is rounded for the matrix instructions.  Among thousands of elements that adds as much variance
+// to a gradient as its own last rounding does; a handful can have bad luck, so a small dz goes in as two terms, itself and
+// what its rounding left (the products are launch-bound there).
+static bool two_terms(int64_t M, int N, int dt) { return dt != LT_DT_F32 && M * N <= 4096; }
+
 struct BwdWs {
-  int64_t dz, part, wide, gemm, bytes;
+  int64_t dz, dz2, part, wide, gemm, bytes;
 };
 // the larger of the two routes: one pass over the rows, or dz and two products
 static BwdWs bwd_ws(int64_t M, int K, int N, int dt, bool x8) {
@@ -265,6 +278,8 @@ static BwdWs bwd_ws(int64_t M, int K, int N, int dt, bool x8) {
   int64_t off = 0;
   w.dz = off;
   off += lt_align_up(M * N * lt_dt_size(dt), 256);
+  w.dz2 = off;
+  off += two_terms(M, N, dt) ? lt_align_up(M * N * lt_dt_size(dt), 256) : 0;
   w.part = off;
   off += lt_align_up((int64_t)dz_plan(M, N).slabs * N * 4, 256);
   w.wide = off;
@@ -322,11 +337,13 @@ extern "C" int lt_linear_bwd(const void* dy, int64_t lddy, const void* x, int64_
     dz = wsb + o.dz;
     lddz = N;
   }
-  LT_DENSE_TYPES(dt, rc = dz_run<T>(dy, lddy, deriv, deriv_kind, M, N, wsb + o.dz, db ? (float*)(wsb + o.part) : nullptr, db, stream));
+  void* dz2 = two_terms(M, N, dt) && (deriv_kind == LT_DERIV_BYTE || deriv_kind == LT_DERIV_FULL) ? wsb + o.dz2 : nullptr;
+  LT_DENSE_TYPES(dt, rc = dz_run<T>(dy, lddy, deriv, deriv_kind, M, N, wsb + o.dz, dz2, db ? (float*)(wsb + o.part) : nullptr, db, stream));
   if (rc) return rc;
   LtGemm g = {};
   g.dt = dt;
   g.act = LT_ACT_NONE;
+  g.Q2 = dz2;
   if (dx && M > 0) {
     g.P = w;
     g.ldp = ldw;

@@ -19,6 +19,7 @@
 struct LtTileArgs {
   const char* P;
   const char* Q;
+  const char* Q2;         // or NULL: the sum goes over Q and, once more with the same P, over Q2 (laid out like Q)
   int64_t ldp, ldq;       // bytes
   int64_t rows, depth;
   int cols;
@@ -290,13 +291,15 @@ __global__ __launch_bounds__(64 * WR * WC) void k_dense(LtTileArgs a) {
   const int col0 = (int)(in / gr) * BC;
   const int64_t k0 = split * a.slice;
   const int64_t kend = k0 + a.slice < a.depth ? k0 + a.slice : a.depth;
-  const int nk = (int)((kend - k0 + TP::BK - 1) / TP::BK);
+  const int nk1 = (int)((kend - k0 + TP::BK - 1) / TP::BK), nk = a.Q2 ? 2 * nk1 : nk1;
   constexpr int PS = P8 ? 1 : (int)sizeof(T);
   const char* pb = a.P + (PKM ? k0 * a.ldp + (int64_t)col0 * PS : col0 * a.ldp + k0 * PS);
-  const char* qb = a.Q + (QKM ? k0 * a.ldq + row0 * (int64_t)sizeof(T) : row0 * a.ldq + k0 * (int64_t)sizeof(T));
+  const int64_t qoff = QKM ? k0 * a.ldq + row0 * (int64_t)sizeof(T) : row0 * a.ldq + k0 * (int64_t)sizeof(T);
   const int64_t pstep = PKM ? TP::BK * a.ldp : TP::BK * PS, qstep = QKM ? TQ::BK * a.ldq : BKB;
   const int64_t pn = a.cols - col0, qn = a.rows - row0;
   const uint8_t* psc = P8 ? a.ps + k0 * a.ldps : nullptr;
+  auto qbase = [&](int t) { return (t < nk1 ? a.Q : a.Q2) + qoff; };   // step t of nk is step t % nk1 along k
+  auto kstep = [&](int t) { return t < nk1 ? t : t - nk1; };
 
   lt_f32x4 acc[FR][FC];
 #pragma unroll
@@ -333,10 +336,11 @@ __global__ __launch_bounds__(64 * WR * WC) void k_dense(LtTileArgs a) {
     sp.init(a.ldp, pn, wave, lane);
     sq.init(a.ldq, qn, wave, lane);
     auto issue = [&](int t) {
-      const int64_t left = kend - k0 - (int64_t)t * TP::BK;
+      const int kt = kstep(t);
+      const int64_t left = kend - k0 - (int64_t)kt * TP::BK;
       char* buf = s_tile + (t % NBUF) * BUF;
-      sp.load(pb + t * pstep, buf, left, wave, lane);
-      sq.load(qb + t * qstep, buf + TP::BYTES, left, wave, lane);
+      sp.load(pb + kt * pstep, buf, left, wave, lane);
+      sq.load(qbase(t) + kt * qstep, buf + TP::BYTES, left, wave, lane);
     };
     issue(0);
     for (int t = 0; t < nk; ++t) {
@@ -349,19 +353,19 @@ __global__ __launch_bounds__(64 * WR * WC) void k_dense(LtTileArgs a) {
   } else {
     LtStaged<T, TP, PKM, P8, NT> sp;
     LtStaged<T, TQ, QKM, false, NT> sq;
-    sp.load(pb, a.ldp, pn, kend - k0, psc, a.ldps, col0, tid);
-    sq.load(qb, a.ldq, qn, kend - k0, nullptr, 0, 0, tid);
+    auto get = [&](int t) {
+      const int kt = kstep(t);
+      const int64_t left = kend - k0 - (int64_t)kt * TP::BK;
+      sp.load(pb + kt * pstep, a.ldp, pn, left, P8 ? psc + kt * (TP::BK * a.ldps) : nullptr, a.ldps, col0, tid);
+      sq.load(qbase(t) + kt * qstep, a.ldq, qn, left, nullptr, 0, 0, tid);
+    };
+    get(0);
     for (int t = 0; t < nk; ++t) {
       char* cur = s_tile + (t & 1) * BUF;
       sp.store(cur, tid);      // its last readers passed the barrier of step t - 1
       sq.store(cur + TP::BYTES, tid);
       __syncthreads();
-      if (t + 1 < nk) {
-        const int64_t left = kend - k0 - (int64_t)(t + 1) * TP::BK;
-        if (P8) psc += TP::BK * a.ldps;
-        sp.load(pb + (t + 1) * pstep, a.ldp, pn, left, psc, a.ldps, col0, tid);
-        sq.load(qb + (t + 1) * qstep, a.ldq, qn, left, nullptr, 0, 0, tid);
-      }
+      if (t + 1 < nk) get(t + 1);
       compute(cur, [] {});
     }
   }

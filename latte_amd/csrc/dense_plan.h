@@ -64,7 +64,7 @@ template <class T> int lt_gemm_launch(const LtGemm& g, const LtPlan& p, float* p
 template <class T, bool PKM, bool QKM, int BR, int BC, int WR, int WC, bool DIRECT, bool P8, int ACT>
 static int lt_launch_tile(const LtTileArgs& a, hipStream_t stream) {
   // a single step needs one buffer: more workgroups a CU (310017 x 32 -> 256 fp32: 196 -> 178 us)
-  const bool one = a.slice <= 128 / (int64_t)sizeof(T);
+  const bool one = a.slice <= 128 / (int64_t)sizeof(T) && !a.Q2;
   const int need = WR * WC * LtTurn<BC / WC / 16>::BYTES;
   int smem = (one ? 1 : 2) * (BR + BC) * 128;
   if (smem < need) smem = need;
@@ -142,6 +142,7 @@ static int lt_gemm_launch_impl(const LtGemm& g, const LtPlan& p, float* part, hi
   LtTileArgs a = {};
   a.P = (const char*)g.P;
   a.Q = (const char*)g.Q;
+  a.Q2 = (const char*)g.Q2;
   a.ldp = g.ldp * (g.p_scales ? 1 : (int64_t)sizeof(T));
   a.ldq = g.ldq * (int64_t)sizeof(T);
   a.rows = g.rows;

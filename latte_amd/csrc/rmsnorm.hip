@@ -5,7 +5,8 @@
 //
 // HBM-bound, one pass: LANES lanes hold a row in registers (8 neighbours a lane and turn), so the sum of squares, the
 // normalised row and its 8-bit form need no second read; workgroups stride over the rows with w in registers.  h is summed
-// in fp32 and enters the norm unrounded; the backward pass reads h as it was stored (its type, or mx8).
+// in fp32 and enters the norm unrounded; the backward pass reads h from fp32 or mx8, or adds x and r again beside 16-bit types
+// (the rounded h would add as much variance to dw as dw's own rounding does; one more read of five).
 #include "dense.h"
 
 struct LtRmsArgs {
@@ -88,10 +89,11 @@ struct LtRmsBwdArgs {
   const void* dy;
   const void* dh;            // or NULL
   const void* h;             // [M][ldh], or NULL when h8 is there
+  const void* h2;            // or NULL: the second summand, h + h2 is the row that was normalised
   const uint8_t *h8, *h8s;
   const void* w;
   const float* rstd;
-  int64_t lddy, lddh, ldh, M;
+  int64_t lddy, lddh, ldh, ldh2, M;
   int C;
   void* dx;                  // or NULL
   float* part;               // [grid][C] column sums of dy n, or NULL
@@ -127,6 +129,12 @@ __global__ __launch_bounds__(256) void k_rms_bwd(LtRmsBwdArgs a) {
           for (int t = 0; t < 8; ++t) n[it][t] = 0.f;
       } else {
         lt_ldv<T, 8>((const T*)a.h + row * a.ldh + col, m, n[it]);
+        if (a.h2) {
+          float v[8];
+          lt_ldv<T, 8>((const T*)a.h2 + row * a.ldh2 + col, m, v);
+#pragma unroll
+          for (int t = 0; t < 8; ++t) n[it][t] += v[t];
+        }
       }
     }
 #pragma unroll
@@ -247,7 +255,7 @@ extern "C" int64_t lt_rms_norm_bwd_workspace_bytes(int64_t M, int32_t C) {
 }
 
 extern "C" int lt_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, int64_t lddh, const void* h, int64_t ldh,
-                               const void* h8, const void* h8_scales, const void* w, const float* rstd, int64_t M, int32_t C,
+                               const void* h2, int64_t ldh2, const void* h8, const void* h8_scales, const void* w, const float* rstd, int64_t M, int32_t C,
                                int32_t dt, void* dx, void* dw, void* ws, int64_t ws_bytes, hipStream_t stream) {
   int rc = check_rms("lt_rms_norm_bwd", M, C, dt);
   if (rc) return rc;
@@ -257,7 +265,7 @@ extern "C" int lt_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, int
   if ((rc = on.enter(stream))) return rc;
   if (M > 0) {
     LT_REQUIRE(dy && w && rstd && (h || (h8 && h8_scales)) && (!dw || ws), LT_ERR_ARG, "lt_rms_norm_bwd: null pointer");
-    const LtRmsBwdArgs a = {dy, dh, h, (const uint8_t*)h8, (const uint8_t*)h8_scales, w, rstd, lddy, lddh, ldh, M, C, dx,
+    const LtRmsBwdArgs a = {dy, dh, h, h2, (const uint8_t*)h8, (const uint8_t*)h8_scales, w, rstd, lddy, lddh, ldh, ldh2, M, C, dx,
                             dw ? (float*)ws : nullptr};
     LT_DENSE_TYPES(dt, rms_dispatch<T, RmsBwdLaunch>(C, a, grid, stream));
     LT_LAUNCH_CHECK();

@@ -187,8 +187,8 @@ Tensor linear(const Tensor& x, const Tensor& w, const std::optional<Tensor>& b_,
 
 // ------------------------------------------------------------------ rms_norm
 struct RmsSaved {
-  Tensor h, h8, h8s, w, rstd;
-  int64_t ldh = 0;
+  Tensor h, h2, h8, h8s, w, rstd;
+  int64_t ldh = 0, ldh2 = 0;
 };
 
 std::pair<Tensor, Tensor> rms_forward(const Tensor& x, const Tensor& w_, const Tensor& r, double eps, bool mx8, RmsSaved* keep) {
@@ -208,9 +208,11 @@ std::pair<Tensor, Tensor> rms_forward(const Tensor& x, const Tensor& w_, const T
   check("lt_rms_norm_fwd", lt.rms_fwd(x2.p(), x2.ld, r2.p(), r2.ld, w.data_ptr(), (float)eps, x2.n, (int32_t)C, dt, ptr(h), y.data_ptr(), nullptr,
                                       nullptr, ptr(h8), ptr(h8s), (float*)ptr(rstd), stream_of(x)));
   if (keep) {
-    if (!mx8) {   // without a residual h is x itself
-      keep->h = r.defined() ? h : x2.t;
-      keep->ldh = r.defined() ? C : x2.ld;
+    if (!mx8) {   // h: x itself without a residual, the stored sum in fp32, the two summands beside 16-bit types
+      const bool sum = r.defined() && dt == LT_DT_F32;
+      keep->h = sum ? h : x2.t;
+      keep->ldh = sum ? C : x2.ld;
+      if (r.defined() && !sum) keep->h2 = r2.t, keep->ldh2 = r2.ld;
     }
     keep->h8 = h8;
     keep->h8s = h8s;
@@ -229,8 +231,8 @@ struct RmsNode : public torch::autograd::Function<RmsNode> {
                                int64_t need) {
     RmsSaved keep;
     auto [y, h] = rms_forward(x, w, r.value_or(Tensor()), eps, mx8, &keep);
-    ctx->save_for_backward({keep.h, keep.h8, keep.h8s, keep.w, keep.rstd});
-    std::vector<int64_t> meta = {keep.ldh, need};
+    ctx->save_for_backward({keep.h, keep.h8, keep.h8s, keep.w, keep.rstd, keep.h2});
+    std::vector<int64_t> meta = {keep.ldh, need, keep.ldh2};
     for (auto s : x.sizes()) meta.push_back(s);
     ctx->saved_data["meta"] = meta;
     ctx->set_materialize_grads(false);   // a sum that nothing reads costs no zeros
@@ -255,10 +257,10 @@ struct RmsNode : public torch::autograd::Function<RmsNode> {
     if (need & NEED_W) dw = at::empty({C}, dy.options());
     const int64_t wsb = dw.defined() ? lt.rms_bwd_ws(M, (int32_t)C) : 0;
     const Tensor ws = dw.defined() ? workspace(wsb, dy) : Tensor();
-    check("lt_rms_norm_bwd", lt.rms_bwd(g.p(), g.ld, gh.p(), gh.ld, ptr(saved[0]), meta[0], ptr(saved[1]), ptr(saved[2]), w.data_ptr(),
+    check("lt_rms_norm_bwd", lt.rms_bwd(g.p(), g.ld, gh.p(), gh.ld, ptr(saved[0]), meta[0], ptr(saved[5]), meta[2], ptr(saved[1]), ptr(saved[2]), w.data_ptr(),
                                         (const float*)rstd.data_ptr(), M, (int32_t)C, dtype_of(dy, "rms_norm"), ptr(dx), ptr(dw), ptr(ws),
                                         ws.defined() ? ws.numel() : 0, stream_of(dy)));
-    if (dx.defined() && meta.size() != 4) dx = dx.view(at::IntArrayRef(meta.data() + 2, meta.size() - 2));
+    if (dx.defined() && meta.size() != 5) dx = dx.view(at::IntArrayRef(meta.data() + 3, meta.size() - 3));
     return {need & NEED_X ? dx : Tensor(), dw, need & NEED_R ? dx : Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };

@@ -47,8 +47,8 @@ def _check_rms(x, w, r, dy, dh, ckpt, eps=1e-6):
     if ckpt:
         N, nerr = R.mx8(h32)[0] * rstd, rel
     else:
-        N, nerr = H * rstd, rel + h_ + 0.0                             # h was stored in its type
-    low = 0.0 if ckpt else lo
+        N, nerr = H * rstd, rel
+    low = 0.0
     NA = N.abs() + low * rstd
     G = dy.double() * W
     dot = (G * N).mean(1, keepdim=True)
