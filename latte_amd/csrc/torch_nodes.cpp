@@ -27,6 +27,11 @@ struct Entry {
   decltype(&lt_rms_norm_fwd) rms_fwd;
   decltype(&lt_rms_norm_bwd_workspace_bytes) rms_bwd_ws;
   decltype(&lt_rms_norm_bwd) rms_bwd;
+  decltype(&lt_bn_workspace_bytes) bn_ws;
+  decltype(&lt_bn_stats) bn_stats;
+  decltype(&lt_bn_apply_mx8) bn_apply;
+  decltype(&lt_bn_bwd_reduce_mx8) bn_reduce;
+  decltype(&lt_bn_bwd_apply_mx8) bn_bwd;
 } lt;
 
 void check(const char* name, int rc) {
@@ -285,6 +290,73 @@ variable_list rms_norm(const Tensor& x, const Tensor& w, const std::optional<Ten
   return RmsNode::apply(x, w, r_, eps, mx8, need);
 }
 
+// ------------------------------------------------------------------ batch_norm with 8-bit checkpoints (fp32, batch statistics)
+void bn_like(const Tensor& t, const Tensor& x, at::IntArrayRef shape, const char* name) {
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat, name, ": expected torch.float32, got ", t.dtype());
+  like(t, x, shape, name);
+}
+
+struct BnNode : public torch::autograd::Function<BnNode> {
+  // -> y, mean, var
+  static variable_list forward(AutogradContext* ctx, const Tensor& x_, const Tensor& gamma_, const Tensor& beta_, const std::optional<Tensor>& r_,
+                               double eps, bool relu, bool post, int64_t need) {
+    const Tensor x = x_.contiguous(), gamma = gamma_.contiguous(), beta = beta_.contiguous();
+    const Tensor r = r_ ? r_->contiguous() : Tensor();
+    const int64_t V = x.size(0);
+    const int32_t C = (int32_t)x.size(1);
+    const lt_stream_t stream = stream_of(x);
+    Tensor y = at::empty_like(x), mean = at::empty({C}, x.options()), var = at::empty({C}, x.options());
+    Tensor q = at::empty({V, C}, x.options().dtype(at::kFloat8_e4m3fn)), s = at::empty({V, (C + 31) / 32}, x.options().dtype(at::kByte)), mask;
+    if (relu) mask = at::empty({V, (C + 15) / 16}, x.options().dtype(at::kShort));
+    const Tensor ws = workspace(lt.bn_ws(V, C), x);
+    check("lt_bn_stats", lt.bn_stats(x.data_ptr<float>(), V, C, ws.data_ptr(), ws.numel(), mean.data_ptr<float>(), var.data_ptr<float>(), stream));
+    check("lt_bn_apply_mx8", lt.bn_apply(x.data_ptr<float>(), mean.data_ptr<float>(), var.data_ptr<float>(), gamma.data_ptr<float>(),
+                                         beta.data_ptr<float>(), (float)eps, (const float*)ptr(r), post ? 3 : relu ? 1 : 0, y.data_ptr<float>(),
+                                         q.data_ptr(), s.data_ptr(), ptr(mask), V, C, stream));
+    ctx->save_for_backward({q, s, mask, mean, var, gamma});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["meta"] = std::vector<int64_t>{need, post};
+    ctx->mark_non_differentiable({mean, var});
+    return {y, mean, var};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    no_second("batch_norm");
+    const auto saved = ctx->get_saved_variables();
+    const auto meta = ctx->saved_data["meta"].toIntVector();
+    const float eps = (float)ctx->saved_data["eps"].toDouble();
+    const int64_t need = meta[0];
+    const bool post = meta[1] != 0;
+    const Tensor dy = grads[0].contiguous();
+    const Tensor &q = saved[0], &s = saved[1], &mask = saved[2], &mean = saved[3], &var = saved[4], &gamma = saved[5];
+    const int64_t V = q.size(0);
+    const int32_t C = (int32_t)q.size(1);
+    const lt_stream_t stream = stream_of(dy);
+    Tensor dgamma = at::empty({C}, dy.options()), dbeta = at::empty({C}, dy.options()), dx, dr;
+    if (need & NEED_X) dx = at::empty_like(dy);
+    if ((need & NEED_R) && !post) dr = at::empty_like(dy);
+    const Tensor ws = workspace(lt.bn_ws(V, C), dy);
+    check("lt_bn_bwd_reduce_mx8", lt.bn_reduce(dy.data_ptr<float>(), q.data_ptr(), s.data_ptr(), ptr(mask), mean.data_ptr<float>(),
+                                               var.data_ptr<float>(), eps, V, C, ws.data_ptr(), ws.numel(), dbeta.data_ptr<float>(),
+                                               dgamma.data_ptr<float>(), stream));
+    if (dx.defined() || dr.defined())
+      check("lt_bn_bwd_apply_mx8",
+            lt.bn_bwd(dy.data_ptr<float>(), q.data_ptr(), s.data_ptr(), ptr(mask), mean.data_ptr<float>(), var.data_ptr<float>(),
+                      gamma.data_ptr<float>(), eps, dbeta.data_ptr<float>(), dgamma.data_ptr<float>(), (float*)ptr(dx), (float*)ptr(dr), V, C, stream));
+    if ((need & NEED_R) && post) dr = dy;   // the residual bypasses the ReLU
+    return {dx, need & NEED_W ? dgamma : Tensor(), need & NEED_B ? dbeta : Tensor(), dr, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+variable_list batch_norm_mx8(const Tensor& x, const Tensor& gamma, const Tensor& beta, const std::optional<Tensor>& r, double eps, bool relu,
+                             bool post) {
+  TORCH_CHECK_VALUE(x.dim() == 2, "batch_norm: expected a [rows, channels] matrix, got shape ", x.sizes());
+  bn_like(x, x, x.sizes(), "batch_norm x");
+  bn_like(gamma, x, {x.size(1)}, "batch_norm gamma");
+  bn_like(beta, x, {x.size(1)}, "batch_norm beta");
+  if (r) bn_like(*r, x, x.sizes(), "batch_norm residual");
+  return BnNode::apply(x, gamma, beta, r, eps, relu, post && relu && r, needs(x, gamma, beta, r.value_or(Tensor())));
+}
+
 // ------------------------------------------------------------------ mx8 (no gradients)
 std::pair<Tensor, Tensor> quantize_mx8(const Tensor& x) {
   const int dt = dtype_of(x, "quantize_mx8");
@@ -357,6 +429,11 @@ void init(const py::dict& d) {
   bind(lt.rms_fwd, d, "lt_rms_norm_fwd");
   bind(lt.rms_bwd_ws, d, "lt_rms_norm_bwd_workspace_bytes");
   bind(lt.rms_bwd, d, "lt_rms_norm_bwd");
+  bind(lt.bn_ws, d, "lt_bn_workspace_bytes");
+  bind(lt.bn_stats, d, "lt_bn_stats");
+  bind(lt.bn_apply, d, "lt_bn_apply_mx8");
+  bind(lt.bn_reduce, d, "lt_bn_bwd_reduce_mx8");
+  bind(lt.bn_bwd, d, "lt_bn_bwd_apply_mx8");
 }
 
 }  // namespace
@@ -365,6 +442,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("init", &init, "entry points of liblatte_hip.so by name (addresses)");
   m.def("linear", &linear, py::call_guard<py::gil_scoped_release>());
   m.def("rms_norm", &rms_norm, py::call_guard<py::gil_scoped_release>());
+  m.def("batch_norm_mx8", &batch_norm_mx8, py::call_guard<py::gil_scoped_release>());
   m.def("quantize_mx8", &quantize_mx8, py::call_guard<py::gil_scoped_release>());
   m.def("dequantize_mx8", &dequantize_mx8, py::call_guard<py::gil_scoped_release>());
   m.def("linear_mx8", &linear_mx8, py::call_guard<py::gil_scoped_release>());

@@ -1,7 +1,7 @@
 """Dense layers on the HIP kernels: linear with its epilogue and its backward, rms_norm, and matrices held in 8 bits ("mx8").
 
-The checks of arguments, the autograd nodes and the calls of the C entry points (`lt_linear_*`, `lt_rms_norm_*`, `lt_mx8_*` of
-include/latte_hip.h) are csrc/torch_nodes.cpp; the public names are re-exported by latte_amd.functional, the modules are
+The checks of arguments, the autograd nodes and the calls of the C entry points (`lt_linear_*`, `lt_rms_norm_*`, `lt_mx8_*`,
+`lt_bn_*_mx8` of include/latte_hip.h) are csrc/torch_nodes.cpp; the public names are re-exported by latte_amd.functional, the modules are
 latte_amd.sparse_modules.Linear / RMSNorm.  Types: fp32, bfloat16, float16 (all operands of a call share one); sums are
 fp32.  GPU tensors only: there is no CPU fallback."""
 from __future__ import annotations
@@ -17,7 +17,8 @@ __all__ = ["Mx8", "quantize_mx8", "linear", "rms_norm"]
 _ACT = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}     # LT_ACT_*
 _ENTRIES = ("lt_last_error", "lt_mx8_quantize", "lt_mx8_dequantize", "lt_linear_mx8_workspace_bytes", "lt_linear_mx8_fwd",
             "lt_linear_workspace_bytes", "lt_linear_fwd", "lt_linear_bwd_workspace_bytes", "lt_linear_bwd", "lt_rms_norm_fwd",
-            "lt_rms_norm_bwd_workspace_bytes", "lt_rms_norm_bwd")
+            "lt_rms_norm_bwd_workspace_bytes", "lt_rms_norm_bwd", "lt_bn_workspace_bytes", "lt_bn_stats", "lt_bn_apply_mx8",
+            "lt_bn_bwd_reduce_mx8", "lt_bn_bwd_apply_mx8")
 _NODES = None
 
 

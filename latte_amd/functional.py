@@ -9,7 +9,7 @@ import numpy as np
 import torch
 from torch.autograd import Function
 
-from . import ops
+from . import dense, ops
 from .dense import Mx8, linear, quantize_mx8, rms_norm
 
 __all__ = ["KernelMap", "get_kernel_offsets", "sparse_conv", "conv_bn", "batch_norm", "spvoxelize", "spdevoxelize",
@@ -467,6 +467,12 @@ def batch_norm(x, gamma, beta, eps=1e-5, residual=None, relu=False, stats_out=No
     an element of x - its channel's mean, give or take an eighth of the channel's standard deviation)."""
     if checkpoint not in (None, "mx8"):
         raise ValueError(f"batch_norm: checkpoint must be None or 'mx8', got {checkpoint!r}")
+    if (checkpoint == "mx8" and SYNC_BN_GROUP is None and x.is_cuda and x.shape[0] > 1 and torch.is_grad_enabled()
+            and any(t is not None and t.requires_grad for t in (x, gamma, beta, residual))):
+        y, mean, var = dense._nodes().batch_norm_mx8(x, gamma, beta, residual, float(eps), bool(relu), bool(post_add))
+        if stats_out is not None:
+            stats_out.append((mean, var))
+        return y
     if x.shape[0] <= 1 and SYNC_BN_GROUP is None:
         # same refusal as torch.nn.functional.batch_norm in training mode; with cross-rank statistics the LOCAL row count
         # says nothing (and every rank must reach the collective), so the call goes through
