@@ -317,7 +317,7 @@ extern "C" int lt_linear_bwd(const void* dy, int64_t lddy, const void* x, int64_
     float* part_w = (float*)wsb;
     float* part_b = (float*)(wsb + lt_align_up((int64_t)rp.grid * N * K * 4, 256));
     const LtRowsBwdArgs a = {dy, x, (const uint8_t*)x_scales, w, deriv, lddy, ldx, ldw, deriv_kind, M, N, K, dx, dw ? part_w : nullptr,
-                             db ? part_b : nullptr, rp.tiles};
+                             db ? part_b : nullptr};
     LT_DENSE_TYPES(dt, rc = lt_rows_bwd_launch<T>(a, rp, stream));
     if (rc) return rc;
     if (dw) {

@@ -6,7 +6,7 @@
 
 // ------------------------------------------------------------------ forward
 // A wave takes strips of 16 rows: its x fragments come straight from memory (a strip ahead), W's from LDS, no barriers.
-//   310017 x 128 -> 96 + residual, fp32: @RF@
+//   310017 x 128 -> 96 + residual, fp32: 103 us (3.9 TB/s; 145 on tiles); bf16: 38 us (5.2 TB/s)
 template <class T, int KC, int FC, int ACT>
 __global__ __launch_bounds__(512) void k_rows_fwd(LtTileArgs a) {
   typedef typename LtMma<T>::frag Frag;
@@ -61,10 +61,11 @@ __global__ __launch_bounds__(512) void k_rows_fwd(LtTileArgs a) {
 }
 
 // ------------------------------------------------------------------ backward
-// One pass: a workgroup takes tiles of 32 rows, forms dz = dy act' on the way into LDS (its column sums stay in registers),
-// and from the two tiles dz [32][N] and x [32][K] its waves compute dx = dz W (W in LDS) and add dz^T x to the workgroup's
+// One pass: a workgroup takes tiles of R rows, forms dz = dy act' on the way into LDS (its column sums stay in registers),
+// and from the two tiles dz [R][N] and x [R][K] its waves compute dx = dz W (W in LDS) and add dz^T x to the workgroup's
 // own dW, which they hold in registers until the end.  dy, act' and x are read once, dz is never written.
-//   310017 x 128 -> 96, fp32: @RB@
+//   310017 x 128 -> 96, fp32: 242 us, half of it the two products at 55 % of the fp32 matrix rate (dz, dx and dW apart: 282
+//   us); bf16: 74 us.
 struct LtRowsBwdArgs {
   const void* dy;
   const void* x;
@@ -78,18 +79,22 @@ struct LtRowsBwdArgs {
   void* dx;               // [M][K] or NULL
   float* dw;              // [grid][N][K] or NULL
   float* db;              // [grid][N] or NULL
-  int tiles;              // of 32 rows
 };
 
 template <class T, int NP, int KP>
 struct LtRowsBwd {
-  static constexpr int CH = 16 / sizeof(T), BKB = 32 * sizeof(T);   // 32 rows of a tile are 32 k of dW's product
+  // rows a tile, the k of dW's product: about 16 KB each of dz and x, so that what a tile waits for memory is small beside
+  // what it moves (310017 x 64 -> 64 bf16: 84 us in tiles of 32 rows, 42 in
+  // tiles of 128)
+  static constexpr int R = NP * KP == 64 * 64 ? 256 / sizeof(T) : sizeof(T) == 2 && NP + KP <= 256 ? 64 : 32;
+  static constexpr int CH = 16 / sizeof(T), BKB = R * sizeof(T);
   typedef LtTile<T, true, NP, BKB> TZ;
   typedef LtTile<T, true, KP, BKB> TX;
-  static constexpr int NT = 1024;   // 16 waves: with 8 the LDS latencies showed (@RB8@)
+  static constexpr int NT = 1024;   // 16 waves: with 8 the LDS latencies showed (128 -> 96 fp32: 261 us, with 16 222)
   static constexpr int NZ = (TZ::BYTES / 16 + NT - 1) / NT, NX = (TX::BYTES / 16 + NT - 1) / NT;
   static constexpr int TN = NP / 64, TK = KP / 64;                  // the waves' 4 x 4 grid over dW: 16 x 16 tiles a wave
-  static constexpr int FX = KP > 128 ? KP / 128 : 1;                // dx: 2 strips x 8 column groups of FX tiles
+  static constexpr int SX = R / 16, GX = 16 / SX;                   // dx: SX strips x GX column groups
+  static constexpr int FX = KP / 16 > GX ? KP / 16 / GX : 1;        // of FX tiles
   static constexpr int BUF = TZ::BYTES + TX::BYTES;
   static int lds(int N, int K) {
     const int nf = (N + 4 * CH - 1) / (4 * CH), kt = (K + 15) / 16;
@@ -103,7 +108,7 @@ __global__ __launch_bounds__(1024) void k_rows_bwd(LtRowsBwdArgs a) {
   typedef typename S::TZ TZ;
   typedef typename S::TX TX;
   typedef typename LtMma<T>::frag Frag;
-  constexpr int CH = S::CH, KF = 4 * CH, KK = sizeof(T) == 2 ? 1 : 2;   // fragments of 32 rows
+  constexpr int CH = S::CH, KF = 4 * CH, KK = S::R / KF;   // fragments along the rows of a tile
   extern __shared__ __attribute__((aligned(1024))) char s_tile[];
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -167,7 +172,7 @@ __global__ __launch_bounds__(1024) void k_rows_bwd(LtRowsBwdArgs a) {
     for (int i = 0; i < S::NZ; ++i) {
       int line, c;
       TZ::where(tid + i * S::NT, line, c);
-      const bool ok = line < 32 && m0 + line < a.M && c * CH < N;
+      const bool ok = line < S::R && m0 + line < a.M && c * CH < N;
       T t[CH], y[CH];
       __builtin_memcpy(y, &gz[i], 16);
       float z[CH];
@@ -200,7 +205,7 @@ __global__ __launch_bounds__(1024) void k_rows_bwd(LtRowsBwdArgs a) {
     for (int i = 0; i < S::NX; ++i) {
       int line, c;
       TX::where(tid + i * S::NT, line, c);
-      const bool ok = line < 32 && m0 + line < a.M && c * CH < K;
+      const bool ok = line < S::R && m0 + line < a.M && c * CH < K;
       lt_i32x4 v = gx[i];
       if (a.xs) {
         const float sc = __uint_as_float(gs[i] << 23);
@@ -226,32 +231,28 @@ __global__ __launch_bounds__(1024) void k_rows_bwd(LtRowsBwdArgs a) {
   e.cols = K;
   e.splits = 1;
   e.epi = LtEpi{nullptr, nullptr, 0, a.dx, K, nullptr, LT_DERIV_NONE, a.M, K};
-  const int strip = wave & 1, xg = wave >> 1;          // dx: rows 16 strip .., columns 16 FX xg ..
+  const int strip = wave % S::SX, xg = wave / S::SX;   // dx: rows 16 strip .., columns 16 FX xg ..
   const int wn = (wave >> 2) * S::TN, wk = (wave & 3) * S::TK;
-  int64_t t = blockIdx.x;
-  if (t < a.tiles) fetch(t * 32);
-  for (int b = 0; t < a.tiles; t += gridDim.x, b ^= 1) {
-    char* buf = s_tile + b * S::BUF;
-    put(buf, t * 32);
-    __syncthreads();       // (W is in place too); the other buffer's readers are past the barrier before
-    if (t + gridDim.x < a.tiles) fetch((t + gridDim.x) * 32);
-    if (a.dx && xg * S::FX < kt) {
-      lt_f32x4 acc[1][S::FX];
+  const int tiles = (int)((a.M + S::R - 1) / S::R);
+  auto do_dx = [&](const char* buf, int64_t m0) {
+    if (!a.dx || xg * S::FX >= kt) return;
+    lt_f32x4 acc[1][S::FX];
 #pragma unroll
-      for (int j = 0; j < S::FX; ++j) acc[0][j] = (lt_f32x4){0.f, 0.f, 0.f, 0.f};
-      const int m = 16 * strip + r;
+    for (int j = 0; j < S::FX; ++j) acc[0][j] = (lt_f32x4){0.f, 0.f, 0.f, 0.f};
+    const int m = 16 * strip + r;
 #pragma unroll 2
-      for (int f = 0; f < nf; ++f) {
-        const int c = f * 4 + g;                       // chunk of CH columns n of row m
-        const Frag q = *reinterpret_cast<const Frag*>(buf + m * (NP * (int)sizeof(T)) + ((c ^ TZ::kswz(m)) << 4));
+    for (int f = 0; f < nf; ++f) {
+      const int c = f * 4 + g;                         // chunk of CH columns n of row m
+      const Frag q = *reinterpret_cast<const Frag*>(buf + m * (NP * (int)sizeof(T)) + ((c ^ TZ::kswz(m)) << 4));
 #pragma unroll
-        for (int j = 0; j < S::FX; ++j)
-          if (xg * S::FX + j < kt)
-            acc[0][j] = LtMma<T>::mma(*reinterpret_cast<const Frag*>(s_w + (f * kt + xg * S::FX + j) * 1024 + lane * 16), q, acc[0][j]);
-      }
-      lt_tile_store_<T, 1, S::FX, LT_ACT_NONE, true>(e, acc, 0, t * 32 + 16 * strip, 16 * S::FX * xg, lane, turn);
+      for (int j = 0; j < S::FX; ++j)
+        if (xg * S::FX + j < kt)
+          acc[0][j] = LtMma<T>::mma(*reinterpret_cast<const Frag*>(s_w + (f * kt + xg * S::FX + j) * 1024 + lane * 16), q, acc[0][j]);
     }
-    if (!a.dw) continue;
+    lt_tile_store_<T, 1, S::FX, LT_ACT_NONE, true>(e, acc, 0, m0 + 16 * strip, 16 * S::FX * xg, lane, turn);
+  };
+  auto do_dw = [&](const char* buf) {
+    if (!a.dw) return;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       Frag p[S::TK];
@@ -267,6 +268,17 @@ __global__ __launch_bounds__(1024) void k_rows_bwd(LtRowsBwdArgs a) {
           if (wk + j < kt) dw[i][j] = LtMma<T>::mma(p[j], q, dw[i][j]);
       }
     }
+  };
+  int t = blockIdx.x;
+  if (t < tiles) fetch((int64_t)t * S::R);
+  for (int b = 0; t < tiles; t += gridDim.x, b ^= 1) {
+    char* buf = s_tile + b * S::BUF;
+    const int64_t m0 = (int64_t)t * S::R;
+    put(buf, m0);
+    __syncthreads();       // (W is in place too); the other buffer's readers are past the barrier before
+    if (t + (int)gridDim.x < tiles) fetch((int64_t)(t + gridDim.x) * S::R);
+    do_dx(buf, m0);
+    do_dw(buf);
   }
   float* out = a.dw ? a.dw + (int64_t)blockIdx.x * N * K : nullptr;
 #pragma unroll
@@ -284,7 +296,7 @@ __global__ __launch_bounds__(1024) void k_rows_bwd(LtRowsBwdArgs a) {
   for (int i = 0; i < S::NZ; ++i) {
     int line, c;
     TZ::where(tid + i * S::NT, line, c);
-    if (line < 32)
+    if (line < S::R)
 #pragma unroll
       for (int j = 0; j < CH; ++j) s_db[line * NP + c * CH + j] = db[i][j];
   }
@@ -292,7 +304,7 @@ __global__ __launch_bounds__(1024) void k_rows_bwd(LtRowsBwdArgs a) {
   for (int n = tid; n < N; n += S::NT) {
     float s = 0.f;
 #pragma unroll 8
-    for (int l = 0; l < 32; ++l) s += s_db[l * NP + n];
+    for (int l = 0; l < S::R; ++l) s += s_db[l * NP + n];
     a.db[(int64_t)blockIdx.x * N + n] = s;
   }
 }
@@ -344,7 +356,7 @@ static int lt_rows_fwd(const LtTileArgs& a, hipStream_t stream) {
 // backward: widths that are multiples of 8 and whose dW a workgroup's registers and whose W its LDS hold
 struct LtRowsBwdPlan {
   bool ok;
-  int np, kp, grid, tiles;
+  int np, kp, grid, lds;
 };
 static inline LtRowsBwdPlan lt_rows_bwd_plan(int64_t M, int K, int N, int dt) {
   LtRowsBwdPlan p = {};
@@ -352,16 +364,20 @@ static inline LtRowsBwdPlan lt_rows_bwd_plan(int64_t M, int K, int N, int dt) {
   if (N > 256 || K > 256 || N % 8 || K % 8 || M < 2048 || M > (int64_t)1 << 34) return p;
   p.np = pad(N);
   p.kp = pad(K);
-  const int sz = lt_dt_size(dt), kf = 64 / sz;
-  const int w = ((N + kf - 1) / kf) * ((K + 15) / 16) * 1024, turn = 16 * 16 * (16 * (p.kp > 128 ? p.kp / 128 : 1) + 4) * 4;
-  p.ok = 2 * 32 * (p.np + p.kp) * sz + w + turn <= 160 * 1024 && p.np * p.kp <= 256 * 128;
-  p.tiles = (int)((M + 31) / 32);
-  p.grid = p.tiles < 256 ? p.tiles : 256;
+  const int sz = lt_dt_size(dt), kf = 64 / sz;   // as in LtRowsBwd, which checks the two against each other
+  const int R = p.np * p.kp == 64 * 64 ? 256 / sz : sz == 2 && p.np + p.kp <= 256 ? 64 : 32;
+  const int gx = 16 / (R / 16), fx = p.kp / 16 > gx ? p.kp / 16 / gx : 1;
+  const int w = ((N + kf - 1) / kf) * ((K + 15) / 16) * 1024, turn = 16 * 16 * (16 * fx + 4) * 4;
+  p.lds = 2 * R * (p.np + p.kp) * sz + w + turn;
+  p.ok = p.lds <= 160 * 1024 && p.np * p.kp <= 256 * 128 && (sz == 2 || p.np + p.kp <= 320);   // fp32 tiles of 128 and 256: no room
+  const int64_t tiles = (M + R - 1) / R;
+  p.grid = (int)(tiles < 256 ? tiles : 256);
   return p;
 }
 template <class T, int NP, int KP>
-static int lt_rows_bwd_go(const LtRowsBwdArgs& a, int grid, hipStream_t stream) {
-  const int smem = LtRowsBwd<T, NP, KP>::lds(a.N, a.K);
+static int lt_rows_bwd_go(const LtRowsBwdArgs& a, const LtRowsBwdPlan& p, hipStream_t stream) {
+  const int smem = LtRowsBwd<T, NP, KP>::lds(a.N, a.K), grid = p.grid;
+  LT_REQUIRE(smem == p.lds, LT_ERR_ARG, "linear: plan and kernel disagree (%d, %d bytes of LDS)", p.lds, smem);
   if (smem > 65536)
     LT_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_rows_bwd<T, NP, KP>), hipFuncAttributeMaxDynamicSharedMemorySize, smem));
   hipLaunchKernelGGL((k_rows_bwd<T, NP, KP>), dim3(grid), dim3(1024), smem, stream, a);
@@ -372,13 +388,18 @@ template <class T> int lt_rows_bwd_launch(const LtRowsBwdArgs& a, const LtRowsBw
 template <class T>
 static int lt_rows_bwd_impl(const LtRowsBwdArgs& a, const LtRowsBwdPlan& p, hipStream_t stream) {
   switch (p.np * 1000 + p.kp) {
-    case 64064: return lt_rows_bwd_go<T, 64, 64>(a, p.grid, stream);
-    case 64128: return lt_rows_bwd_go<T, 64, 128>(a, p.grid, stream);
-    case 64256: return lt_rows_bwd_go<T, 64, 256>(a, p.grid, stream);
-    case 128064: return lt_rows_bwd_go<T, 128, 64>(a, p.grid, stream);
-    case 128128: return lt_rows_bwd_go<T, 128, 128>(a, p.grid, stream);
-    case 128256: return lt_rows_bwd_go<T, 128, 256>(a, p.grid, stream);
-    case 256064: return lt_rows_bwd_go<T, 256, 64>(a, p.grid, stream);
-    default: return lt_rows_bwd_go<T, 256, 128>(a, p.grid, stream);
+    case 64064: return lt_rows_bwd_go<T, 64, 64>(a, p, stream);
+    case 64128: return lt_rows_bwd_go<T, 64, 128>(a, p, stream);
+    case 64256: return lt_rows_bwd_go<T, 64, 256>(a, p, stream);
+    case 128064: return lt_rows_bwd_go<T, 128, 64>(a, p, stream);
+    case 128128: return lt_rows_bwd_go<T, 128, 128>(a, p, stream);
+    case 256064: return lt_rows_bwd_go<T, 256, 64>(a, p, stream);
+    default:
+      if constexpr (sizeof(T) == 2) {
+        if (p.kp == 256) return lt_rows_bwd_go<T, 128, 256>(a, p, stream);
+        return lt_rows_bwd_go<T, 256, 128>(a, p, stream);
+      }
+      lt_set_error("linear: no one-pass backward for %d x %d", p.np, p.kp);
+      return LT_ERR_ARG;
   }
 }
