@@ -38,7 +38,7 @@ static int gemm_run(const LtGemm& g, void* ws, int64_t ws_bytes, hipStream_t str
   const LtPlan p = lt_gemm_plan(g.rows, g.cols, g.depth, g.dt, !g.p_kmajor && !g.q_kmajor, direct, true);
   LT_REQUIRE(part_bytes(p, g.rows, g.cols) <= ws_bytes, LT_ERR_WORKSPACE, "linear: workspace too small (%lld bytes)",
              (long long)ws_bytes);
-  LT_REQUIRE((int64_t)p.tr * p.tc * p.splits < (int64_t)1 << 31, LT_ERR_RANGE, "linear: too many tiles");
+  LT_REQUIRE((int64_t)p.tr * p.tc * p.splits < (int64_t)1 << 22, LT_ERR_RANGE, "linear: too many tiles");
   LT_DENSE_TYPES(g.dt, return lt_gemm_launch<T>(g, p, (float*)ws, stream));
 }
 

@@ -59,7 +59,7 @@ extern "C" int lt_linear_mx8_fwd(const void* x, const void* x_scales, const void
   const bool direct = K % 16 == 0 && ((uintptr_t)x & 15) == 0 && ((uintptr_t)w & 15) == 0 && (int64_t)K * 256 < (int64_t)1 << 31;
   const LtPlan p = plan8(M, K, N, direct);
   LT_REQUIRE(part8(p, M, N) <= (ws ? ws_bytes : 0), LT_ERR_WORKSPACE, "lt_linear_mx8_fwd: workspace too small");
-  LT_REQUIRE((int64_t)p.tr * p.tc * p.splits < (int64_t)1 << 31, LT_ERR_RANGE, "lt_linear_mx8_fwd: too many tiles");
+  LT_REQUIRE((int64_t)p.tr * p.tc * p.splits < (int64_t)1 << 22, LT_ERR_RANGE, "lt_linear_mx8_fwd: too many tiles");
   LtTile8Args b = {};
   b.t.P = (const char*)w;
   b.t.Q = (const char*)x;

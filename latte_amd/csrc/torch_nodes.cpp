@@ -3,6 +3,7 @@
 // Host time is what small layers cost: as Python Functions a forward and backward took about 120 us of it, most in
 // interpreter code on two threads that hand the interpreter lock to each other; the device needs 20 to 40 us for the same.
 // The entry points come from the library that latte_amd._lib has loaded (init), so this module links none of them.
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
@@ -104,6 +105,7 @@ struct LinearSaved {
 
 Tensor linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r, int64_t act, bool mx8, int64_t need,
                       LinearSaved* keep) {
+  const c10::DeviceGuard on(x.device());   // a null stream is the current device's
   const int dt = dtype_of(x, "linear x");
   const int64_t N = w.size(0), K = w.size(1);
   const Rows x2(x, K), w2(w, K), r2(r, N);
@@ -151,6 +153,7 @@ struct LinearNode : public torch::autograd::Function<LinearNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     no_second("linear");
+    const c10::DeviceGuard on(grads[0].device());
     const auto saved = ctx->get_saved_variables();
     const auto meta = ctx->saved_data["meta"].toIntVector();
     const int64_t K = meta[0], N = meta[1], need = meta[5];
@@ -197,6 +200,7 @@ struct RmsSaved {
 };
 
 std::pair<Tensor, Tensor> rms_forward(const Tensor& x, const Tensor& w_, const Tensor& r, double eps, bool mx8, RmsSaved* keep) {
+  const c10::DeviceGuard on(x.device());
   const int dt = dtype_of(x, "rms_norm x");
   const int64_t C = x.size(-1);
   const Rows x2(x, C), r2(r, C);
@@ -256,6 +260,7 @@ struct RmsNode : public torch::autograd::Function<RmsNode> {
       if (dh.defined() && (need & NEED_W)) dw = at::zeros_like(w);
       return {need & NEED_X ? dh : Tensor(), dw, need & NEED_R ? dh : Tensor(), Tensor(), Tensor(), Tensor()};
     }
+    const c10::DeviceGuard on(dy.device());
     const int64_t C = w.size(0), M = rstd.size(0);
     const Rows g(dy, C), gh(dh, C);
     if (need & (NEED_X | NEED_R)) dx = at::empty({M, C}, dy.options());
@@ -300,6 +305,7 @@ struct BnNode : public torch::autograd::Function<BnNode> {
   // -> y, mean, var
   static variable_list forward(AutogradContext* ctx, const Tensor& x_, const Tensor& gamma_, const Tensor& beta_, const std::optional<Tensor>& r_,
                                double eps, bool relu, bool post, int64_t need) {
+    const c10::DeviceGuard on(x_.device());
     const Tensor x = x_.contiguous(), gamma = gamma_.contiguous(), beta = beta_.contiguous();
     const Tensor r = r_ ? r_->contiguous() : Tensor();
     const int64_t V = x.size(0);
@@ -326,6 +332,7 @@ struct BnNode : public torch::autograd::Function<BnNode> {
     const float eps = (float)ctx->saved_data["eps"].toDouble();
     const int64_t need = meta[0];
     const bool post = meta[1] != 0;
+    const c10::DeviceGuard on(grads[0].device());
     const Tensor dy = grads[0].contiguous();
     const Tensor &q = saved[0], &s = saved[1], &mask = saved[2], &mean = saved[3], &var = saved[4], &gamma = saved[5];
     const int64_t V = q.size(0);
@@ -362,10 +369,12 @@ std::pair<Tensor, Tensor> quantize_mx8(const Tensor& x) {
   const int dt = dtype_of(x, "quantize_mx8");
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "quantize_mx8: expected rows of at least one element, got shape ", x.sizes());
   at::NoGradGuard off;
+  const c10::DeviceGuard on(x.device());
   return quantize(Rows(x, x.size(-1)), x.size(-1), dt);
 }
 
 Tensor dequantize_mx8(const Tensor& q, const Tensor& s, at::ScalarType dtype) {
+  const c10::DeviceGuard on(q.device());
   Tensor out = at::empty(q.sizes(), q.options().dtype(dtype));
   check("lt_mx8_dequantize", lt.mx8_dequantize(q.data_ptr(), s.data_ptr(), q.size(0), (int32_t)q.size(1), dtype_of(out, "Mx8.dequantize"),
                                                out.data_ptr(), stream_of(q)));
@@ -381,6 +390,7 @@ Tensor linear_mx8(const Tensor& x, const Tensor& xs, const Tensor& w, const Tens
                   const std::optional<Tensor>& r_, int64_t act, std::optional<at::ScalarType> dtype) {
   const Tensor b = b_.value_or(Tensor()), r = r_.value_or(Tensor());
   no_gradient("linear: mx8 operands carry no gradient", {b, r});
+  const c10::DeviceGuard on(x.device());
   const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
   TORCH_CHECK_VALUE(w.size(1) == K && K >= 1 && N >= 1, "linear: x ", x.sizes(), " and weight ", w.sizes(), " do not go together");
   TORCH_CHECK_VALUE(w.device() == x.device(), "linear weight: on ", w.device(), ", the other operands on ", x.device());
@@ -403,6 +413,7 @@ variable_list rms_norm_mx8(const Tensor& x, const Tensor& w, const std::optional
   const Tensor r = r_.value_or(Tensor());
   const int dt = check_rms(x, w, r);
   no_gradient("rms_norm: out='mx8' carries no gradient", {x, w, r});
+  const c10::DeviceGuard on(x.device());
   const int64_t C = x.size(-1);
   const Rows x2(x, C), r2(r, C);
   Tensor q = at::empty({x2.n, C}, x.options().dtype(at::kFloat8_e4m3fn)), s = at::empty({x2.n, (C + 31) / 32}, x.options().dtype(at::kByte)), h;

@@ -204,7 +204,7 @@ class NetProgram:
                     return False
             elif conv.bias is not None or conv.kernel.requires_grad:
                 return False
-            if getattr(bn, "checkpoint", None) is not None:   # 8-bit checkpoints: the module path
+            if getattr(bn, "checkpoint", None) is not None and torch.is_grad_enabled():   # 8-bit checkpoints: the module path
                 return False
             tracked = bn.track_running_stats and bn.running_mean is not None
             if tracked:   # eval mode: running estimates; train mode: they would have to be updated

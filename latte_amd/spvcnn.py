@@ -40,7 +40,7 @@ def _conv_bn_impl(seq, x: SparseTensor, i: int, relu: bool, residual=None) -> Sp
     from . import functional as LF
     if (conv.kernel_volume > 1 and conv.bias is None and x.feats.is_cuda and x.feats.shape[1] % 16 == 0
             and batch_stats and not updates_running and not conv.kernel.requires_grad and x.feats.shape[0] > 1
-            and getattr(bn, "checkpoint", None) is None   # the composite keeps the conv's output in full
+            and not (getattr(bn, "checkpoint", None) and torch.is_grad_enabled())   # the composite keeps the conv's output in full
             and LF.SYNC_BN_GROUP is None):   # cross-rank statistics: the all-reduce sits between conv and BN apply
         y = spnn.conv3d_bn(x, conv, bn, relu=relu, residual=residual)
         if y is not None:

@@ -22,6 +22,7 @@ import torch.nn.functional as F
 from . import ops
 from .functional import gather_rows
 from .hr_module import CR_Block, HR_Block
+from .sparse_modules import set_activation_checkpoint
 from .spvcnn import inverse_to_all
 
 __all__ = ["ensure_side_stream", "MAX_STEPS_IN_FLIGHT", "configure_model_norm", "configure_model_all", "create_ema_model", "update_ema_norm", "update_ema_all", "refine_pseudo_labels", "pc2img_logit",
@@ -353,7 +354,7 @@ class LatteStep:
     def __init__(self, model_3d: nn.Module, num_classes: int, hr_cfg: Dict, lr: float = 1e-3, conf_perc=None,
                  lambda_hr_23: float = 0.3, lambda_hr_32: float = 0.3, lambda_ety_ps: float = 1.0, class_weights=None,
                  process_group=None, side_stream: bool = True, fused_optimizer: bool = True, sync_bn: bool = False,
-                 update_params: str = "norm", force_collective: bool = False):
+                 update_params: str = "norm", force_collective: bool = False, activation_checkpoint: str | None = None):
         # update_params: cfg.TRAIN.UPDATE_PARAMS (latte/tta/tta.py:129-138) -- "norm" (every shipped latte.yaml: only the
         # norm layers' gamma / beta train) or "all" (every parameter trains: conv kernels through lt_spconv_bwd_weight)
         self.update_params = str(update_params).lower()
@@ -364,6 +365,10 @@ class LatteStep:
         else:
             raise IndexError(f"Required update params has not been defined yet: {update_params}")   # the reference's error
         self.ema_model, _ = create_ema_model(self.model)
+        # activation_checkpoint = "mx8": the student's BatchNorms keep what their backward pass reads in 8 bits (less memory
+        # between forward and backward; the student walks its module tree, the teacher, which has no backward, does not)
+        if activation_checkpoint is not None:
+            set_activation_checkpoint(self.model, activation_checkpoint)
         self.hr = HR_Block(**hr_cfg)
         self.cr = CR_Block(reduction="mean", conf_mask=True, ety_weight=True)
         if self.update_params == "norm":
