@@ -47,20 +47,21 @@ static int gemm_run(const LtGemm& g, void* ws, int64_t ws_bytes, hipStream_t str
 // four columns, a workgroup a slab of rows; the slabs' sums are joined in a fixed order by k_col_join.
 template <class T, int DK>
 __global__ __launch_bounds__(256) void k_dz(const T* __restrict__ dy, int64_t lddy, const void* __restrict__ deriv, int64_t M,
-                                            int N, int tx, int64_t rows_per, T* __restrict__ dz, T* __restrict__ dz2, float* __restrict__ part,
+                                            int N, int lddz, int tx, int64_t rows_per, T* __restrict__ dz, T* __restrict__ dz2, float* __restrict__ part,
                                             T* __restrict__ db) {
   __shared__ lt_f32x4 s_sum[256];
   const int x = threadIdx.x % tx, yy = threadIdx.x / tx, ty = 256 / tx;
   const int col = (blockIdx.x * tx + x) * 4;
-  const int n = N - col;
+  const int n = N - col, nz = lddz - col;   // lddz > N: zeros behind the columns
   const int64_t r0 = blockIdx.y * rows_per, r1 = r0 + rows_per < M ? r0 + rows_per : M;
   lt_f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  if (n > 0) {
+  if (nz > 0) {
 #pragma unroll 4
     for (int64_t row = r0 + yy; row < r1; row += ty) {
       float g[4], d[4];
       lt_ldv<T, 4>(dy + row * lddy + col, n, g);
-      if constexpr (DK == LT_DERIV_BITS) {
+      if (n <= 0) {   // padding: g is 0
+      } else if constexpr (DK == LT_DERIV_BITS) {
         const unsigned m = ((const uint16_t*)deriv)[row * ((N + 15) >> 4) + (col >> 4)] >> (col & 15);
 #pragma unroll
         for (int i = 0; i < 4; ++i) g[i] = (m >> i) & 1 ? g[i] : 0.f;
@@ -86,12 +87,12 @@ __global__ __launch_bounds__(256) void k_dz(const T* __restrict__ dy, int64_t ld
 #pragma unroll
         for (int i = 0; i < 4; ++i) g[i] *= d[i];
       }
-      if constexpr (DK != LT_DERIV_NONE) lt_stv<T, 4>(dz + row * N + col, n, g);
+      if (DK != LT_DERIV_NONE || dz) lt_stv<T, 4>(dz + row * lddz + col, nz, g);
       if constexpr (sizeof(T) == 2 && (DK == LT_DERIV_BYTE || DK == LT_DERIV_FULL)) {
         if (dz2) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) d[i] = g[i] - (float)(T)g[i];
-          lt_stv<T, 4>(dz2 + row * N + col, n, d);
+          lt_stv<T, 4>(dz2 + row * lddz + col, nz, d);
         }
       }
 #pragma unroll
@@ -130,17 +131,17 @@ static DzPlan dz_plan(int64_t M, int N) {
 }
 
 template <class T>
-static int dz_run(const void* dy, int64_t lddy, const void* deriv, int dkind, int64_t M, int N, void* dz, void* dz2, float* part, void* db,
+static int dz_run(const void* dy, int64_t lddy, const void* deriv, int dkind, int64_t M, int N, int lddz, void* dz, void* dz2, float* part, void* db,
                   hipStream_t stream) {
-  const DzPlan p = dz_plan(M, N);
-  if (p.slabs > 0 && (part || dkind != LT_DERIV_NONE)) {
+  const DzPlan p = dz_plan(M, lddz);
+  if (p.slabs > 0 && (part || dz)) {
     const dim3 grid(p.gx, p.slabs), block(256);
     const T* g = (const T*)dy;
     switch (dkind) {
-      case LT_DERIV_BITS: hipLaunchKernelGGL((k_dz<T, LT_DERIV_BITS>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, (T*)dz2, part, (T*)db); break;
-      case LT_DERIV_BYTE: hipLaunchKernelGGL((k_dz<T, LT_DERIV_BYTE>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, (T*)dz2, part, (T*)db); break;
-      case LT_DERIV_FULL: hipLaunchKernelGGL((k_dz<T, LT_DERIV_FULL>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, (T*)dz2, part, (T*)db); break;
-      default: hipLaunchKernelGGL((k_dz<T, LT_DERIV_NONE>), grid, block, 0, stream, g, lddy, deriv, M, N, p.tx, p.rows_per, (T*)dz, (T*)dz2, part, (T*)db); break;
+      case LT_DERIV_BITS: hipLaunchKernelGGL((k_dz<T, LT_DERIV_BITS>), grid, block, 0, stream, g, lddy, deriv, M, N, lddz, p.tx, p.rows_per, (T*)dz, (T*)dz2, part, (T*)db); break;
+      case LT_DERIV_BYTE: hipLaunchKernelGGL((k_dz<T, LT_DERIV_BYTE>), grid, block, 0, stream, g, lddy, deriv, M, N, lddz, p.tx, p.rows_per, (T*)dz, (T*)dz2, part, (T*)db); break;
+      case LT_DERIV_FULL: hipLaunchKernelGGL((k_dz<T, LT_DERIV_FULL>), grid, block, 0, stream, g, lddy, deriv, M, N, lddz, p.tx, p.rows_per, (T*)dz, (T*)dz2, part, (T*)db); break;
+      default: hipLaunchKernelGGL((k_dz<T, LT_DERIV_NONE>), grid, block, 0, stream, g, lddy, deriv, M, N, lddz, p.tx, p.rows_per, (T*)dz, (T*)dz2, part, (T*)db); break;
     }
     LT_LAUNCH_CHECK();
   }
@@ -276,19 +277,20 @@ struct BwdWs {
 static BwdWs bwd_ws(int64_t M, int K, int N, int dt, bool x8) {
   BwdWs w;
   int64_t off = 0;
+  const LtRowsBwdPlan p = lt_rows_bwd_plan(M, K, N, dt);
+  const int N8 = p.ok ? (N + 7) / 8 * 8 : N;
   w.dz = off;
-  off += lt_align_up(M * N * lt_dt_size(dt), 256);
+  off += lt_align_up(M * N8 * lt_dt_size(dt), 256);
   w.dz2 = off;
   off += two_terms(M, N, dt) ? lt_align_up(M * N * lt_dt_size(dt), 256) : 0;
   w.part = off;
-  off += lt_align_up((int64_t)dz_plan(M, N).slabs * N * 4, 256);
+  off += lt_align_up((int64_t)dz_plan(M, N8).slabs * N * 4, 256);
   w.wide = off;
   if (x8 && widen_first(M, K, N)) off += lt_align_up(M * K * lt_dt_size(dt), 256);
   w.gemm = off;
   const int64_t a = gemm_ws_bytes(M, K, N, dt, false), b = gemm_ws_bytes(N, K, M, dt, false);
   off += a > b ? a : b;
-  const LtRowsBwdPlan p = lt_rows_bwd_plan(M, K, N, dt);
-  const int64_t rows = p.ok ? lt_align_up((int64_t)p.grid * N * K * 4, 256) + (int64_t)p.grid * N * 4 : 0;
+  const int64_t rows = p.ok ? w.gemm + lt_align_up((int64_t)p.grid * N * K * 4, 256) + (int64_t)p.grid * N * 4 : 0;
   w.bytes = off > rows ? off : rows;
   return w;
 }
@@ -314,10 +316,21 @@ extern "C" int lt_linear_bwd(const void* dy, int64_t lddy, const void* x, int64_
   char* wsb = (char*)ws;
   const LtRowsBwdPlan rp = lt_rows_bwd_plan(M, K, N, dt);
   if (rp.ok) {   // whichever gradients are asked for: each has the same bits alone as with the others
-    float* part_w = (float*)wsb;
-    float* part_b = (float*)(wsb + lt_align_up((int64_t)rp.grid * N * K * 4, 256));
-    const LtRowsBwdArgs a = {dy, x, (const uint8_t*)x_scales, w, deriv, lddy, ldx, ldw, deriv_kind, M, N, K, dx, dw ? part_w : nullptr,
-                             db ? part_b : nullptr};
+    float* part_w = (float*)(wsb + o.gemm);
+    float* part_b = (float*)(wsb + o.gemm + lt_align_up((int64_t)rp.grid * N * K * 4, 256));
+    LtRowsBwdArgs a = {dy, x, (const uint8_t*)x_scales, w, deriv, lddy, ldx, ldw, deriv_kind, M, N, K, N, dx, dw ? part_w : nullptr,
+                       db ? part_b : nullptr};
+    if (N % 8) {   // odd widths (class counts): dz and db in a pass of their own, with whole chunks for this one
+      const int N8 = (N + 7) / 8 * 8;
+      LT_DENSE_TYPES(dt, rc = dz_run<T>(dy, lddy, deriv, deriv_kind, M, N, N8, wsb + o.dz, nullptr, db ? (float*)(wsb + o.part) : nullptr, db, stream));
+      if (rc) return rc;
+      a.dy = wsb + o.dz;
+      a.lddy = a.N = N8;
+      a.dkind = LT_DERIV_NONE;
+      a.db = nullptr;
+      db = nullptr;
+      if (!dx && !dw) return LT_OK;
+    }
     LT_DENSE_TYPES(dt, rc = lt_rows_bwd_launch<T>(a, rp, stream));
     if (rc) return rc;
     if (dw) {
@@ -338,7 +351,7 @@ extern "C" int lt_linear_bwd(const void* dy, int64_t lddy, const void* x, int64_
     lddz = N;
   }
   void* dz2 = two_terms(M, N, dt) && (deriv_kind == LT_DERIV_BYTE || deriv_kind == LT_DERIV_FULL) ? wsb + o.dz2 : nullptr;
-  LT_DENSE_TYPES(dt, rc = dz_run<T>(dy, lddy, deriv, deriv_kind, M, N, wsb + o.dz, dz2, db ? (float*)(wsb + o.part) : nullptr, db, stream));
+  LT_DENSE_TYPES(dt, rc = dz_run<T>(dy, lddy, deriv, deriv_kind, M, N, N, deriv_kind != LT_DERIV_NONE ? wsb + o.dz : nullptr, dz2, db ? (float*)(wsb + o.part) : nullptr, db, stream));
   if (rc) return rc;
   LtGemm g = {};
   g.dt = dt;

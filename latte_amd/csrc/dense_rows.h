@@ -75,10 +75,11 @@ struct LtRowsBwdArgs {
   int64_t lddy, ldx, ldw; // elements
   int dkind;
   int64_t M;
-  int N, K;
+  int N, K;               // columns of dy (a multiple of 8) and of x
+  int n_out;              // rows of W, dW and db: N, or less where dy's last columns are padding
   void* dx;               // [M][K] or NULL
-  float* dw;              // [grid][N][K] or NULL
-  float* db;              // [grid][N] or NULL
+  float* dw;              // [grid][n_out][K] or NULL
+  float* db;              // [grid][n_out] or NULL
 };
 
 template <class T, int NP, int KP>
@@ -121,7 +122,7 @@ __global__ __launch_bounds__(1024) void k_rows_bwd(LtRowsBwdArgs a) {
       const int l = i & 63, c = (i >> 6) % kt, f = (i >> 6) / kt, k = 16 * c + (l & 15), n0 = f * KF + (l >> 4) * CH;
       Frag v;
 #pragma unroll
-      for (int j = 0; j < CH; ++j) v[j] = (n0 + j < N && k < K) ? ((const T*)a.w)[(int64_t)(n0 + j) * a.ldw + k] : (T)0.f;
+      for (int j = 0; j < CH; ++j) v[j] = (n0 + j < a.n_out && k < K) ? ((const T*)a.w)[(int64_t)(n0 + j) * a.ldw + k] : (T)0.f;
       *reinterpret_cast<Frag*>(s_w + i * 16) = v;
     }
   }
@@ -280,14 +281,14 @@ __global__ __launch_bounds__(1024) void k_rows_bwd(LtRowsBwdArgs a) {
     do_dx(buf, m0);
     do_dw(buf);
   }
-  float* out = a.dw ? a.dw + (int64_t)blockIdx.x * N * K : nullptr;
+  float* out = a.dw ? a.dw + (int64_t)blockIdx.x * a.n_out * K : nullptr;
 #pragma unroll
   for (int i = 0; i < S::TN; ++i)
 #pragma unroll
     for (int j = 0; j < S::TK; ++j) {
       const int n = 16 * (wn + i) + r, k = 16 * (wk + j) + 4 * g;
       const float v[4] = {dw[i][j][0], dw[i][j][1], dw[i][j][2], dw[i][j][3]};
-      if (out && n < N && k < K) lt_stv<float, 4>(out + (int64_t)n * K + k, K - k, v);
+      if (out && n < a.n_out && k < K) lt_stv<float, 4>(out + (int64_t)n * K + k, K - k, v);
     }
   if (!a.db) return;
   __syncthreads();
@@ -301,11 +302,11 @@ __global__ __launch_bounds__(1024) void k_rows_bwd(LtRowsBwdArgs a) {
       for (int j = 0; j < CH; ++j) s_db[line * NP + c * CH + j] = db[i][j];
   }
   __syncthreads();
-  for (int n = tid; n < N; n += S::NT) {
+  for (int n = tid; n < a.n_out; n += S::NT) {
     float s = 0.f;
 #pragma unroll 8
     for (int l = 0; l < S::R; ++l) s += s_db[l * NP + n];
-    a.db[(int64_t)blockIdx.x * N + n] = s;
+    a.db[(int64_t)blockIdx.x * a.n_out + n] = s;
   }
 }
 
@@ -358,10 +359,13 @@ struct LtRowsBwdPlan {
   bool ok;
   int np, kp, grid, lds;
 };
-static inline LtRowsBwdPlan lt_rows_bwd_plan(int64_t M, int K, int N, int dt) {
+// at least 256 rows (three launches instead of four to six; a 16-bit dz of up to 4096 elements goes in as two terms: dense.hip),
+// widths that are multiples of 8 (N may also be padded: dz is then written out with zeros behind its columns)
+static inline LtRowsBwdPlan lt_rows_bwd_plan(int64_t M, int K, int N_, int dt) {
   LtRowsBwdPlan p = {};
+  const int N = N_ <= 256 ? (N_ + 7) / 8 * 8 : N_;
   auto pad = [](int v) { return v <= 64 ? 64 : v <= 128 ? 128 : 256; };
-  if (N > 256 || K > 256 || N % 8 || K % 8 || M < 2048 || M > (int64_t)1 << 34) return p;
+  if (N > 256 || K > 256 || K % 8 || M < 256 || (dt != LT_DT_F32 && M * N_ <= 4096) || M > (int64_t)1 << 34) return p;
   p.np = pad(N);
   p.kp = pad(K);
   const int sz = lt_dt_size(dt), kf = 64 / sz;   // as in LtRowsBwd, which checks the two against each other

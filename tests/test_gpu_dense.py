@@ -296,7 +296,8 @@ def test_linear_on_another_stream_matches():
 
 
 ROWS = [(8192, 32, 256), (8200, 128, 96), (9001, 96, 20), (8193, 256, 64), (2048, 64, 64), (2049, 33, 65), (3000, 130, 100), (2500, 256, 128),
-        (2100, 100, 256), (20000, 17, 5), (8197, 250, 31)]
+        (2100, 100, 256), (20000, 17, 5), (8197, 250, 31), (256, 64, 17), (300, 128, 96), (3001, 96, 10), (40000, 96, 9),
+        (1000, 256, 250), (2600, 40, 129)]
 
 
 @pytest.mark.parametrize("ckpt", [None, "mx8"])
