@@ -24,8 +24,8 @@ struct LtRmsArgs {
 };
 
 // sum over the LANES lanes of a row, the same bits in each of them
-template <int LANES>
-__device__ __forceinline__ float row_sum(float v, float* s_red) {
+template <int LANES, class F>
+__device__ __forceinline__ F row_sum(F v, F* s_red) {
 #pragma unroll
   for (int o = 1; o < (LANES < 64 ? LANES : 64); o <<= 1) v += __shfl_xor(v, o, 64);
   if constexpr (LANES == 256) {
@@ -37,9 +37,21 @@ __device__ __forceinline__ float row_sum(float v, float* s_red) {
   return v;
 }
 
+// y + c (|c| of a few last places of y) to fp32 with the last bit set where anything is left out: rounding that once more to 4
+// bits is rounding y + c itself.  NaN and infinite parts change nothing.
+__device__ __forceinline__ float round_odd(float y, float c) {
+#pragma clang fp contract(off)   // y is a product and c the rest of it: fused with one another they would count twice
+  const float f = y + c, e = c - (f - y);
+  unsigned b = __float_as_uint(f);
+  const unsigned by = (e > 0.f) == !(b >> 31) ? 1u : ~0u;
+  b += (e > 0.f || e < 0.f) && !(b & 1u) ? by : 0u;
+  return __uint_as_float(b);
+}
+
 template <class T, int LANES, int ITEMS>
 __global__ __launch_bounds__(256) void k_rms_fwd(LtRmsArgs a) {
   __shared__ float s_red[4];
+  __shared__ double s_redd[4];
   constexpr int RPB = 256 / LANES;
   const int l = threadIdx.x % LANES, nb = (a.C + 31) >> 5;
   float w[ITEMS][8];
@@ -67,8 +79,22 @@ __global__ __launch_bounds__(256) void k_rms_fwd(LtRmsArgs a) {
     for (int it = 0; it < ITEMS; ++it)
 #pragma unroll
       for (int t = 0; t < 8; ++t) ss = __fmaf_rn(h[it][t], h[it][t], ss);
-    ss = row_sum<LANES>(ss, s_red);
+    ss = row_sum<LANES, float>(ss, s_red);
     const float rstd = 1.f / sqrtf(ss / (float)a.C + a.eps);
+    // y that is held in 8 bits comes from a 64-bit sum and from products with their rounding errors carried along: the last
+    // bit of an fp32 y would decide between two neighbours some 2^-4 apart once in a million elements (8192 x 4096 bf16: 48 us
+    // in plain fp32, 51 us this way)
+    float rhi = 0.f, rlo = 0.f;
+    if (a.y8) {
+      double s8 = 0.0;
+#pragma unroll
+      for (int it = 0; it < ITEMS; ++it)
+#pragma unroll
+        for (int t = 0; t < 8; ++t) s8 = fma((double)h[it][t], (double)h[it][t], s8);
+      const double r8 = 1.0 / sqrt(row_sum<LANES, double>(s8, s_redd) / (double)a.C + (double)a.eps);
+      rhi = (float)r8;
+      rlo = (float)(r8 - (double)rhi);
+    }
     if (a.rstd && l == 0 && live) a.rstd[row] = rstd;
 #pragma unroll
     for (int it = 0; it < ITEMS; ++it) {
@@ -77,10 +103,20 @@ __global__ __launch_bounds__(256) void k_rms_fwd(LtRmsArgs a) {
       if (a.h) lt_stv<T, 8>((T*)a.h + at, n, h[it]);
       if (a.h8) lt_mx8_put8(h[it], n, 127, a.h8 + at, a.h8s + row * nb + (col >> 5));   // read back in 32 bits
       float y[8];
+      if (a.y) {
 #pragma unroll
-      for (int t = 0; t < 8; ++t) y[t] = h[it][t] * rstd * w[it][t];
-      if (a.y) lt_stv<T, 8>((T*)a.y + at, n, y);
-      if (a.y8) lt_mx8_put8(y, n, LtType<T>::kMaxExp, a.y8 + at, a.y8s + row * nb + (col >> 5));
+        for (int t = 0; t < 8; ++t) y[t] = h[it][t] * rstd * w[it][t];
+        lt_stv<T, 8>((T*)a.y + at, n, y);
+      }
+      if (a.y8) {
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          const float n1 = h[it][t] * rhi, n2 = __fmaf_rn(h[it][t], rlo, __fmaf_rn(h[it][t], rhi, -n1));
+          const float y1 = n1 * w[it][t];
+          y[t] = round_odd(y1, __fmaf_rn(n2, w[it][t], __fmaf_rn(n1, w[it][t], -y1)));
+        }
+        lt_mx8_put8(y, n, LtType<T>::kMaxExp, a.y8 + at, a.y8s + row * nb + (col >> 5));
+      }
     }
   }
 }
@@ -146,7 +182,7 @@ __global__ __launch_bounds__(256) void k_rms_bwd(LtRmsBwdArgs a) {
         g[it][t] *= w[it][t];
         dot = __fmaf_rn(g[it][t], n[it][t], dot);
       }
-    dot = row_sum<LANES>(dot, s_red) / (float)a.C;
+    dot = row_sum<LANES, float>(dot, s_red) / (float)a.C;
     if (!a.dx) continue;
 #pragma unroll
     for (int it = 0; it < ITEMS; ++it) {

@@ -103,6 +103,24 @@ def test_rms_norm_mx8_output(dt):
         assert torch.equal(hs, h32.to(dt))
 
 
+@pytest.mark.parametrize("dt", TYPES)
+def test_rms_norm_mx8_output_is_the_nearest(dt):
+    """the held y is the 64-bit y rounded once: equal to rounding it here, but for elements within 2^-48 of the middle between
+    two neighbours (none among these)"""
+    from latte_amd import functional as LF
+    M, C = 3000, 416
+    x, w = _rn(13, dt, (M, C), (C,))
+    with torch.no_grad():
+        q = LF.rms_norm(x, w, out="mx8", eps=2.0 ** -20)
+    H = x.double()
+    Y = H / torch.sqrt(H.square().mean(1, keepdim=True) + 2.0 ** -20) * w.double()
+    scale = R.two_to(q.scales.to(torch.int64) - 127).repeat_interleave(32, 1)[:, :C]
+    v = Y / scale
+    step = R.two_to((torch.frexp(v.abs())[1] - 4).clamp(min=-9))
+    want = torch.round(v / step) * step * scale
+    assert torch.equal(q.dequantize().double(), want)
+
+
 def test_rms_norm_layouts_and_unused_outputs():
     from latte_amd import functional as LF
     for dt in TYPES:
