@@ -50,6 +50,26 @@ template <> struct LtMma<float> {
   }
 };
 
+// acc[i][j] += P_j Q_i for a block of fragments: fp32 goes round the block four times, so that no
+// instruction waits for the one just before it (k_rows_bwd, 310017 x 128 -> 96, fp32: 240.5 -> 237.8 us)
+template <class T, int FR, int FC>
+__device__ __forceinline__ void lt_mma_block(const typename LtMma<T>::frag (&p)[FC], const typename LtMma<T>::frag (&q)[FR],
+                                             lt_f32x4 (&acc)[FR][FC]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < FR; ++i)
+#pragma unroll
+        for (int j = 0; j < FC; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[j][t], q[i][t], acc[i][j], 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < FR; ++i)
+#pragma unroll
+      for (int j = 0; j < FC; ++j) acc[i][j] = LtMma<T>::mma(p[j], q[i], acc[i][j]);
+  }
+}
+
 template <> struct LtMma<uint8_t> { typedef lt_i32x8 frag; };   // mx8: dense8.h
 
 template <class T, bool KM, int R, int BKB>   // an operand's tile: R rows (or columns) of the product, BKB bytes' worth of k
@@ -323,11 +343,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_dense(LtTileArgs a) {
     ahead();
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-      for (int i = 0; i < FR; ++i)
-#pragma unroll
-        for (int j = 0; j < FC; ++j) acc[i][j] = LtMma<T>::mma(p[kk][j], q[kk][i], acc[i][j]);
+    for (int kk = 0; kk < KK; ++kk) lt_mma_block<T, FR, FC>(p[kk], q[kk], acc);
   };
 
   if constexpr (DIRECT) {

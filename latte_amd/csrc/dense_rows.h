@@ -51,10 +51,13 @@ __global__ __launch_bounds__(512) void k_rows_fwd(LtTileArgs a) {
 #pragma unroll
       for (int j = 0; j < FC; ++j) acc[0][j] = (lt_f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int kk = 0; kk < KC; ++kk)
+      for (int kk = 0; kk < KC; ++kk) {
+        Frag p[FC];
 #pragma unroll
-        for (int j = 0; j < FC; ++j)
-          acc[0][j] = LtMma<T>::mma(*reinterpret_cast<const Frag*>(s_tile + (kk * NT + cg * FC + j) * 1024 + lane * 16), x[kk], acc[0][j]);
+        for (int j = 0; j < FC; ++j) p[j] = *reinterpret_cast<const Frag*>(s_tile + (kk * NT + cg * FC + j) * 1024 + lane * 16);
+        const Frag q[1] = {x[kk]};
+        lt_mma_block<T, 1, FC>(p, q, acc);
+      }
       lt_tile_store_<T, 1, FC, ACT, true>(a, acc, 0, s * 16, cg * 16 * FC, lane, turn);
     }
   }
@@ -64,8 +67,8 @@ __global__ __launch_bounds__(512) void k_rows_fwd(LtTileArgs a) {
 // One pass: a workgroup takes tiles of R rows, forms dz = dy act' on the way into LDS (its column sums stay in registers),
 // and from the two tiles dz [R][N] and x [R][K] its waves compute dx = dz W (W in LDS) and add dz^T x to the workgroup's
 // own dW, which they hold in registers until the end.  dy, act' and x are read once, dz is never written.
-//   310017 x 128 -> 96, fp32: 242 us, half of it the two products at 55 % of the fp32 matrix rate (dz, dx and dW apart: 282
-//   us); bf16: 74 us.
+//   310017 x 128 -> 96, fp32: 238 us, half of it the two products at 55 % of the fp32 matrix rate (dz, dx and dW apart: 282
+//   us); bf16: 73 us.
 struct LtRowsBwdArgs {
   const void* dy;
   const void* x;
@@ -241,33 +244,26 @@ __global__ __launch_bounds__(1024) void k_rows_bwd(LtRowsBwdArgs a) {
 #pragma unroll
     for (int j = 0; j < S::FX; ++j) acc[0][j] = (lt_f32x4){0.f, 0.f, 0.f, 0.f};
     const int m = 16 * strip + r;
-#pragma unroll 2
+#pragma unroll 4
     for (int f = 0; f < nf; ++f) {
       const int c = f * 4 + g;                         // chunk of CH columns n of row m
       const Frag q = *reinterpret_cast<const Frag*>(buf + m * (NP * (int)sizeof(T)) + ((c ^ TZ::kswz(m)) << 4));
 #pragma unroll
-      for (int j = 0; j < S::FX; ++j)
-        if (xg * S::FX + j < kt)
-          acc[0][j] = LtMma<T>::mma(*reinterpret_cast<const Frag*>(s_w + (f * kt + xg * S::FX + j) * 1024 + lane * 16), q, acc[0][j]);
+      for (int j = 0; j < S::FX; ++j)   // (a tile past the last column multiplies whatever lies behind W: it is not stored)
+        acc[0][j] = LtMma<T>::mma(*reinterpret_cast<const Frag*>(s_w + (f * kt + xg * S::FX + j) * 1024 + lane * 16), q, acc[0][j]);
     }
     lt_tile_store_<T, 1, S::FX, LT_ACT_NONE, true>(e, acc, 0, m0 + 16 * strip, 16 * S::FX * xg, lane, turn);
   };
   auto do_dw = [&](const char* buf) {
-    if (!a.dw) return;
+    if (!a.dw || wn >= nt || wk >= kt) return;   // a wave's tiles are all multiplied or none: no branches between the products
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
-      Frag p[S::TK];
+      Frag p[S::TK], q[S::TN];
 #pragma unroll
-      for (int j = 0; j < S::TK; ++j)
-        if (wk + j < kt) p[j] = TX::frag(buf + TZ::BYTES, 16 * (wk + j), kk, lane);
+      for (int j = 0; j < S::TK; ++j) p[j] = TX::frag(buf + TZ::BYTES, 16 * (wk + j), kk, lane);
 #pragma unroll
-      for (int i = 0; i < S::TN; ++i) {
-        if (wn + i >= nt) continue;
-        const Frag q = TZ::frag(buf, 16 * (wn + i), kk, lane);
-#pragma unroll
-        for (int j = 0; j < S::TK; ++j)
-          if (wk + j < kt) dw[i][j] = LtMma<T>::mma(p[j], q, dw[i][j]);
-      }
+      for (int i = 0; i < S::TN; ++i) q[i] = TZ::frag(buf, 16 * (wn + i), kk, lane);
+      lt_mma_block<T, S::TN, S::TK>(p, q, dw);
     }
   };
   int t = blockIdx.x;
