@@ -75,6 +75,13 @@ struct Rows {
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 // the current stream of the tensor's own device, whatever device is current
 lt_stream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+// the shape of a result: x's with the last extent n.  Results are made in it: a view made inside a node could not be
+// changed in place afterwards
+std::vector<int64_t> last(const Tensor& x, int64_t n) {
+  std::vector<int64_t> s(x.sizes().begin(), x.sizes().end());
+  s.back() = n;
+  return s;
+}
 // workspace of one call: torch's allocator (and a graph's private pool) keeps it from any other stream or graph
 Tensor workspace(int64_t bytes, const Tensor& like) { return at::empty({bytes > 256 ? bytes : 256}, like.options().dtype(at::kByte)); }
 
@@ -113,7 +120,7 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, const T
   const int64_t M = x2.n;
   int kind = LT_DERIV_NONE;
   if (act != LT_ACT_NONE && (need & (NEED_X | NEED_W | NEED_B))) kind = act == LT_ACT_RELU ? LT_DERIV_BITS : mx8 ? LT_DERIV_BYTE : LT_DERIV_FULL;
-  Tensor y = at::empty({M, N}, x.options()), deriv;
+  Tensor y = at::empty(last(x, N), x.options()), deriv;
   if (kind == LT_DERIV_BITS) deriv = at::empty({M, (N + 15) / 16}, x.options().dtype(at::kShort));
   else if (kind == LT_DERIV_BYTE) deriv = at::empty({M, N}, x.options().dtype(at::kByte));
   else if (kind == LT_DERIV_FULL) deriv = at::empty({M, N}, x.options().dtype(dt == LT_DT_F32 ? at::kFloat : at::kShort));
@@ -136,10 +143,7 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, const T
     keep->meta = {K, N, kind, ldx, w2.ld, need};
     for (auto s : x.sizes()) keep->meta.push_back(s);
   }
-  if (x.dim() == 2) return y;
-  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
-  shape.back() = N;
-  return y.view(shape);
+  return y;
 }
 
 struct LinearNode : public torch::autograd::Function<LinearNode> {
@@ -184,9 +188,7 @@ Tensor linear(const Tensor& x, const Tensor& w, const std::optional<Tensor>& b_,
   like(w, x, w.sizes(), "linear weight");
   if (b.defined()) like(b, x, {w.size(0)}, "linear bias");
   if (r.defined()) {
-    std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
-    shape.back() = w.size(0);
-    like(r, x, shape, "linear residual");
+    like(r, x, last(x, w.size(0)), "linear residual");
   }
   const int64_t need = needs(x, w, b, r);
   if (!need) return linear_forward(x, w, b, r, act, mx8, 0, nullptr);
@@ -205,8 +207,8 @@ std::pair<Tensor, Tensor> rms_forward(const Tensor& x, const Tensor& w_, const T
   const int64_t C = x.size(-1);
   const Rows x2(x, C), r2(r, C);
   const Tensor w = w_.contiguous();
-  Tensor y = at::empty({x2.n, C}, x.options()), h, h8, h8s, rstd;
-  if (r.defined()) h = at::empty({x2.n, C}, x.options());
+  Tensor y = at::empty(x.sizes(), x.options()), h, h8, h8s, rstd;
+  if (r.defined()) h = at::empty(x.sizes(), x.options());
   if (keep) {
     rstd = at::empty({x2.n}, x.options().dtype(at::kFloat));
     if (mx8) {
@@ -227,10 +229,6 @@ std::pair<Tensor, Tensor> rms_forward(const Tensor& x, const Tensor& w_, const T
     keep->h8s = h8s;
     keep->w = w;
     keep->rstd = rstd;
-  }
-  if (x.dim() != 2) {
-    y = y.view(x.sizes());
-    if (h.defined()) h = h.view(x.sizes());
   }
   return {y, h};
 }
@@ -417,10 +415,10 @@ variable_list rms_norm_mx8(const Tensor& x, const Tensor& w, const std::optional
   const int64_t C = x.size(-1);
   const Rows x2(x, C), r2(r, C);
   Tensor q = at::empty({x2.n, C}, x.options().dtype(at::kFloat8_e4m3fn)), s = at::empty({x2.n, (C + 31) / 32}, x.options().dtype(at::kByte)), h;
-  if (r.defined()) h = at::empty({x2.n, C}, x.options());
+  if (r.defined()) h = at::empty(x.sizes(), x.options());
   check("lt_rms_norm_fwd", lt.rms_fwd(x2.p(), x2.ld, r2.p(), r2.ld, w.contiguous().data_ptr(), (float)eps, x2.n, (int32_t)C, dt, ptr(h), nullptr,
                                       q.data_ptr(), s.data_ptr(), nullptr, nullptr, nullptr, stream_of(x)));
-  if (h.defined()) return {q, s, h.view(x.sizes())};
+  if (h.defined()) return {q, s, h};
   return {q, s};
 }
 

@@ -187,3 +187,29 @@ def test_tta_step_with_checkpoints():
         assert step.ema_model.net_3d.stem[1].checkpoint is None
     for k in losses[0]:
         assert abs(losses[0][k] - losses[1][k]) < 1e-3 * (1 + abs(losses[0][k])), (k, losses)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_results_may_be_changed_in_place(dt):
+    from latte_amd import functional as F
+    g = torch.Generator().manual_seed(9)
+    make = lambda *s: torch.randn(*s, generator=g).to(dt).cuda().requires_grad_()  # noqa: E731
+    x, w, b, r, rw = make(3, 5, 24), make(16, 24), make(16), make(3, 5, 24), make(24)
+    F.linear(x, w, b, act="gelu").mul(2).sum().backward()
+    want = [t.grad.clone() for t in (x, w, b)]
+    x.grad = w.grad = b.grad = None
+    y = F.linear(x, w, b, act="gelu")
+    y.mul_(2)
+    y.sum().backward()
+    assert all(torch.equal(t.grad, v) for t, v in zip((x, w, b), want))
+    x.grad = None
+    y, _ = F.rms_norm(x, rw, r)
+    y.mul(2).sum().backward()
+    want = [t.grad.clone() for t in (x, rw, r)]
+    x.grad = rw.grad = r.grad = None
+    y, h = F.rms_norm(x, rw, r)
+    y.mul_(2)
+    if dt is not torch.float32:   # beside fp32 the sum is what the backward pass reads
+        h.add_(1)
+    y.sum().backward()
+    assert all(torch.equal(t.grad, v) for t, v in zip((x, rw, r), want))
