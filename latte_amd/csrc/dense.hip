@@ -3,7 +3,8 @@
 //   forward    z = x W^T + b (fp32 sums);  y = act(z) + r;  kept: x (or mx8(x)), W, act'(z)
 //   backward   dz = dy act'(z);  dx = dz W;  dW = dz^T x;  db = sum_rows dz;  dr = dy
 // act' is kept instead of z: the ReLU's is one bit, the others fit a uniform grid (8 bits with a checkpoint, |error| <=
-// 1/384; 16 bits beside 16-bit types, 1e-5), and the backward pass needs no exponential.  dz is rounded to the operands' type, as the matrix instructions take it.
+// 1/384; 16 bits beside 16-bit types, 1e-5), and the backward pass needs no exponential.  dz is rounded to the operands'
+// type, as the matrix instructions take it.
 //
 // Replaces the library products of nn.Linear (point branches and heads: latte/models/spvcnn.py:95-111,
 // latte/models/xmuda_arch.py:326-335) where a layer trains or keeps its activations in 8 bits.
@@ -194,7 +195,9 @@ static int check_dense(const char* who, int64_t M, int64_t K, int64_t N, int dt)
   LT_REQUIRE(dt == LT_DT_F32 || dt == LT_DT_BF16 || dt == LT_DT_F16, LT_ERR_ARG, "%s: type %d is none of LT_DT_*", who, dt);
   LT_REQUIRE(M >= 0 && K >= 1 && N >= 1 && K <= INT32_MAX - 1024 && N <= INT32_MAX - 1024, LT_ERR_ARG,
              "%s: bad sizes M=%lld K=%lld N=%lld", who, (long long)M, (long long)K, (long long)N);
-  LT_REQUIRE(M <= (int64_t)1 << 40, LT_ERR_RANGE, "%s: M=%lld is too large", who, (long long)M);
+  const int64_t most = (int64_t)1 << 42;   // elements: more than any memory holds, and byte counts stay within 64 bits
+  LT_REQUIRE(M <= most / (K > N ? K : N) && K <= most / N, LT_ERR_RANGE, "%s: M=%lld K=%lld N=%lld is too large", who, (long long)M,
+             (long long)K, (long long)N);
   return LT_OK;
 }
 

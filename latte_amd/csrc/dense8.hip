@@ -33,8 +33,10 @@ static LtPlan plan8(int64_t M, int K, int N, bool direct) {
 static int64_t part8(const LtPlan& p, int64_t M, int N) { return p.splits > 1 ? p.splits * M * N * 4 : 0; }
 
 static int check8(const char* who, int64_t M, int32_t K, int32_t N) {
-  LT_REQUIRE(M >= 0 && M <= (int64_t)1 << 40 && K >= 1 && N >= 1 && K <= INT32_MAX - 1024 && N <= INT32_MAX - 1024, LT_ERR_ARG,
+  LT_REQUIRE(M >= 0 && K >= 1 && N >= 1 && K <= INT32_MAX - 1024 && N <= INT32_MAX - 1024, LT_ERR_ARG,
              "%s: bad sizes M=%lld K=%d N=%d", who, (long long)M, K, N);
+  const int64_t most = (int64_t)1 << 42;   // elements: more than any memory holds, and byte counts stay within 64 bits
+  LT_REQUIRE(M <= most / (K > N ? K : N) && K <= most / N, LT_ERR_RANGE, "%s: M=%lld K=%d N=%d is too large", who, (long long)M, K, N);
   return LT_OK;
 }
 

@@ -116,3 +116,15 @@ def test_workspaces_cover_every_plan(dt):
             f, b = lib.lt_linear_workspace_bytes(M, K, N, dt), lib.lt_linear_bwd_workspace_bytes(M, K, N, dt, 1)
             assert 0 <= f <= 4 * 256 * max(M, 1) * N + 256 and b >= M * N * (4 if dt == 0 else 2)
             assert b < 20 * (M * (K + N) + 1024 * (K * N + N) + 4096)
+
+
+def test_sizes_past_any_memory_are_refused():
+    """products of the sizes stay within 64 bits: a byte count never wraps round to a small one"""
+    lib = _lib.load()
+    big = (1 << 31) - 2048
+    for M, K, N in ((1 << 40, 1 << 20, 1 << 20), (4, big, big), (1 << 39, 16, 1), (1 << 39, 1, 16)):
+        for dt in (0, 1):
+            assert lib.lt_linear_workspace_bytes(M, K, N, dt) == -1 and b"too large" in lib.lt_last_error()
+            assert lib.lt_linear_bwd_workspace_bytes(M, K, N, dt, 1) == -1
+        assert lib.lt_linear_mx8_workspace_bytes(M, K, N) == -1 and b"too large" in lib.lt_last_error()
+    assert lib.lt_linear_workspace_bytes(1 << 30, 1024, 1024, 1) >= 0
