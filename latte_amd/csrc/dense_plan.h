@@ -26,16 +26,16 @@ static inline LtPlan lt_gemm_plan(int64_t rows, int cols, int64_t depth, int dt,
   const int bk = dt == LT_DT_F32 ? 32 : 64;
   auto tiles = [&](int br, int bc) { return ((rows + br - 1) / br) * ((cols + bc - 1) / bc); };
   int br, bc;
-  // 128 x 128 tiles where they nearly fill the chip, else 64 x 64, four of which share a CU (1777 x 1000 -> 1000 bf16: 26 us
-  // on 112 of the larger, split four ways, 12 us on 448 of the smaller)
   // the widest tile needs the fewest operand bytes a product, and one workgroup a CU: 192 of them, or fewer whose k is long
-  // enough to be split into at least 32 steps each (training 16384 x 1024 -> 4096, bf16:
-  // its dW on 128 x 128 tiles 618 us a step, on 256 x 256 tiles split four ways 554 us)
+  // enough to be split into at least 32 steps each (training 16384 x 1024 -> 4096, bf16: its dW on 128 x 128 tiles 618 us a
+  // step, on 256 x 256 tiles split four ways 554 us)
   const int64_t t256 = tiles(256, 256);
   const bool wide = direct && dt != LT_DT_F32 && cols >= 192 && rows >= 192;
   if (wide && (t256 >= 192 || (t256 >= 16 && depth >= 64 * 32 * (256 / t256)))) p.tile = LT_TILE_256x256, br = 256, bc = 256;
   else if (cols <= 32 && direct) p.tile = LT_TILE_256x32, br = 256, bc = 32;
   else if (cols <= 64 && direct) p.tile = LT_TILE_128x64, br = 128, bc = 64;
+  // 128 x 128 tiles where they nearly fill the chip, else 64 x 64, four of which share a CU (1777 x 1000 -> 1000 bf16: 26 us
+  // on 112 of the larger, split four ways, 12 us on 448 of the smaller)
   else if (tiles(128, 128) >= 224) p.tile = LT_TILE_128x128, br = 128, bc = 128;
   else p.tile = LT_TILE_64x64, br = 64, bc = 64;
   p.tr = (int)((rows + br - 1) / br);

@@ -88,13 +88,12 @@ struct LtRowsBwdArgs {
 template <class T, int NP, int KP>
 struct LtRowsBwd {
   // rows a tile, the k of dW's product: about 16 KB each of dz and x, so that what a tile waits for memory is small beside
-  // what it moves (310017 x 64 -> 64 bf16: 84 us in tiles of 32 rows, 42 in
-  // tiles of 128)
+  // what it moves (310017 x 64 -> 64 bf16: 84 us in tiles of 32 rows, 42 in tiles of 128)
   static constexpr int R = NP * KP == 64 * 64 ? 256 / sizeof(T) : sizeof(T) == 2 && NP + KP <= 256 ? 64 : 32;
   static constexpr int CH = 16 / sizeof(T), BKB = R * sizeof(T);
   typedef LtTile<T, true, NP, BKB> TZ;
   typedef LtTile<T, true, KP, BKB> TX;
-  static constexpr int NT = 1024;   // 16 waves: with 8 the LDS latencies showed (128 -> 96 fp32: 261 us, with 16 222)
+  static constexpr int NT = 1024;   // 16 waves: with 8 the LDS latencies showed (128 -> 96 fp32 took 39 us more)
   static constexpr int NZ = (TZ::BYTES / 16 + NT - 1) / NT, NX = (TX::BYTES / 16 + NT - 1) / NT;
   static constexpr int TN = NP / 64, TK = KP / 64;                  // the waves' 4 x 4 grid over dW: 16 x 16 tiles a wave
   static constexpr int SX = R / 16, GX = 16 / SX;                   // dx: SX strips x GX column groups
