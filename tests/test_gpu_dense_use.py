@@ -213,3 +213,44 @@ def test_results_may_be_changed_in_place(dt):
         h.add_(1)
     y.sum().backward()
     assert all(torch.equal(t.grad, v) for t, v in zip((x, rw, r), want))
+
+
+def test_checkpoints_with_cross_rank_statistics():
+    """one rank, a real collective: the statistics go through fp64 sums and come back within an fp32 rounding, so the result
+    and its gradients are those of the local path (a few roundings of 2^-24, each on terms no larger than the largest); a
+    rank without rows takes part in both collectives"""
+    import os
+    import socket
+
+    import torch.distributed as dist
+    from latte_amd import functional as LF
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    C = 40
+    gamma, beta = (t.requires_grad_() for t in _rn(31, torch.float32, (C,), (C,)))
+
+    def run(rows, **kw):
+        x, r, dy = _rn(32 + rows, torch.float32, (rows, C), (rows, C), (rows, C))
+        leaves = [x.requires_grad_(), gamma, beta, r.requires_grad_()]
+        y = LF.batch_norm(x, gamma, beta, residual=r, relu=True, **kw)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+    want = run(700, checkpoint="mx8")
+    dist.init_process_group("gloo", rank=0, world_size=1, init_method=f"tcp://127.0.0.1:{port}")
+    calls, real = [], LF._allreduce_small
+    LF._allreduce_small = lambda t, g: (calls.append(t.numel()), real(t, g))[1]
+    LF.SYNC_BN_GROUP = dist.group.WORLD
+    try:
+        got, plain = run(700, checkpoint="mx8"), run(700)
+        assert torch.equal(got[0], plain[0]) and calls == [2 * C + 1, 2 * C] * 2
+        for a, b in zip(got, want):
+            assert (a - b).abs().max() <= 64 * 2.0 ** -24 * b.abs().max()
+        for rows in (0, 1):
+            calls.clear()
+            out = run(rows, checkpoint="mx8")
+            assert calls == [2 * C + 1, 2 * C] and out[0].shape == out[1].shape == (rows, C)
+            assert all(torch.isfinite(t).all() for t in out)
+    finally:
+        LF.SYNC_BN_GROUP = None
+        LF._allreduce_small = real
+        dist.destroy_process_group()
