@@ -4,6 +4,7 @@
 // interpreter code on two threads that hand the interpreter lock to each other; the device needs 20 to 40 us for the same.
 // The entry points come from the library that latte_amd._lib has loaded (init), so this module links none of them.
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
@@ -101,7 +102,22 @@ enum { NEED_X = 1, NEED_W = 2, NEED_B = 4, NEED_R = 8 };
 int64_t needs(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r) {
   if (!at::GradMode::is_enabled()) return 0;
   auto need = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
-  return (need(x) ? NEED_X : 0) | (need(w) ? NEED_W : 0) | (need(b) ? NEED_B : 0) | (need(r) ? NEED_R : 0);
+  const int64_t n = (need(x) ? NEED_X : 0) | (need(w) ? NEED_W : 0) | (need(b) ? NEED_B : 0) | (need(r) ? NEED_R : 0);
+  if (!n) return 0;
+  // While an eager graph of a leaf lives, the leaf's gradient is accumulated on that graph's stream.  A captured backward
+  // pass would make that stream wait for the capturing one, which ends the capture and the process with it.
+  const c10::DeviceGuard on(x.device());
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
+    const c10::StreamId here = c10::hip::getCurrentHIPStream(x.get_device()).id();   // the same id under torch's device name
+    for (const Tensor* t : {&x, &w, &b, &r}) {
+      if (!need(*t) || !t->is_leaf()) continue;
+      const auto acc = torch::autograd::impl::try_get_grad_accumulator(*t);
+      const auto stream = acc ? acc->stream() : std::optional<c10::Stream>();
+      TORCH_CHECK(!stream || stream->id() == here, "a backward pass of this leaf can not be captured: a graph made on another stream still holds it; "
+                  "let go of that graph's results first");
+    }
+  }
+  return n;
 }
 
 // ------------------------------------------------------------------ linear

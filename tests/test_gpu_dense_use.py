@@ -254,3 +254,33 @@ def test_checkpoints_with_cross_rank_statistics():
         LF.SYNC_BN_GROUP = None
         LF._allreduce_small = real
         dist.destroy_process_group()
+
+
+def test_capture_is_refused_while_an_eager_graph_holds_a_leaf():
+    from latte_amd import functional as LF
+    x, w, g = (t.requires_grad_() for t in _rn(41, torch.float32, (64, 32), (48, 32), (32,)))
+
+    def step():
+        return LF.linear(x, w, act="relu", checkpoint="mx8"), LF.rms_norm(x, g), LF.batch_norm(x, g, g, checkpoint="mx8")
+    dys = _rn(42, torch.float32, (64, 48), (64, 32), (64, 32))
+    want = torch.autograd.grad(step(), [x, w, g], dys)
+    held = step()
+    for leaf in (lambda: LF.linear(x, w), lambda: LF.rms_norm(x, g), lambda: LF.batch_norm(x, g, g, checkpoint="mx8")):
+        graph = torch.cuda.CUDAGraph()
+        dead = torch.zeros(1, device="cuda")
+        with pytest.raises(RuntimeError, match="still holds it"):
+            with torch.cuda.graph(graph):
+                dead.add_(1)   # a graph of something: the refused call has recorded nothing
+                leaf()
+        with torch.no_grad():   # no backward pass, nothing to refuse
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                leaf()
+    del held
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = torch.autograd.grad(step(), [x, w, g], dys)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        step()
