@@ -75,16 +75,10 @@ __global__ __launch_bounds__(256) void k_rms_fwd(LtRmsArgs a) {
         for (int t = 0; t < 8; ++t) h[it][t] += r[t];
       }
     }
-#pragma unroll
-    for (int it = 0; it < ITEMS; ++it)
-#pragma unroll
-      for (int t = 0; t < 8; ++t) ss = __fmaf_rn(h[it][t], h[it][t], ss);
-    ss = row_sum<LANES, float>(ss, s_red);
-    const float rstd = 1.f / sqrtf(ss / (float)a.C + a.eps);
     // y that is held in 8 bits comes from a 64-bit sum and from products with their rounding errors carried along: the last
     // bit of an fp32 y would decide between two neighbours some 2^-4 apart once in a million elements (8192 x 4096 bf16: 48 us
-    // in plain fp32, 51 us this way)
-    float rhi = 0.f, rlo = 0.f;
+    // in plain fp32, 49 us this way)
+    float rstd, rhi = 0.f, rlo = 0.f;
     if (a.y8) {
       double s8 = 0.0;
 #pragma unroll
@@ -92,8 +86,15 @@ __global__ __launch_bounds__(256) void k_rms_fwd(LtRmsArgs a) {
 #pragma unroll
         for (int t = 0; t < 8; ++t) s8 = fma((double)h[it][t], (double)h[it][t], s8);
       const double r8 = 1.0 / sqrt(row_sum<LANES, double>(s8, s_redd) / (double)a.C + (double)a.eps);
-      rhi = (float)r8;
+      rstd = rhi = (float)r8;
       rlo = (float)(r8 - (double)rhi);
+    } else {
+#pragma unroll
+      for (int it = 0; it < ITEMS; ++it)
+#pragma unroll
+        for (int t = 0; t < 8; ++t) ss = __fmaf_rn(h[it][t], h[it][t], ss);
+      ss = row_sum<LANES, float>(ss, s_red);
+      rstd = 1.f / sqrtf(ss / (float)a.C + a.eps);
     }
     if (a.rstd && l == 0 && live) a.rstd[row] = rstd;
 #pragma unroll
