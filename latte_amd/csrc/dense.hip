@@ -123,6 +123,7 @@ static DzPlan dz_plan(int64_t M, int N) {
   p.gx = (cg + p.tx - 1) / p.tx;
   const int ty = 256 / p.tx;
   int64_t s = (2048 + p.gx - 1) / p.gx, most = (M + ty * 4 - 1) / (ty * 4);   // four rows a thread at least
+  if (M <= ty * 16) most = 1;   // one slab is db: no join to launch (64 x 128 -> 128 bf16, a training step: 70.4 -> 66.0 us)
   if (s > most) s = most;
   if (s < 1) s = 1;
   p.rows_per = (M + s - 1) / s;

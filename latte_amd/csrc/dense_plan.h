@@ -28,7 +28,8 @@ static inline LtPlan lt_gemm_plan(int64_t rows, int cols, int64_t depth, int dt,
   int br, bc;
   // the widest tile needs the fewest operand bytes a product, and one workgroup a CU: 192 of them, or fewer whose k is long
   // enough to be split into at least 32 steps each (training 16384 x 1024 -> 4096, bf16: its dW on 128 x 128 tiles 618 us a
-  // step, on 256 x 256 tiles split four ways 554 us)
+  // step, on 256 x 256 tiles split four ways 554 us).  256 x 128 tiles, also one a CU, lose to two of 128 x 128 (training
+  // 4096 x 2048 -> 2048, bf16: 187 us a step and 146).
   const int64_t t256 = tiles(256, 256);
   const bool wide = direct && dt != LT_DT_F32 && cols >= 192 && rows >= 192;
   if (wide && (t256 >= 192 || (t256 >= 16 && depth >= 64 * 32 * (256 / t256)))) p.tile = LT_TILE_256x256, br = 256, bc = 256;
