@@ -307,6 +307,7 @@ struct LtGemm {
   int cols;
   int dt;
   bool p_kmajor, q_kmajor;
+  bool padded;               // 16-byte pieces that reach past a line's end read zeros (or nothing that an output takes)
   const uint8_t* p_scales;   // P is mx8 (k-major only): e4m3 values [k][ldp], scales [k][ceil(cols/32)]
   int act;
   LtEpi epi;

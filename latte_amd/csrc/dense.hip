@@ -21,6 +21,23 @@ static int64_t part_bytes(const LtPlan& p, int64_t rows, int cols) {
   return p.splits > 1 ? lt_align_up(p.splits * rows * cols * 4, 256) : 0;
 }
 
+// Lines whose length is no multiple of 16 bytes are staged through registers, in 128 x 128 tiles at most.  A large product is
+// worth a copy of its operands with their lines filled up by zeros: whole pieces go straight into LDS.  TFLOP/s measured
+// without and with (beside the copies): 16 bits forward 480 and 700, backward 240 and 700; fp32 backward 78 and 103, forward alike.
+// 9000 x 1001 -> 4001 fp16: forward 150 us as it is, 129 with the copies, a training step 786 and 359 (fp32 2539 and 2196); 3000 x
+// 1001 -> 1003 fp16: 108 and 86.
+static bool pad_pays(double products, double copied, int dt, double as_is, double filled) {
+  const double gain = 2e-6 * products * (1 / as_is - 1 / filled);   // us
+  return gain > 10 + 1e6 * copied * 2 * lt_dt_size(dt) / 3.5e12;    // two launches, a read and a write of `copied` elements
+}
+static int64_t up_to_16(int64_t n, int dt) {
+  const int64_t ch = 16 / lt_dt_size(dt);
+  return (n + ch - 1) / ch * ch;
+}
+static bool pad_fwd(int64_t M, int K, int N, int dt) {
+  return dt != LT_DT_F32 && up_to_16(K, dt) != K && pad_pays((double)M * N * K, (double)(M + N) * K, dt, 480, 700);
+}
+
 // the larger of what the two staging paths want: which one runs depends on the operands' alignment
 static int64_t gemm_ws_bytes(int64_t rows, int cols, int64_t depth, int dt, bool nn) {
   const int64_t a = part_bytes(lt_gemm_plan(rows, cols, depth, dt, nn, true, true), rows, cols);
@@ -28,11 +45,33 @@ static int64_t gemm_ws_bytes(int64_t rows, int cols, int64_t depth, int dt, bool
   return a > b ? a : b;
 }
 
+// rows of n elements -> rows of ldo >= n, filled up with zeros.  HBM-bound; a thread takes eight neighbours.
+template <class T>
+__global__ __launch_bounds__(256) void k_pad(const T* __restrict__ x, int64_t ldx, int64_t M, int n, int ldo, T* __restrict__ out) {
+  const int L = (ldo + 7) >> 3;
+  const int64_t total = M * L, stride = (int64_t)gridDim.x * 256;
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < total; i += stride) {
+    int64_t row;
+    int l;
+    lt_divmod(i, L, row, l);
+    float v[8];
+    lt_ldv<T, 8>(x + row * ldx + l * 8, n - l * 8, v);
+    lt_stv<T, 8>(out + row * ldo + l * 8, ldo - l * 8, v);
+  }
+}
+static int pad_run(const void* x, int64_t ldx, int64_t M, int n, int dt, void* out, hipStream_t stream) {
+  const int ldo = (int)up_to_16(n, dt);
+  LT_DENSE_TYPES(dt, hipLaunchKernelGGL((k_pad<T>), dim3(lt_grid(M * ((ldo + 7) >> 3), 256)), dim3(256), 0, stream, (const T*)x, ldx, M,
+                                        n, ldo, (T*)out));
+  LT_LAUNCH_CHECK();
+  return LT_OK;
+}
+
 static int gemm_run(const LtGemm& g, void* ws, int64_t ws_bytes, hipStream_t stream) {
   const int sz = lt_dt_size(g.dt), ch = 16 / sz;
   auto aligned = [&](const void* p, int64_t ld, int64_t run, bool kmajor) {
     // whole 16-byte chunks along memory, and a tile's offsets within the 31 bits of a buffer descriptor
-    return ((uintptr_t)p & 15) == 0 && ld * sz % 16 == 0 && run % ch == 0 && (kmajor ? 64 : 256) * ld * sz < (int64_t)1 << 31;
+    return ((uintptr_t)p & 15) == 0 && ld * sz % 16 == 0 && (run % ch == 0 || g.padded) && (kmajor ? 64 : 256) * ld * sz < (int64_t)1 << 31;
   };
   const bool direct = !g.p_scales && aligned(g.P, g.ldp, g.p_kmajor ? g.cols : g.depth, g.p_kmajor) &&
                       aligned(g.Q, g.ldq, g.q_kmajor ? g.rows : g.depth, g.q_kmajor);
@@ -176,7 +215,7 @@ __global__ __launch_bounds__(256) void k_mx8_quantize(const T* __restrict__ x, i
 
 template <class T>
 __global__ __launch_bounds__(256) void k_mx8_dequantize(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sc, int64_t M,
-                                                        int K, T* __restrict__ out) {
+                                                        int K, int ldo, T* __restrict__ out) {
   const int nb = (K + 31) >> 5, L = nb * 4;
   const int64_t n = M * L, stride = (int64_t)gridDim.x * 256;
   for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += stride) {
@@ -187,7 +226,7 @@ __global__ __launch_bounds__(256) void k_mx8_dequantize(const uint8_t* __restric
     if (m <= 0) continue;
     float v[8];
     lt_mx8_get8(q + row * K + col, m, sc[row * nb + (l >> 2)], v);
-    lt_stv<T, 8>(out + row * K + col, m, v);
+    lt_stv<T, 8>(out + row * ldo + col, ldo - col, v);   // ldo > K: zeros behind the row
   }
 }
 
@@ -217,6 +256,14 @@ extern "C" int lt_mx8_quantize(const void* x, int64_t ldx, int64_t M, int32_t K,
   return LT_OK;
 }
 
+static int dequantize_run(const void* values, const void* scales, int64_t M, int K, int ldo, int dt, void* out, hipStream_t stream) {
+  const int64_t n = M * (int64_t)((K + 31) / 32 * 4);
+  LT_DENSE_TYPES(dt, hipLaunchKernelGGL((k_mx8_dequantize<T>), dim3(lt_grid(n, 256)), dim3(256), 0, stream, (const uint8_t*)values,
+                                        (const uint8_t*)scales, M, K, ldo, (T*)out));
+  LT_LAUNCH_CHECK();
+  return LT_OK;
+}
+
 extern "C" int lt_mx8_dequantize(const void* values, const void* scales, int64_t M, int32_t K, int32_t dt, void* out,
                                  hipStream_t stream) {
   int rc = check_dense("lt_mx8_dequantize", M, K, 1, dt);
@@ -225,16 +272,13 @@ extern "C" int lt_mx8_dequantize(const void* values, const void* scales, int64_t
   LT_REQUIRE(out && values && scales, LT_ERR_ARG, "lt_mx8_dequantize: null pointer");
   LtOnStream on;
   if ((rc = on.enter(stream))) return rc;
-  const int64_t n = M * (int64_t)((K + 31) / 32 * 4);
-  LT_DENSE_TYPES(dt, hipLaunchKernelGGL((k_mx8_dequantize<T>), dim3(lt_grid(n, 256)), dim3(256), 0, stream, (const uint8_t*)values,
-                                        (const uint8_t*)scales, M, K, (T*)out));
-  LT_LAUNCH_CHECK();
-  return LT_OK;
+  return dequantize_run(values, scales, M, K, K, dt, out, stream);
 }
 
 extern "C" int64_t lt_linear_workspace_bytes(int64_t M, int32_t K, int32_t N, int32_t dt) {
   if (check_dense("lt_linear_workspace_bytes", M, K, N, dt)) return -1;
-  return gemm_ws_bytes(M, N, K, dt, true);
+  const int64_t pad = pad_fwd(M, K, N, dt) ? lt_align_up((M + N) * up_to_16(K, dt) * lt_dt_size(dt), 256) : 0;
+  return pad + gemm_ws_bytes(M, N, K, dt, true);
 }
 
 extern "C" int lt_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res,
@@ -261,7 +305,19 @@ extern "C" int lt_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t 
   g.dt = dt;
   g.act = act;
   g.epi = LtEpi{bias, res, ldres, y, N, deriv, deriv_kind, M, N};
-  return gemm_run(g, ws, ws ? ws_bytes : 0, stream);
+  ws_bytes = ws ? ws_bytes : 0;
+  if (pad_fwd(M, K, N, dt)) {
+    const int64_t K8 = up_to_16(K, dt), row = K8 * lt_dt_size(dt), pad = lt_align_up((M + N) * row, 256);
+    LT_REQUIRE(pad <= ws_bytes, LT_ERR_WORKSPACE, "lt_linear_fwd: workspace too small (%lld bytes)", (long long)ws_bytes);
+    if ((rc = pad_run(w, ldw, N, K, dt, ws, stream)) || (rc = pad_run(x, ldx, M, K, dt, (char*)ws + N * row, stream))) return rc;
+    g.P = ws;
+    g.Q = (char*)ws + N * row;
+    g.ldp = g.ldq = K8;
+    g.padded = true;
+    ws = (char*)ws + pad;
+    ws_bytes -= pad;
+  }
+  return gemm_run(g, ws, ws_bytes, stream);
 }
 
 // dW = dz^T x with x in mx8: up to 256 output columns the product widens x while it stages it (x is read once or twice);
@@ -274,23 +330,33 @@ static bool widen_first(int64_t M, int K, int N) { return N > 256 && M > 0; }
 // what its rounding left (the products are launch-bound there).
 static bool two_terms(int64_t M, int N, int dt) { return dt != LT_DT_F32 && M * N <= 4096; }
 
+// the backward pass's dz, x and W with their lines filled up (dz comes that way at no cost where there is an act')
+static bool pad_bwd(int64_t M, int K, int N, int dt) {
+  const bool k = up_to_16(K, dt) != K, n = up_to_16(N, dt) != N;
+  return (k || n) && pad_pays(2.0 * M * N * K, (k ? (double)(M + N) * K : 0.0) + (n ? (double)M * N : 0.0), dt,
+                              dt == LT_DT_F32 ? 78 : 240, dt == LT_DT_F32 ? 103 : 700);
+}
+
 struct BwdWs {
-  int64_t dz, dz2, part, wide, gemm, bytes;
+  int64_t dz, dz2, part, wide, w, gemm, bytes;
 };
 // the larger of the two routes: one pass over the rows, or dz and two products
 static BwdWs bwd_ws(int64_t M, int K, int N, int dt, bool x8) {
   BwdWs w;
   int64_t off = 0;
   const LtRowsBwdPlan p = lt_rows_bwd_plan(M, K, N, dt);
-  const int N8 = p.ok ? (N + 7) / 8 * 8 : N;
+  const bool pad = !p.ok && pad_bwd(M, K, N, dt);
+  const int64_t N8 = p.ok ? (N + 7) / 8 * 8 : pad ? up_to_16(N, dt) : N, K8 = pad ? up_to_16(K, dt) : K;
   w.dz = off;
   off += lt_align_up(M * N8 * lt_dt_size(dt), 256);
   w.dz2 = off;
   off += two_terms(M, N, dt) ? lt_align_up(M * N * lt_dt_size(dt), 256) : 0;
   w.part = off;
-  off += lt_align_up((int64_t)dz_plan(M, N8).slabs * N * 4, 256);
+  off += lt_align_up((int64_t)dz_plan(M, (int)N8).slabs * N * 4, 256);
   w.wide = off;
-  if (x8 && widen_first(M, K, N)) off += lt_align_up(M * K * lt_dt_size(dt), 256);
+  if ((x8 && (widen_first(M, K, N) || pad)) || K8 != K) off += lt_align_up(M * K8 * lt_dt_size(dt), 256);
+  w.w = off;
+  if (K8 != K) off += lt_align_up(N * K8 * lt_dt_size(dt), 256);
   w.gemm = off;
   const int64_t a = gemm_ws_bytes(M, K, N, dt, false), b = gemm_ws_bytes(N, K, M, dt, false);
   off += a > b ? a : b;
@@ -348,22 +414,31 @@ extern "C" int lt_linear_bwd(const void* dy, int64_t lddy, const void* x, int64_
     }
     return LT_OK;
   }
+  const bool pad = pad_bwd(M, K, N, dt);
+  const int N8 = pad ? (int)up_to_16(N, dt) : N, K8 = pad ? (int)up_to_16(K, dt) : K;
   const void* dz = dy;
   int64_t lddz = lddy;
-  if (deriv_kind != LT_DERIV_NONE) {
+  const bool own_dz = deriv_kind != LT_DERIV_NONE || N8 != N;
+  if (own_dz) {
     dz = wsb + o.dz;
-    lddz = N;
+    lddz = N8;
   }
   void* dz2 = two_terms(M, N, dt) && (deriv_kind == LT_DERIV_BYTE || deriv_kind == LT_DERIV_FULL) ? wsb + o.dz2 : nullptr;
-  LT_DENSE_TYPES(dt, rc = dz_run<T>(dy, lddy, deriv, deriv_kind, M, N, N, deriv_kind != LT_DERIV_NONE ? wsb + o.dz : nullptr, dz2, db ? (float*)(wsb + o.part) : nullptr, db, stream));
+  LT_DENSE_TYPES(dt, rc = dz_run<T>(dy, lddy, deriv, deriv_kind, M, N, N8, own_dz ? wsb + o.dz : nullptr, dz2, db ? (float*)(wsb + o.part) : nullptr, db, stream));
   if (rc) return rc;
   LtGemm g = {};
   g.dt = dt;
   g.act = LT_ACT_NONE;
   g.Q2 = dz2;
+  g.padded = pad;
   if (dx && M > 0) {
     g.P = w;
     g.ldp = ldw;
+    if (K8 != K) {
+      if ((rc = pad_run(w, ldw, N, K, dt, wsb + o.w, stream))) return rc;
+      g.P = wsb + o.w;
+      g.ldp = K8;
+    }
     g.p_kmajor = true;
     g.Q = dz;
     g.ldq = lddz;
@@ -378,11 +453,15 @@ extern "C" int lt_linear_bwd(const void* dy, int64_t lddy, const void* x, int64_
     g.ldp = ldx;
     g.p_kmajor = true;
     g.p_scales = (const uint8_t*)x_scales;
-    if (x_scales && widen_first(M, K, N)) {
-      if ((rc = lt_mx8_dequantize(x, x_scales, M, K, dt, wsb + o.wide, stream))) return rc;
+    if (x_scales && (widen_first(M, K, N) || pad)) {
+      if ((rc = dequantize_run(x, x_scales, M, K, K8, dt, wsb + o.wide, stream))) return rc;
       g.P = wsb + o.wide;
-      g.ldp = K;
+      g.ldp = K8;
       g.p_scales = nullptr;
+    } else if (K8 != K) {
+      if ((rc = pad_run(x, ldx, M, K, dt, wsb + o.wide, stream))) return rc;
+      g.P = wsb + o.wide;
+      g.ldp = K8;
     }
     g.Q = dz;
     g.ldq = lddz;

@@ -310,3 +310,40 @@ def test_linear_long_and_narrow(size, dt, ckpt):
     x, w, b, r, dy = _inputs(*size, dt, seed=12)
     _check_linear(x, w, b, None, dy, "silu", ckpt)
     _check_linear(x[:, 1:], w[:, 1:], None, r, dy, "none", ckpt) if size[1] > 1 else None
+
+
+@pytest.mark.parametrize("ckpt", [None, "mx8"])
+@pytest.mark.parametrize("dt", TYPES)
+def test_linear_large_odd_sizes(dt, ckpt):
+    """lines that are no multiple of 16 bytes, large enough for copies with their lines filled up"""
+    for M, K, N in ((2500, 1001, 1003), (2300, 1002, 1100)) if dt is torch.float32 else ((9000, 1001, 1505), (9001, 1000, 1503), (8999, 1003, 1504)):
+        x, w, b, r, dy = _inputs(M, K, N, dt, seed=4)
+        _check_linear(x, w, b, r, dy, "gelu" if K == 1001 else "none", ckpt)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_linear_large_odd_sizes_layouts_and_values(dt):
+    """the same from strided operands, and non-finite values that stay in their rows and columns; each gradient alone has the same bits"""
+    from latte_amd import functional as LF
+    M, K, N = (2500, 1001, 1003) if dt is torch.float32 else (9000, 1001, 1505)
+    x, w, b, r, dy = _inputs(M, K, N, dt, seed=5)
+    wide = torch.full((M, K + 6), float("nan"), device="cuda", dtype=dt)
+    wide[:, 3:K + 3] = x
+    xs, ws, dys = wide[:, 3:K + 3], w.t().contiguous().t(), torch.cat([dy, dy], 1)[:, N:]
+    out = []
+    for a, c, d in ((x, w, dy), (xs, ws, dys)):
+        a, c = a.requires_grad_(True), c.requires_grad_(True)
+        y = LF.linear(a, c, b, act="silu")
+        both = torch.autograd.grad(y, (a, c), d, retain_graph=True)
+        assert torch.equal(both[1], torch.autograd.grad(y, c, d, retain_graph=True)[0])
+        assert torch.equal(both[0], torch.autograd.grad(y, a, d)[0])
+        out.append((y.detach(), *both))
+    assert all(torch.equal(p, q) for p, q in zip(*out))
+    x2, dy2 = x.detach().clone(), dy.clone()
+    x2[7, K - 1], dy2[11, N - 1] = float("nan"), float("inf")
+    x2.requires_grad_(True)
+    y = LF.linear(x2, w, b)
+    assert torch.isnan(y[7]).all() and torch.isfinite(y).all(1).sum() == M - 1
+    gx, gw = torch.autograd.grad(y, (x2, w), dy2)
+    assert (~torch.isfinite(gx)).any(1).nonzero().flatten().tolist() == [11]
+    assert (~torch.isfinite(gw[:-1])).any(0).nonzero().flatten().tolist() == [K - 1] and not torch.isfinite(gw[-1]).any()
