@@ -331,9 +331,9 @@ static bool widen_first(int64_t M, int K, int N) { return N > 256 && M > 0; }
 static bool two_terms(int64_t M, int N, int dt) { return dt != LT_DT_F32 && M * N <= 4096; }
 
 // the backward pass's dz, x and W with their lines filled up (dz comes that way at no cost where there is an act')
-static bool pad_bwd(int64_t M, int K, int N, int dt) {
+static bool pad_bwd(int64_t M, int K, int N, int dt, bool has_act) {
   const bool k = up_to_16(K, dt) != K, n = up_to_16(N, dt) != N;
-  return (k || n) && pad_pays(2.0 * M * N * K, (k ? (double)(M + N) * K : 0.0) + (n ? (double)M * N : 0.0), dt,
+  return (k || n) && pad_pays(2.0 * M * N * K, (k ? (double)(M + N) * K : 0.0) + (n && !has_act ? (double)M * N : 0.0), dt,
                               dt == LT_DT_F32 ? 78 : 240, dt == LT_DT_F32 ? 103 : 700);
 }
 
@@ -345,14 +345,15 @@ static BwdWs bwd_ws(int64_t M, int K, int N, int dt, bool x8) {
   BwdWs w;
   int64_t off = 0;
   const LtRowsBwdPlan p = lt_rows_bwd_plan(M, K, N, dt);
-  const bool pad = !p.ok && pad_bwd(M, K, N, dt);
+  const bool pad = !p.ok && pad_bwd(M, K, N, dt, true);   // with an act' more often than without
   const int64_t N8 = p.ok ? (N + 7) / 8 * 8 : pad ? up_to_16(N, dt) : N, K8 = pad ? up_to_16(K, dt) : K;
   w.dz = off;
   off += lt_align_up(M * N8 * lt_dt_size(dt), 256);
   w.dz2 = off;
   off += two_terms(M, N, dt) ? lt_align_up(M * N * lt_dt_size(dt), 256) : 0;
   w.part = off;
-  off += lt_align_up((int64_t)dz_plan(M, (int)N8).slabs * N * 4, 256);
+  const int64_t s = dz_plan(M, N).slabs, s8 = dz_plan(M, (int)N8).slabs;
+  off += lt_align_up((s > s8 ? s : s8) * N * 4, 256);
   w.wide = off;
   if ((x8 && (widen_first(M, K, N) || pad)) || K8 != K) off += lt_align_up(M * K8 * lt_dt_size(dt), 256);
   w.w = off;
@@ -414,7 +415,7 @@ extern "C" int lt_linear_bwd(const void* dy, int64_t lddy, const void* x, int64_
     }
     return LT_OK;
   }
-  const bool pad = pad_bwd(M, K, N, dt);
+  const bool pad = pad_bwd(M, K, N, dt, deriv_kind != LT_DERIV_NONE);
   const int N8 = pad ? (int)up_to_16(N, dt) : N, K8 = pad ? (int)up_to_16(K, dt) : K;
   const void* dz = dy;
   int64_t lddz = lddy;

@@ -347,3 +347,11 @@ def test_linear_large_odd_sizes_layouts_and_values(dt):
     gx, gw = torch.autograd.grad(y, (x2, w), dy2)
     assert (~torch.isfinite(gx)).any(1).nonzero().flatten().tolist() == [11]
     assert (~torch.isfinite(gw[:-1])).any(0).nonzero().flatten().tolist() == [K - 1] and not torch.isfinite(gw[-1]).any()
+
+
+@pytest.mark.parametrize("act", ["none", "silu", "relu"])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_linear_long_with_many_odd_columns(dt, act):
+    """an odd number of columns, few inputs: dz comes with its lines filled up where there is an act', dy as it is else"""
+    x, w, b, r, dy = _inputs(40001, 96, 511, dt, seed=6, exact=act == "relu")
+    _check_linear(x, w, b, r, dy, act)

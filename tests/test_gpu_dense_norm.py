@@ -321,6 +321,29 @@ def test_linear_mx8_large_tiles_and_nan():
     assert torch.equal(y2[keep], y[keep]) and bool(torch.isnan(y2[7]).all())
 
 
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_linear_mx8_large_odd_rows(act):
+    """rows of values that are no multiple of 16 bytes, large enough for copies with their ends filled up"""
+    from latte_amd import functional as LF
+    M, K, N = 3001, 2047, 2050
+    x, w, b = _rn(10, torch.float32, (M, K), (N, K), (N,))
+    b = b.half()
+    xq, wq = LF.quantize_mx8(x), LF.quantize_mx8(w * K ** -0.5)
+    X, W = R.mx8(x)[0], R.mx8(w * K ** -0.5)[0]
+    with torch.no_grad():
+        y = LF.linear(xq, wq, b, act=act)
+    Z = X @ W.t() + b.double()
+    zerr = (K + 1) * U * (X.abs() @ W.abs().t() + b.double().abs()) + _mx8_sum_err(X, W)
+    Y = R.act(Z, act)[0]
+    tol = 1.13 * zerr + (3e-6 * (1 + Z.abs()) if act == "silu" else 0)
+    _close(y, Y, tol + R.EPS[y.dtype] * (Y.abs() + tol) + R.LOW[y.dtype], "y")
+    x[5, K - 1] = float("inf")
+    with torch.no_grad():
+        y2 = LF.linear(LF.quantize_mx8(x), wq, b, act=act)
+    keep = [i for i in range(M) if i != 5]
+    assert torch.equal(y2[keep], y[keep]) and bool(torch.isnan(y2[5]).all())
+
+
 def test_serving_block_together():
     """norm -> 8-bit product -> residual, as a serving layer calls them, against the same in 64 bits from the held values"""
     from latte_amd import functional as LF
