@@ -120,10 +120,21 @@ int64_t needs(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r
   return n;
 }
 
+// which of these this backward pass was asked for (autograd.grad of some of the inputs).  A node's edges are its tensors that exist,
+// in the order of its arguments.
+int64_t asked(const AutogradContext* ctx, int64_t need, bool has_b) {
+  int64_t n = 0;
+  if ((need & NEED_X) && ctx->needs_input_grad(0)) n |= NEED_X;
+  if ((need & NEED_W) && ctx->needs_input_grad(1)) n |= NEED_W;
+  if ((need & NEED_B) && ctx->needs_input_grad(2)) n |= NEED_B;
+  if ((need & NEED_R) && ctx->needs_input_grad(has_b ? 3 : 2)) n |= NEED_R;
+  return n;
+}
+
 // ------------------------------------------------------------------ linear
 struct LinearSaved {
   Tensor x, scales, w, deriv;
-  std::vector<int64_t> meta;   // K, N, deriv kind, row strides of x and w, needs, then the shape of x
+  std::vector<int64_t> meta;   // K, N, deriv kind, row strides of x and w, needs, a bias or none, then the shape of x
 };
 
 Tensor linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r, int64_t act, bool mx8, int64_t need,
@@ -156,7 +167,7 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, const T
     }
     if (need & NEED_X) keep->w = w2.t;
     keep->deriv = deriv;
-    keep->meta = {K, N, kind, ldx, w2.ld, need};
+    keep->meta = {K, N, kind, ldx, w2.ld, need, b.defined()};
     for (auto s : x.sizes()) keep->meta.push_back(s);
   }
   return y;
@@ -176,7 +187,7 @@ struct LinearNode : public torch::autograd::Function<LinearNode> {
     const c10::DeviceGuard on(grads[0].device());
     const auto saved = ctx->get_saved_variables();
     const auto meta = ctx->saved_data["meta"].toIntVector();
-    const int64_t K = meta[0], N = meta[1], need = meta[5];
+    const int64_t K = meta[0], N = meta[1], need = asked(ctx, meta[5], meta[6]);
     const Tensor& dy = grads[0];
     Tensor dx, dw, db;
     if (need & (NEED_X | NEED_W | NEED_B)) {
@@ -189,7 +200,7 @@ struct LinearNode : public torch::autograd::Function<LinearNode> {
       check("lt_linear_bwd",
             lt.linear_bwd(g.p(), g.ld, ptr(saved[0]), meta[3], ptr(saved[1]), ptr(saved[2]), meta[4], ptr(saved[3]), (int32_t)meta[2], g.n,
                           (int32_t)K, (int32_t)N, dt, ptr(dx), ptr(dw), ptr(db), ws.data_ptr(), ws.numel(), stream_of(dy)));
-      if (dx.defined() && meta.size() != 8) dx = dx.view(at::IntArrayRef(meta.data() + 6, meta.size() - 6));
+      if (dx.defined() && meta.size() != 9) dx = dx.view(at::IntArrayRef(meta.data() + 7, meta.size() - 7));
     }
     return {dx, dw, db, need & NEED_R ? dy : Tensor(), Tensor(), Tensor(), Tensor()};
   }
@@ -266,7 +277,7 @@ struct RmsNode : public torch::autograd::Function<RmsNode> {
     no_second("rms_norm");
     const auto saved = ctx->get_saved_variables();
     const auto meta = ctx->saved_data["meta"].toIntVector();
-    const int64_t need = meta[1];
+    const int64_t need = asked(ctx, meta[1], false);
     const Tensor &w = saved[3], &rstd = saved[4];
     const Tensor dy = grads[0], dh = grads.size() > 1 ? grads[1] : Tensor();
     Tensor dx, dw;
@@ -344,7 +355,7 @@ struct BnNode : public torch::autograd::Function<BnNode> {
     const auto saved = ctx->get_saved_variables();
     const auto meta = ctx->saved_data["meta"].toIntVector();
     const float eps = (float)ctx->saved_data["eps"].toDouble();
-    const int64_t need = meta[0];
+    const int64_t need = asked(ctx, meta[0], true);
     const bool post = meta[1] != 0;
     const c10::DeviceGuard on(grads[0].device());
     const Tensor dy = grads[0].contiguous();

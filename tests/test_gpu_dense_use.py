@@ -284,3 +284,29 @@ def test_capture_is_refused_while_an_eager_graph_holds_a_leaf():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
         step()
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_some_of_the_gradients(dt):
+    """a backward pass asked for some inputs of several gives the same bits for them"""
+    from itertools import combinations
+
+    from latte_amd import functional as LF
+    M, K, N = 700, 96, 40
+    x, w, b, r, dy, g, rx, dyx = _rn(51, dt, (M, K), (N, K), (N,), (M, N), (M, N), (K,), (M, K), (M, K))
+    leaves = [t.requires_grad_() for t in (x, w, b, r, g, rx)]
+    calls = [((x, w, b, r), dy, lambda: LF.linear(x, w, b, act="silu", residual=r)),
+             ((x, w, r), dy, lambda: LF.linear(x, w, act="relu", residual=r, checkpoint="mx8")),
+             ((x, w), dy, lambda: LF.linear(x, w, b.detach())),
+             ((x, g, rx), dyx, lambda: LF.rms_norm(x, g, rx)[0])]
+    if dt is torch.float32:
+        beta = _rn(52, dt, (K,))[0].requires_grad_()
+        calls.append(((x, g, beta, rx), dyx, lambda: LF.batch_norm(x, g, beta, residual=rx, relu=True, checkpoint="mx8")))
+    for args, d, call in calls:
+        y = call()
+        full = torch.autograd.grad(y, args, d, retain_graph=True)
+        for n in range(1, len(args)):
+            for pick in combinations(range(len(args)), n):
+                some = torch.autograd.grad(y, [args[i] for i in pick], d, retain_graph=True)
+                assert all(torch.equal(s, full[i]) for s, i in zip(some, pick)), pick
+    assert all(t.grad is None for t in leaves)
