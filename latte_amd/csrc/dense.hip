@@ -24,7 +24,7 @@ static int64_t part_bytes(const LtPlan& p, int64_t rows, int cols) {
 // Lines whose length is no multiple of 16 bytes are staged through registers, in 128 x 128 tiles at most.  A large product is
 // worth a copy of its operands with their lines filled up by zeros: whole pieces go straight into LDS.  TFLOP/s measured
 // without and with (beside the copies): 16 bits forward 480 and 700, backward 240 and 700; fp32 backward 78 and 103, forward alike.
-// 9000 x 1001 -> 4001 fp16: forward 150 us as it is, 129 with the copies, a training step 786 and 359 (fp32 2539 and 2196); 3000 x
+// 9000 x 1001 -> 4001 fp16: forward 150 us as it is, 129 with the copies, a training step 786 and 359; 3000 x
 // 1001 -> 1003 fp16: 108 and 86.
 static bool pad_pays(double products, double copied, int dt, double as_is, double filled) {
   const double gain = 2e-6 * products * (1 / as_is - 1 / filled);   // us

@@ -36,8 +36,10 @@ static inline LtPlan lt_gemm_plan(int64_t rows, int cols, int64_t depth, int dt,
   else if (cols <= 32 && direct) p.tile = LT_TILE_256x32, br = 256, bc = 32;
   else if (cols <= 64 && direct) p.tile = LT_TILE_128x64, br = 128, bc = 64;
   // 128 x 128 tiles where they nearly fill the chip, else 64 x 64, four of which share a CU (1777 x 1000 -> 1000 bf16: 26 us
-  // on 112 of the larger, split four ways, 12 us on 448 of the smaller)
-  else if (tiles(128, 128) >= 224) p.tile = LT_TILE_128x128, br = 128, bc = 128;
+  // on 112 of the larger, split four ways, 12 us on 448 of the smaller).  fp32 is bound by the matrix rate alone, so there the
+  // smaller tiles cost 6 % (8192 x 1024 -> 1024: 137 and 144 us) and a chip half idle in its last turn costs more (3000 x 1500
+  // -> 1500: 191 and 154 us): the larger ones where the turns of two a CU are 93 % full.
+  else if (dt == LT_DT_F32 ? (double)rows * cols >= 0.93 * 128 * 128 * 512 * ((tiles(128, 128) + 511) / 512) : tiles(128, 128) >= 224) p.tile = LT_TILE_128x128, br = 128, bc = 128;
   else p.tile = LT_TILE_64x64, br = 64, bc = 64;
   p.tr = (int)((rows + br - 1) / br);
   p.tc = (cols + bc - 1) / bc;
