@@ -349,8 +349,8 @@ static BwdWs bwd_ws(int64_t M, int K, int N, int dt, bool x8) {
   const int64_t N8 = p.ok ? (N + 7) / 8 * 8 : pad ? up_to_16(N, dt) : N, K8 = pad ? up_to_16(K, dt) : K;
   w.dz = off;
   off += lt_align_up(M * N8 * lt_dt_size(dt), 256);
-  w.dz2 = off;
-  off += two_terms(M, N, dt) ? lt_align_up(M * N * lt_dt_size(dt), 256) : 0;
+  w.dz2 = off;   // the second term has the first one's rows, their filled-up ends among them
+  off += two_terms(M, N, dt) ? lt_align_up(M * N8 * lt_dt_size(dt), 256) : 0;
   w.part = off;
   const int64_t s = dz_plan(M, N).slabs, s8 = dz_plan(M, (int)N8).slabs;
   off += lt_align_up((s > s8 ? s : s8) * N * 4, 256);
