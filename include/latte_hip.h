@@ -314,8 +314,8 @@ int lt_devoxelize_cell_bwd(const float* gout, const int32_t* cells, const int32_
  * with a row stride (ld*, in elements; rows may start at any element, a stride of 0 repeats a row); y, deriv and the
  * gradients are contiguous.  dt = LT_DT_*: the type of x, w, bias, res, y and of the gradients; sums are fp32.
  * mx8: e4m3 values [M][K] and one scale byte per 32 neighbours [M][ceil(K/32)], value * 2^(scale - 127); the scale is the
- * smallest power of two that brings the block's largest finite magnitude to at most 448, rounding is to nearest even,
- * non-finite elements are held as NaN. */
+ * smallest power of two that brings the block's largest finite magnitude to at most 448, rounding is to nearest even (down to
+ * 240 where 256 times the scale would be infinite in the block's own type), non-finite elements are held as NaN. */
 #define LT_DT_F32 0
 #define LT_DT_BF16 1
 #define LT_DT_F16 2

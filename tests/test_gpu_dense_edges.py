@@ -16,3 +16,50 @@ def test_two_terms_of_dz_with_filled_up_rows(size, dt):
     """a small dz over a very wide input: it goes in as two terms, and both come with their rows filled up"""
     x, w, b, _, dy = _inputs(*size, dt, seed=1)
     _check_linear(x, w, b, None, dy, "gelu")
+
+
+def _mx8(x):
+    """(values read back, scale exponents + 127) of quantize_mx8 in 64 bits: the smallest scale that brings the block to 448, cut
+    at 240 only where 256 times the scale is infinite in the type"""
+    M, K = x.shape
+    b = torch.nn.functional.pad(x.double(), (0, (-K) % 32)).view(M, -1, 32)
+    m, e = torch.frexp(b.abs().amax(2, keepdim=True))                        # m 2^e, m in [0.5, 1)
+    E = torch.where(m > 0, e - 9 + (m > 0.875), torch.full_like(e, -126)).clamp(min=-126)
+    s = R.two_to(E)
+    lim = torch.where(256 * s > torch.finfo(x.dtype).max, 240.0, 448.0).to(b)
+    v = torch.maximum(torch.minimum(b / s, lim), -lim)
+    step = R.two_to((torch.frexp(v.abs())[1] - 4).clamp(min=-9))
+    return (torch.round(v / step) * step * s).view(M, -1)[:, :K], (E + 127).view(M, -1)
+
+
+@pytest.mark.parametrize("dt", HALF)
+def test_mx8_over_every_value(dt):
+    """every finite 16-bit number alone in its block, and beside the largest of the blocks of its binade"""
+    from latte_amd import functional as LF
+    every = torch.arange(65536, device="cuda").to(torch.int32).to(torch.int16).view(dt)
+    every = every[torch.isfinite(every)].view(-1, 1)
+    top = torch.ldexp(torch.ones((), device="cuda", dtype=torch.float64), torch.frexp(every.double())[1]) * 1.0   # next power of two
+    for x in (every, torch.cat([every, (top * 0.875).to(dt), (top * 0.5).to(dt)], 1)):
+        x = torch.where(torch.isfinite(x), x, torch.zeros_like(x))
+        q = LF.quantize_mx8(x)
+        val, sc = _mx8(x)
+        assert torch.equal(q.scales.int(), sc.int()) and torch.equal(q.dequantize().double(), val)
+        back = q.dequantize(dt).double()
+        assert torch.equal(back, val.to(dt).double()) and bool(torch.isfinite(back).all())
+        big = x.double().abs() > torch.finfo(dt).tiny * 2 ** 14              # above the scales' lower end
+        assert bool(((val - x.double()).abs() <= 2.0 ** -4 * x.double().abs())[big].all())
+
+
+def test_mx8_checkpoint_of_large_half_values():
+    """a layer over fp16 inputs of the last binade: its weight gradient is that of values within 2^-4 of x"""
+    from latte_amd import functional as LF
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = (torch.rand(64, 96, generator=g, device="cuda") * 24000 + 33000).half()
+    w = (torch.randn(48, 96, generator=g, device="cuda") * 1e-4).half().requires_grad_(True)
+    dy = torch.randint(-2, 3, (64, 48), generator=g, device="cuda").half() / 1024
+    gw, = torch.autograd.grad(LF.linear(x, w, checkpoint="mx8"), w, dy)
+    held = _mx8(x)[0]
+    assert float(((held - x.double()) / x.double()).abs().max()) <= 2.0 ** -4
+    want = dy.double().t() @ held
+    t = 64 * U * (dy.double().abs().t() @ held.abs())
+    _close(gw, want, t + R.EPS[torch.float16] * (want.abs() + t), "dw")
