@@ -58,6 +58,9 @@ void like(const Tensor& t, const Tensor& ref, at::IntArrayRef shape, const char*
   TORCH_CHECK_VALUE(t.sizes() == shape, name, ": expected shape ", shape, ", got ", t.sizes());
 }
 
+// the C entry points take row lengths and output widths as 32-bit numbers
+bool fits32(int64_t n) { return n >= 1 && n < INT32_MAX; }
+
 // a 2-D tensor with neighbouring columns and its row stride: a view wherever the strides allow one
 struct Rows {
   Tensor t;
@@ -209,9 +212,8 @@ struct LinearNode : public torch::autograd::Function<LinearNode> {
 Tensor linear(const Tensor& x, const Tensor& w, const std::optional<Tensor>& b_, const std::optional<Tensor>& r_, int64_t act, bool mx8) {
   const Tensor b = b_.value_or(Tensor()), r = r_.value_or(Tensor());
   dtype_of(x, "linear x");
-  TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1) && w.size(0) >= 1 && w.size(1) >= 1 && w.size(0) < INT32_MAX &&
-                        w.size(1) < INT32_MAX,
-                    "linear: x ", x.sizes(), " and weight ", w.sizes(), " do not go together");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1) && fits32(w.size(0)) && fits32(w.size(1)), "linear: x ",
+                    x.sizes(), " and weight ", w.sizes(), " do not go together");
   like(w, x, w.sizes(), "linear weight");
   if (b.defined()) like(b, x, {w.size(0)}, "linear bias");
   if (r.defined()) {
@@ -381,7 +383,7 @@ struct BnNode : public torch::autograd::Function<BnNode> {
 
 variable_list batch_norm_mx8(const Tensor& x, const Tensor& gamma, const Tensor& beta, const std::optional<Tensor>& r, double eps, bool relu,
                              bool post) {
-  TORCH_CHECK_VALUE(x.dim() == 2, "batch_norm: expected a [rows, channels] matrix, got shape ", x.sizes());
+  TORCH_CHECK_VALUE(x.dim() == 2 && fits32(x.size(1)), "batch_norm: expected a [rows, channels] matrix, got shape ", x.sizes());
   bn_like(x, x, x.sizes(), "batch_norm x");
   bn_like(gamma, x, {x.size(1)}, "batch_norm gamma");
   bn_like(beta, x, {x.size(1)}, "batch_norm beta");
@@ -392,13 +394,14 @@ variable_list batch_norm_mx8(const Tensor& x, const Tensor& gamma, const Tensor&
 // ------------------------------------------------------------------ mx8 (no gradients)
 std::pair<Tensor, Tensor> quantize_mx8(const Tensor& x) {
   const int dt = dtype_of(x, "quantize_mx8");
-  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "quantize_mx8: expected rows of at least one element, got shape ", x.sizes());
+  TORCH_CHECK_VALUE(x.dim() >= 1 && fits32(x.size(-1)), "quantize_mx8: expected rows of 1 to 2^31 - 2 elements, got shape ", x.sizes());
   at::NoGradGuard off;
   const c10::DeviceGuard on(x.device());
   return quantize(Rows(x, x.size(-1)), x.size(-1), dt);
 }
 
 Tensor dequantize_mx8(const Tensor& q, const Tensor& s, at::ScalarType dtype) {
+  TORCH_CHECK_VALUE(fits32(q.size(1)), "Mx8.dequantize: expected rows of 1 to 2^31 - 2 elements, got shape ", q.sizes());
   const c10::DeviceGuard on(q.device());
   Tensor out = at::empty(q.sizes(), q.options().dtype(dtype));
   check("lt_mx8_dequantize", lt.mx8_dequantize(q.data_ptr(), s.data_ptr(), q.size(0), (int32_t)q.size(1), dtype_of(out, "Mx8.dequantize"),
@@ -417,7 +420,7 @@ Tensor linear_mx8(const Tensor& x, const Tensor& xs, const Tensor& w, const Tens
   no_gradient("linear: mx8 operands carry no gradient", {b, r});
   const c10::DeviceGuard on(x.device());
   const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
-  TORCH_CHECK_VALUE(w.size(1) == K && K >= 1 && N >= 1, "linear: x ", x.sizes(), " and weight ", w.sizes(), " do not go together");
+  TORCH_CHECK_VALUE(w.size(1) == K && fits32(K) && fits32(N), "linear: x ", x.sizes(), " and weight ", w.sizes(), " do not go together");
   TORCH_CHECK_VALUE(w.device() == x.device(), "linear weight: on ", w.device(), ", the other operands on ", x.device());
   const at::ScalarType out = dtype ? *dtype : b.defined() ? b.scalar_type() : r.defined() ? r.scalar_type() : at::kBFloat16;
   TORCH_CHECK_TYPE(out == at::kBFloat16 || out == at::kHalf, "linear: results of mx8 operands are bfloat16 or float16, not ", out);
