@@ -89,9 +89,17 @@ std::vector<int64_t> last(const Tensor& x, int64_t n) {
 // workspace of one call: torch's allocator (and a graph's private pool) keeps it from any other stream or graph
 Tensor workspace(int64_t bytes, const Tensor& like) { return at::empty({bytes > 256 ? bytes : 256}, like.options().dtype(at::kByte)); }
 
-void no_second(const char* name) {
+// Forward-mode tangents would be lost without a word: the kernels see values only.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+void no_tangents(std::initializer_list<Tensor> ts) {
+  for (const auto& t : ts)
+    TORCH_CHECK(!has_tangent(t), "forward-mode derivatives are not implemented for the dense operators (forward_ad.unpack_dual gives the value)");
+}
+
+void no_second(const char* name, const variable_list& grads) {
   // a backward pass runs with gradients enabled only where its own graph is asked for, which these kernels do not build
   TORCH_CHECK(!at::GradMode::is_enabled(), name, ": gradients of gradients are not implemented (create_graph=True)");
+  for (const auto& g : grads) no_tangents({g});
 }
 
 // x held in mx8: e4m3 values and a scale byte per 32 neighbours
@@ -103,6 +111,7 @@ std::pair<Tensor, Tensor> quantize(const Rows& x, int64_t K, int dt) {
 
 enum { NEED_X = 1, NEED_W = 2, NEED_B = 4, NEED_R = 8 };
 int64_t needs(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r) {
+  no_tangents({x, w, b, r});
   if (!at::GradMode::is_enabled()) return 0;
   auto need = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
   const int64_t n = (need(x) ? NEED_X : 0) | (need(w) ? NEED_W : 0) | (need(b) ? NEED_B : 0) | (need(r) ? NEED_R : 0);
@@ -186,7 +195,7 @@ struct LinearNode : public torch::autograd::Function<LinearNode> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    no_second("linear");
+    no_second("linear", grads);
     const c10::DeviceGuard on(grads[0].device());
     const auto saved = ctx->get_saved_variables();
     const auto meta = ctx->saved_data["meta"].toIntVector();
@@ -276,7 +285,7 @@ struct RmsNode : public torch::autograd::Function<RmsNode> {
     return {y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    no_second("rms_norm");
+    no_second("rms_norm", grads);
     const auto saved = ctx->get_saved_variables();
     const auto meta = ctx->saved_data["meta"].toIntVector();
     const int64_t need = asked(ctx, meta[1], false);
@@ -353,7 +362,7 @@ struct BnNode : public torch::autograd::Function<BnNode> {
     return {y, mean, var};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    no_second("batch_norm");
+    no_second("batch_norm", grads);
     const auto saved = ctx->get_saved_variables();
     const auto meta = ctx->saved_data["meta"].toIntVector();
     const float eps = (float)ctx->saved_data["eps"].toDouble();
@@ -410,6 +419,7 @@ Tensor dequantize_mx8(const Tensor& q, const Tensor& s, at::ScalarType dtype) {
 }
 
 void no_gradient(const char* what, std::initializer_list<Tensor> ts) {
+  no_tangents(ts);
   for (const auto& t : ts)
     TORCH_CHECK(!(at::GradMode::is_enabled() && t.defined() && t.requires_grad()), what, "; call it under torch.no_grad()");
 }

@@ -92,7 +92,7 @@ def linear(x, weight, bias=None, act: str = "none", residual=None, checkpoint: s
     """act(x @ weight.T + bias) + residual as one kernel; act: "none" | "relu" | "gelu" (exact) | "silu".
 
     x [..., K], weight [N, K], bias [N], residual [..., N] -> [..., N], all of one type (float32, bfloat16, float16), sums in
-    fp32.  Differentiable in all four, once; the backward pass reads x, weight and act'.  checkpoint="mx8" keeps what it reads
+    fp32.  Differentiable in all four, once, in reverse mode; the backward pass reads x, weight and act'.  checkpoint="mx8" keeps what it reads
     of x in 8 bits (quantize_mx8: relative error at most 2^-4 an element) and act' of GELU / SiLU on a uniform 8-bit grid
     (error at most 1/384); the ReLU's act' is one bit either way.  The output does not depend on `checkpoint`.
 
@@ -120,8 +120,8 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, checkpoint: str | None
     residual.
 
     x [..., C], residual the same shape, weight [C], all float32, bfloat16 or float16, C <= 16384; the sum of squares and the
-    row's scale are fp32, h enters the norm unrounded.  Differentiable in all three, once; checkpoint="mx8": the backward
-    pass reads h from 8 bits.  out="mx8" (serving, no gradient): y comes as Mx8 [rows, C], for linear() with an Mx8 weight."""
+    row's scale are fp32, h enters the norm unrounded.  Differentiable in all three, once, in reverse mode; checkpoint="mx8": the
+    backward pass reads h from 8 bits.  out="mx8" (serving, no gradient): y comes as Mx8 [rows, C], for linear() with an Mx8 weight."""
     if checkpoint not in (None, "mx8"):
         raise ValueError(f"rms_norm: checkpoint must be None or 'mx8', got {checkpoint!r}")
     if out not in (None, "mx8"):

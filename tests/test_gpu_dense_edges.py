@@ -63,3 +63,34 @@ def test_mx8_checkpoint_of_large_half_values():
     want = dy.double().t() @ held
     t = 64 * U * (dy.double().abs().t() @ held.abs())
     _close(gw, want, t + R.EPS[torch.float16] * (want.abs() + t), "dw")
+
+
+def test_forward_mode_is_refused():
+    """a tangent is never dropped without a word, with and without a graph for the backward pass, and not in a backward pass either"""
+    from latte_amd import functional as LF
+    from torch.autograd import forward_ad as fw
+    x, w, g, b = (torch.randn(*s, device="cuda") for s in ((6, 8), (5, 8), (8,), (5,)))
+    x8, w8 = LF.quantize_mx8(x), LF.quantize_mx8(w)
+    y, n = LF.linear(x, w.clone().requires_grad_(True)), LF.rms_norm(x, g.clone().requires_grad_(True))
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        calls = [lambda: LF.linear(dual(x), w), lambda: LF.linear(x, dual(w)), lambda: LF.linear(x, w, dual(b)),
+                 lambda: LF.linear(x, w, residual=dual(x[:, :5])), lambda: LF.linear(dual(x), w.requires_grad_(True)),
+                 lambda: LF.rms_norm(dual(x), g), lambda: LF.rms_norm(x, dual(g)), lambda: LF.rms_norm(x, g, dual(x)),
+                 lambda: LF.rms_norm(dual(x), g, out="mx8"), lambda: LF.linear(x8, w8, dual(b.half())),
+                 lambda: LF.batch_norm(dual(x), g.requires_grad_(True), g.detach(), checkpoint="mx8"),
+                 lambda: y.backward(dual(torch.ones_like(y))), lambda: n.backward(dual(torch.ones_like(n)))]
+        for grad in (False, True):
+            for call in calls[:10] if not grad else calls:
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+        assert fw.unpack_dual(LF.linear(fw.unpack_dual(dual(x)).primal, w.detach())).tangent is None
+
+
+def test_function_transforms_are_refused():
+    from latte_amd import functional as LF
+    x, w = torch.randn(6, 8, device="cuda"), torch.randn(8, 8, device="cuda")
+    for call in (lambda: torch.func.grad(lambda t: LF.linear(t, w).sum())(x), lambda: torch.func.vmap(lambda t: LF.linear(t, w))(x),
+                 lambda: torch.func.jvp(lambda t: LF.rms_norm(t, w[0]), (x,), (x,))):
+        with pytest.raises(RuntimeError):
+            call()
