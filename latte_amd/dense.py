@@ -46,7 +46,7 @@ def _on_gpu(t, name: str) -> None:
 
 class Mx8:
     """A matrix held in 8 bits: `values` float8_e4m3fn [M, K] and `scales` uint8 [M, ceil(K / 32)] -- element (i, j) stands for
-    values[i, j] * 2^(scales[i, j // 32] - 127)."""
+    values[i, j] * 2^(scales[i, j // 32] - 127); a scale byte of 255 makes its block NaN."""
 
     __slots__ = ("values", "scales")
 
@@ -83,7 +83,7 @@ class Mx8:
 
 def quantize_mx8(x: torch.Tensor) -> Mx8:
     """x [..., K] -> Mx8 [rows, K]: 32 neighbours share the smallest power of two that brings their largest finite magnitude
-    to at most 448; nearest even e4m3.  Infinities and NaN are held as NaN."""
+    to at most 448; nearest even e4m3.  Infinities and NaN are held as NaN.  The result carries no gradient."""
     _on_gpu(x, "quantize_mx8")
     return Mx8._of(*_nodes().quantize_mx8(x))
 

@@ -94,3 +94,20 @@ def test_function_transforms_are_refused():
                  lambda: torch.func.jvp(lambda t: LF.rms_norm(t, w[0]), (x,), (x,))):
         with pytest.raises(RuntimeError):
             call()
+
+
+def test_mx8_scales_at_their_ends():
+    """scale bytes 0 and 255 (only a caller's own Mx8 has them) stand for 2^-127 and NaN, read back and in the matrix instruction"""
+    from latte_amd import functional as LF
+    v = torch.zeros(1, 32, device="cuda")
+    v[0, :2] = torch.tensor([1.0, -448.0])
+    one = torch.zeros(16, 32, device="cuda")
+    one[0, 0] = one[1, 1] = 1
+    one = LF.quantize_mx8(one)
+    for byte in (0, 1, 127, 245, 255):
+        q = LF.Mx8(v.to(torch.float8_e4m3fn), torch.full((1, 1), byte, dtype=torch.uint8, device="cuda"))
+        want = v.double() * 2.0 ** (byte - 127) if byte < 255 else torch.full_like(v, float("nan")).double()
+        assert torch.equal(torch.nan_to_num(q.dequantize().double(), nan=-7.0), torch.nan_to_num(want, nan=-7.0))
+        with torch.no_grad():
+            y = LF.linear(q, one)[0, :2].double()
+        assert torch.equal(torch.nan_to_num(y, nan=-7.0), torch.nan_to_num(want[0, :2], nan=-7.0))
