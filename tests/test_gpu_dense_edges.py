@@ -111,3 +111,19 @@ def test_mx8_scales_at_their_ends():
         with torch.no_grad():
             y = LF.linear(q, one)[0, :2].double()
         assert torch.equal(torch.nan_to_num(y, nan=-7.0), torch.nan_to_num(want[0, :2], nan=-7.0))
+
+
+@pytest.mark.parametrize("dt", HALF)
+def test_activation_tails(dt):
+    """GELU and SiLU of 16-bit types far below zero keep their relative accuracy: the fp32 value is within 5e-5 of itself there (3.2e-5
+    of the tail's polynomial; the exponent's argument, at most 128, is off by 2^-24 of itself twice: 1.1e-5; some last places), and
+    is rounded once.  One input, weight 1, no bias: z is x."""
+    from latte_amd import functional as LF
+    x = -torch.linspace(0, 13, 4001, device="cuda").to(dt).view(-1, 1)
+    one = torch.ones(1, 1, device="cuda", dtype=dt)
+    for act in ("gelu", "silu"):
+        want = R.act(x.double(), act)[0]
+        for xi in (x, x[::200]):                     # tiles, few rows
+            y, t = LF.linear(xi, one, act=act), R.act(xi.double(), act)[0]
+            _close(y, t, (R.EPS[dt] * 1.00005 + 5e-5) * t.abs() + R.LOW[dt], act)
+        assert float(want.abs().min()) == 0          # x = 0 among them
