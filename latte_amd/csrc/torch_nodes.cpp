@@ -359,10 +359,12 @@ struct BnNode : public torch::autograd::Function<BnNode> {
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["meta"] = std::vector<int64_t>{need, post};
     ctx->mark_non_differentiable({mean, var});
+    ctx->set_materialize_grads(false);   // the statistics' gradients are never there: no zeros for them
     return {y, mean, var};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     no_second("batch_norm", grads);
+    if (!grads[0].defined()) return variable_list(8);
     const auto saved = ctx->get_saved_variables();
     const auto meta = ctx->saved_data["meta"].toIntVector();
     const float eps = (float)ctx->saved_data["eps"].toDouble();
@@ -374,13 +376,17 @@ struct BnNode : public torch::autograd::Function<BnNode> {
     const int64_t V = q.size(0);
     const int32_t C = (int32_t)q.size(1);
     const lt_stream_t stream = stream_of(dy);
-    Tensor dgamma = at::empty({C}, dy.options()), dbeta = at::empty({C}, dy.options()), dx, dr;
+    Tensor dgamma, dbeta, dx, dr;
     if (need & NEED_X) dx = at::empty_like(dy);
     if ((need & NEED_R) && !post) dr = at::empty_like(dy);
-    const Tensor ws = workspace(lt.bn_ws(V, C), dy);
-    check("lt_bn_bwd_reduce_mx8", lt.bn_reduce(dy.data_ptr<float>(), q.data_ptr(), s.data_ptr(), ptr(mask), mean.data_ptr<float>(),
-                                               var.data_ptr<float>(), eps, V, C, ws.data_ptr(), ws.numel(), dbeta.data_ptr<float>(),
-                                               dgamma.data_ptr<float>(), stream));
+    const bool sums = need & (NEED_X | NEED_W | NEED_B);   // the residual's gradient needs none
+    if (sums || dr.defined()) dgamma = at::empty({C}, dy.options()), dbeta = at::empty({C}, dy.options());
+    if (sums) {
+      const Tensor ws = workspace(lt.bn_ws(V, C), dy);
+      check("lt_bn_bwd_reduce_mx8", lt.bn_reduce(dy.data_ptr<float>(), q.data_ptr(), s.data_ptr(), ptr(mask), mean.data_ptr<float>(),
+                                                 var.data_ptr<float>(), eps, V, C, ws.data_ptr(), ws.numel(), dbeta.data_ptr<float>(),
+                                                 dgamma.data_ptr<float>(), stream));
+    }
     if (dx.defined() || dr.defined())
       check("lt_bn_bwd_apply_mx8",
             lt.bn_bwd(dy.data_ptr<float>(), q.data_ptr(), s.data_ptr(), ptr(mask), mean.data_ptr<float>(), var.data_ptr<float>(),

@@ -127,3 +127,21 @@ def test_activation_tails(dt):
             y, t = LF.linear(xi, one, act=act), R.act(xi.double(), act)[0]
             _close(y, t, (R.EPS[dt] * 1.00005 + 5e-5) * t.abs() + R.LOW[dt], act)
         assert float(want.abs().min()) == 0          # x = 0 among them
+
+
+@pytest.mark.parametrize("post", [False, True])
+def test_bn_residual_gradient_alone(post):
+    """the residual's gradient needs no column sums: asked for alone it takes its own memory (none where it is dy itself) and
+    comes out as with the others"""
+    from latte_amd import functional as LF
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x, r, dy = (torch.randn(3000, 96, generator=g, device="cuda") for _ in range(3))
+    leaves = [t.requires_grad_(True) for t in (x, torch.ones(96, device="cuda"), torch.zeros(96, device="cuda"), r)]
+    y = LF.batch_norm(*leaves[:3], residual=r, relu=True, post_add=post, checkpoint="mx8")
+    full = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    made = lambda: torch.cuda.memory_stats()["allocation.all.allocated"]  # noqa: E731
+    before = made()
+    alone, = torch.autograd.grad(y, r, dy, retain_graph=True)
+    count = made() - before
+    assert torch.equal(alone, full[3]) and torch.equal(alone, dy if post else dy * (y > 0))
+    assert count <= (0 if post else 3)               # the gradient, and two unread vectors that the kernel is handed
