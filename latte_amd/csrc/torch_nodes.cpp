@@ -96,10 +96,28 @@ void no_tangents(std::initializer_list<Tensor> ts) {
     TORCH_CHECK(!has_tangent(t), "forward-mode derivatives are not implemented for the dense operators (forward_ad.unpack_dual gives the value)");
 }
 
+// A captured backward pass that goes on into a graph made before the capture on the default stream makes that stream wait for the
+// capturing one as well (any other stream joins the capture).  Only the pass itself knows which gradients it was asked for.
+void not_into_eager(const Tensor& dy) {
+  const c10::DeviceGuard on(dy.device());
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  const c10::StreamId def = c10::hip::getDefaultHIPStream(dy.get_device()).id();
+  for (size_t i = 0; i < node->num_outputs(); ++i) {
+    if (!node->task_should_compute_output(i)) continue;
+    const auto stream = node->next_edge(i).function->stream();
+    TORCH_CHECK(!stream || stream->id() != def, "this backward pass can not be captured: it goes on into a graph that was made on the "
+                "default stream before the capture; compute that part within the capture, or detach it");
+  }
+}
+
 void no_second(const char* name, const variable_list& grads) {
   // a backward pass runs with gradients enabled only where its own graph is asked for, which these kernels do not build
   TORCH_CHECK(!at::GradMode::is_enabled(), name, ": gradients of gradients are not implemented (create_graph=True)");
   for (const auto& g : grads) no_tangents({g});
+  for (const auto& g : grads)
+    if (g.defined()) return not_into_eager(g);
 }
 
 // x held in mx8: e4m3 values and a scale byte per 32 neighbours
@@ -117,7 +135,8 @@ int64_t needs(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r
   const int64_t n = (need(x) ? NEED_X : 0) | (need(w) ? NEED_W : 0) | (need(b) ? NEED_B : 0) | (need(r) ? NEED_R : 0);
   if (!n) return 0;
   // While an eager graph of a leaf lives, the leaf's gradient is accumulated on that graph's stream.  A captured backward
-  // pass would make that stream wait for the capturing one, which ends the capture and the process with it.
+  // pass would make that stream wait for the capturing one, which ends the capture and the process with it.  (Inputs that
+  // were themselves computed before the capture: not_into_eager.)
   const c10::DeviceGuard on(x.device());
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
     const c10::StreamId here = c10::hip::getCurrentHIPStream(x.get_device()).id();   // the same id under torch's device name

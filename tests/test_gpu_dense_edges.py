@@ -145,3 +145,27 @@ def test_bn_residual_gradient_alone(post):
     count = made() - before
     assert torch.equal(alone, full[3]) and torch.equal(alone, dy if post else dy * (y > 0))
     assert count <= (0 if post else 3)               # the gradient, and two unread vectors that the kernel is handed
+
+
+def test_capture_over_inputs_that_were_computed_before_it():
+    """the gradient of such an input leads back into an eager graph on the default stream: refused; of the others it is captured"""
+    from latte_amd import functional as LF
+    g = torch.Generator(device="cuda").manual_seed(4)
+    leaf, w, n, dy, dn = (torch.randn(*s, generator=g, device="cuda") for s in ((64, 32), (48, 32), (32,), (64, 48), (64, 32)))
+    leaf.requires_grad_(True)
+    h, n, w = leaf * 2, n.requires_grad_(True), w.requires_grad_(True)
+    calls = [(lambda: LF.linear(h, w, act="gelu", checkpoint="mx8"), w, dy), (lambda: LF.rms_norm(h, n), n, dn),
+             (lambda: LF.batch_norm(h, n, n, checkpoint="mx8"), n, dn)]
+    for call, other, d in calls:
+        with pytest.raises(RuntimeError, match="can not be captured"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                torch.autograd.grad(call(), h, d)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out, = torch.autograd.grad(call(), other, d)
+        want, = torch.autograd.grad(call(), other, d)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+            want = torch.autograd.grad(call(), other, d)[0]
