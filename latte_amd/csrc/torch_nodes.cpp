@@ -61,6 +61,10 @@ void like(const Tensor& t, const Tensor& ref, at::IntArrayRef shape, const char*
 // the C entry points take row lengths and output widths as 32-bit numbers
 bool fits32(int64_t n) { return n >= 1 && n < INT32_MAX; }
 
+// the kernels read memory as it lies: the lazy minus sign of a view (the imaginary part of a conjugate) is carried out first
+Tensor plain(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+Tensor dense(const Tensor& t) { return plain(t).contiguous(); }
+
 // a 2-D tensor with neighbouring columns and its row stride: a view wherever the strides allow one
 struct Rows {
   Tensor t;
@@ -68,7 +72,7 @@ struct Rows {
   Rows() = default;
   Rows(const Tensor& x, int64_t cols) {
     if (!x.defined()) return;
-    t = x.dim() == 2 ? x : x.reshape({-1, cols});
+    t = x.dim() == 2 ? plain(x) : plain(x).reshape({-1, cols});
     if (t.stride(1) != 1 && cols > 1) t = t.contiguous();
     n = t.size(0);
     ld = n > 1 ? t.stride(0) : cols;   // a single row's stride means nothing
@@ -174,7 +178,7 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, const T
   const int dt = dtype_of(x, "linear x");
   const int64_t N = w.size(0), K = w.size(1);
   const Rows x2(x, K), w2(w, K), r2(r, N);
-  const Tensor bias = b.defined() ? b.contiguous() : b;
+  const Tensor bias = b.defined() ? dense(b) : b;
   const int64_t M = x2.n;
   int kind = LT_DERIV_NONE;
   if (act != LT_ACT_NONE && (need & (NEED_X | NEED_W | NEED_B))) kind = act == LT_ACT_RELU ? LT_DERIV_BITS : mx8 ? LT_DERIV_BYTE : LT_DERIV_FULL;
@@ -263,7 +267,7 @@ std::pair<Tensor, Tensor> rms_forward(const Tensor& x, const Tensor& w_, const T
   const int dt = dtype_of(x, "rms_norm x");
   const int64_t C = x.size(-1);
   const Rows x2(x, C), r2(r, C);
-  const Tensor w = w_.contiguous();
+  const Tensor w = dense(w_);
   Tensor y = at::empty(x.sizes(), x.options()), h, h8, h8s, rstd;
   if (r.defined()) h = at::empty(x.sizes(), x.options());
   if (keep) {
@@ -361,8 +365,8 @@ struct BnNode : public torch::autograd::Function<BnNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x_, const Tensor& gamma_, const Tensor& beta_, const std::optional<Tensor>& r_,
                                double eps, bool relu, bool post, int64_t need) {
     const c10::DeviceGuard on(x_.device());
-    const Tensor x = x_.contiguous(), gamma = gamma_.contiguous(), beta = beta_.contiguous();
-    const Tensor r = r_ ? r_->contiguous() : Tensor();
+    const Tensor x = dense(x_), gamma = dense(gamma_), beta = dense(beta_);
+    const Tensor r = r_ ? dense(*r_) : Tensor();
     const int64_t V = x.size(0);
     const int32_t C = (int32_t)x.size(1);
     const lt_stream_t stream = stream_of(x);
@@ -390,7 +394,7 @@ struct BnNode : public torch::autograd::Function<BnNode> {
     const int64_t need = asked(ctx, meta[0], true);
     const bool post = meta[1] != 0;
     const c10::DeviceGuard on(grads[0].device());
-    const Tensor dy = grads[0].contiguous();
+    const Tensor dy = dense(grads[0]);
     const Tensor &q = saved[0], &s = saved[1], &mask = saved[2], &mean = saved[3], &var = saved[4], &gamma = saved[5];
     const int64_t V = q.size(0);
     const int32_t C = (int32_t)q.size(1);
@@ -462,7 +466,7 @@ Tensor linear_mx8(const Tensor& x, const Tensor& xs, const Tensor& w, const Tens
   Tensor y = at::empty({M, N}, x.options().dtype(out));
   if (b.defined()) like(b, y, {N}, "linear bias");
   if (r.defined()) like(r, y, {M, N}, "linear residual");
-  const Tensor bias = b.defined() ? b.contiguous() : b;
+  const Tensor bias = b.defined() ? dense(b) : b;
   const Rows r2(r, N);
   const int64_t wsb = lt.linear_mx8_ws(M, (int32_t)K, (int32_t)N);
   const Tensor ws = wsb > 0 ? workspace(wsb, x) : Tensor();
@@ -481,7 +485,7 @@ variable_list rms_norm_mx8(const Tensor& x, const Tensor& w, const std::optional
   const Rows x2(x, C), r2(r, C);
   Tensor q = at::empty({x2.n, C}, x.options().dtype(at::kFloat8_e4m3fn)), s = at::empty({x2.n, (C + 31) / 32}, x.options().dtype(at::kByte)), h;
   if (r.defined()) h = at::empty(x.sizes(), x.options());
-  check("lt_rms_norm_fwd", lt.rms_fwd(x2.p(), x2.ld, r2.p(), r2.ld, w.contiguous().data_ptr(), (float)eps, x2.n, (int32_t)C, dt, ptr(h), nullptr,
+  check("lt_rms_norm_fwd", lt.rms_fwd(x2.p(), x2.ld, r2.p(), r2.ld, dense(w).data_ptr(), (float)eps, x2.n, (int32_t)C, dt, ptr(h), nullptr,
                                       q.data_ptr(), s.data_ptr(), nullptr, nullptr, nullptr, stream_of(x)));
   if (h.defined()) return {q, s, h};
   return {q, s};

@@ -169,3 +169,34 @@ def test_capture_over_inputs_that_were_computed_before_it():
             torch.cuda.synchronize()
             assert torch.equal(out, want)
             want = torch.autograd.grad(call(), other, d)[0]
+
+
+def test_lazily_negated_views():
+    """the imaginary part of a conjugate is a view with a minus sign still to be carried out: in every operand it is"""
+    from latte_amd import functional as LF
+    g = torch.Generator(device="cuda").manual_seed(5)
+
+    def neg(*s):
+        t = torch.conj(torch.randn(*s, generator=g, device="cuda", dtype=torch.complex64)).imag
+        flat = torch._neg_view(torch.randn(*s, generator=g, device="cuda"))
+        assert t.is_neg() and flat.is_neg()
+        return flat if s[-1] > 1 else t              # a single column has no stride that would ask for a copy
+    real = lambda *ts: [t.resolve_neg().clone() for t in ts]  # noqa: E731
+    for M, K, N in ((40, 1, 24), (40, 32, 24)):
+        x, w, b, r, dy, n, beta, dx = neg(M, K), neg(N, K), neg(N), neg(M, N), neg(M, N), neg(K), neg(K), neg(M, K)
+        calls = [(lambda *t: LF.linear(*t[:3], act="silu", residual=t[3]), (x, w, b, r), dy),
+                 (lambda *t: LF.rms_norm(*t)[0], (x, n, dx), dx)]
+        if K > 1:
+            calls.append((lambda *t: LF.batch_norm(*t[:3], residual=t[3], relu=True, checkpoint="mx8"), (x, n, beta, dx), dx))
+        for call, args, d in calls:
+            out = []
+            for ts, dd in ((args, d), (real(*args), *real(d))):
+                ts = [t.detach().requires_grad_(True) for t in ts]
+                y = call(*ts)
+                out.append([y.detach(), *torch.autograd.grad(y, ts, dd)])
+            assert all(torch.equal(a, c) for a, c in zip(*out))
+        q, p = LF.quantize_mx8(x), LF.quantize_mx8(*real(x))
+        assert torch.equal(q.dequantize(), p.dequantize())
+        with torch.no_grad():
+            assert torch.equal(LF.linear(q, LF.quantize_mx8(w), torch._neg_view(b.resolve_neg().half())), LF.linear(p, LF.quantize_mx8(*real(w)), -b.resolve_neg().half()))
+            assert torch.equal(LF.rms_norm(x, n, out="mx8").dequantize(), LF.rms_norm(*real(x, n), out="mx8").dequantize())
