@@ -200,3 +200,31 @@ def test_lazily_negated_views():
         with torch.no_grad():
             assert torch.equal(LF.linear(q, LF.quantize_mx8(w), torch._neg_view(b.resolve_neg().half())), LF.linear(p, LF.quantize_mx8(*real(w)), -b.resolve_neg().half()))
             assert torch.equal(LF.rms_norm(x, n, out="mx8").dequantize(), LF.rms_norm(*real(x, n), out="mx8").dequantize())
+
+
+@pytest.mark.parametrize("act", ["none", "gelu", "silu"])
+@pytest.mark.parametrize("dt", HALF)
+@pytest.mark.parametrize("size", [(1, 512, 1000), (16, 300, 48), (40, 77, 100), (64, 128, 64), (300, 96, 130), (2048, 320, 256), (2600, 40, 129),
+                                  (20000, 64, 24)], ids=str)
+def test_sixteen_bit_gradients_keep_what_is_kept(size, dt, act):
+    """what the backward pass of a 16-bit layer may lose, and no more: act' is within 1e-5 (its 16-bit grid), dz is rounded once for
+    the products, to h^2 of itself where it goes in as two terms (up to 4096 elements, GELU and SiLU), and not at all for db"""
+    from latte_amd import functional as LF
+    M, K, N = size
+    x, w, b, _, dy = _inputs(M, K, N, dt, seed=7)
+    h, lo = R.EPS[dt], R.LOW[dt]
+    t = [v.clone().requires_grad_(True) for v in (x, w, b)]
+    gx, gw, gb = torch.autograd.grad(LF.linear(*t, act=act), t, dy)
+    X, W, DY = x.double(), w.double(), dy.double()
+    Z = X @ W.t() + b.double()
+    zerr = (K + 1) * U * (X.abs() @ W.abs().t() + b.double().abs())
+    D = R.act(Z, act)[1]
+    derr = torch.zeros_like(D) if act == "none" else 1e-5 + 0.8 * zerr + 3e-6 * (1 + Z.abs())
+    DZ = DY * D
+    zabs = DZ.abs() + DY.abs() * derr
+    summed = DY.abs() * derr + 2 * U * zabs
+    dzerr = summed if act == "none" else summed + (h * h if M * N <= 4096 else h) * zabs + lo
+    for got, want, e, mag, n in ((gx, DZ @ W, dzerr @ W.abs(), zabs @ W.abs(), 2 * N), (gw, DZ.t() @ X, dzerr.t() @ X.abs(), zabs.t() @ X.abs(), 2 * M),
+                                 (gb, DZ.sum(0), summed.sum(0), zabs.sum(0), M + 2)):
+        e = e + n * U * mag
+        _close(got, want, e + h * (want.abs() + e) + lo, act)
