@@ -40,8 +40,8 @@ static bool pad_fwd(int64_t M, int K, int N, int dt) {
 
 // the larger of what the two staging paths want: which one runs depends on the operands' alignment
 static int64_t gemm_ws_bytes(int64_t rows, int cols, int64_t depth, int dt, bool nn) {
-  const int64_t a = part_bytes(lt_gemm_plan(rows, cols, depth, dt, nn, true, true), rows, cols);
-  const int64_t b = part_bytes(lt_gemm_plan(rows, cols, depth, dt, nn, false, true), rows, cols);
+  const int64_t a = part_bytes(lt_gemm_plan(rows, cols, depth, dt, nn, true), rows, cols);
+  const int64_t b = part_bytes(lt_gemm_plan(rows, cols, depth, dt, nn, false), rows, cols);
   return a > b ? a : b;
 }
 
@@ -75,7 +75,7 @@ static int gemm_run(const LtGemm& g, void* ws, int64_t ws_bytes, hipStream_t str
   };
   const bool direct = !g.p_scales && aligned(g.P, g.ldp, g.p_kmajor ? g.cols : g.depth, g.p_kmajor) &&
                       aligned(g.Q, g.ldq, g.q_kmajor ? g.rows : g.depth, g.q_kmajor);
-  const LtPlan p = lt_gemm_plan(g.rows, g.cols, g.depth, g.dt, !g.p_kmajor && !g.q_kmajor, direct, true);
+  const LtPlan p = lt_gemm_plan(g.rows, g.cols, g.depth, g.dt, !g.p_kmajor && !g.q_kmajor, direct);
   LT_REQUIRE(part_bytes(p, g.rows, g.cols) <= ws_bytes, LT_ERR_WORKSPACE, "linear: workspace too small (%lld bytes)",
              (long long)ws_bytes);
   LT_REQUIRE((int64_t)p.tr * p.tc * p.splits < (int64_t)1 << 22, LT_ERR_RANGE, "linear: too many tiles");

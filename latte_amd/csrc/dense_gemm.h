@@ -283,7 +283,6 @@ __device__ __forceinline__ void lt_tile_store_(const LtTileArgs& a, const lt_f32
 // wait for the wave's own loads and LDS reads, then for the other waves
 __device__ __forceinline__ void lt_wait_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-
 template <class T, int FR, int FC, int ACT>
 __device__ __forceinline__ void lt_tile_store(const LtTileArgs& a, const lt_f32x4 (&acc)[FR][FC], unsigned split, int64_t row0, int col0,
                                               int lane, float* s) {
@@ -392,7 +391,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_dense(LtTileArgs a) {
                                 reinterpret_cast<float*>(s_tile + wave * LtTurn<FC>::BYTES));
 }
 
-// out = epilogue(sum over the splits, in a fixed order: the same bits every time).  G threads share four neighbours and take
+// out = epilogue(sum over the splits, in a fixed order: the same bits every time).  G threads share eight neighbours and take
 // the splits in turn; one thread adding up 256 splits alone would wait for memory 256 times.
 template <class T, int ACT, int G>
 __global__ __launch_bounds__(256) void k_dense_join(const float* __restrict__ part, int splits, LtEpi e) {

@@ -12,16 +12,16 @@ struct LtPlan {
   bool few, rows, direct;
 };
 
-static inline LtPlan lt_gemm_plan(int64_t rows, int cols, int64_t depth, int dt, bool nn, bool direct, bool few_ok) {
+static inline LtPlan lt_gemm_plan(int64_t rows, int cols, int64_t depth, int dt, bool nn, bool direct) {
   LtPlan p = {};
   p.direct = direct;
   p.splits = 1;
   p.slice = depth;
   // up to 32 rows the tile kernels would leave most of a tile idle; both operands must run along k (64 rows, 4096 -> 4096
   // bf16: 22 us this way, 17 us on tiles)
-  p.few = few_ok && nn && rows <= 32;
+  p.few = nn && rows <= 32;
   if (p.few || rows <= 0 || depth <= 0) return p;
-  p.rows = few_ok && nn && (dt == LT_DT_F32 ? lt_rows_fwd_ok<float>(rows, cols, (int)depth) : lt_rows_fwd_ok<lt_bf16>(rows, cols, (int)depth));
+  p.rows = nn && (dt == LT_DT_F32 ? lt_rows_fwd_ok<float>(rows, cols, (int)depth) : lt_rows_fwd_ok<lt_bf16>(rows, cols, (int)depth));
   if (p.rows) return p;
   const int bk = dt == LT_DT_F32 ? 32 : 64;
   auto tiles = [&](int br, int bc) { return ((rows + br - 1) / br) * ((cols + bc - 1) / bc); };
