@@ -62,9 +62,10 @@ __device__ __forceinline__ void lt_divmod(int64_t i, int d, int64_t& q, int& r) 
 
 // ---- mx8: 32 neighbours of a row share the scale 2^E, E the smallest integer with amax <= 448 * 2^E (amax over the
 // finite values; 448 is e4m3's largest), never below -126; the scale byte is E + 127.  Nothing saturates, so a value that
-// is held reads back within 2^-4 of itself (2^-10 * 2^E at the bottom).  Where 256 * 2^E would be infinite in the block's own
-// type (its largest value lies in the upper quarter of the last binade, above 1.75 of it and so below 256 * 2^E), values are
-// cut at 240 * 2^E, which is within 2^-4 of everything above it.  Infinities and NaN are held as NaN, each in its own place.
+// is held reads back within 2^-4 of itself (2^-10 * 2^E at the bottom).  Where the block's largest value lies in the last
+// binade of its type and above 1.75 times its power of two, 256 * 2^E is infinite in that type and larger than all of them:
+// values are then cut at 240 * 2^E, which is within 2^-4 of everything above it.  (A y that is computed in fp32 and lies
+// beyond float16 is held as it is.)  Infinities and NaN are held as NaN, each in its own place.
 __device__ __forceinline__ int lt_mx8_exp(float amax) {
   const unsigned u = __float_as_uint(amax);            // finite and >= 0
   int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0);   // mantissa over 1.75: one more
@@ -81,7 +82,9 @@ __device__ __forceinline__ int lt_mx8_pack2(float a, float b, float inv, float l
   const float v = __builtin_amdgcn_fmed3f(b * inv, -lim, lim) + (b - b);
   return __builtin_amdgcn_cvt_pk_fp8_f32(u, v, 0, false);
 }
-__device__ __forceinline__ float lt_mx8_lim(int e, int max_exp) { return e + 8 > max_exp ? 240.f : 448.f; }
+__device__ __forceinline__ float lt_mx8_lim(float amax, int e, int max_exp) {
+  return (int)(__float_as_uint(amax) >> 23) - 127 == max_exp && e + 8 > max_exp ? 240.f : 448.f;
+}
 template <int WHICH>   // bytes 2 * WHICH, 2 * WHICH + 1 of a word of four e4m3 values, times s = 2^E
 __device__ __forceinline__ void lt_mx8_get2(int word, float s, float& a, float& b) {
   auto v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(word, s, WHICH != 0);
@@ -99,7 +102,7 @@ __device__ __forceinline__ void lt_mx8_put8(const float (&v)[8], int n, int max_
   a = fmaxf(a, __shfl_xor(a, 2, 64));
   if (n <= 0) return;
   const int e = lt_mx8_exp(a);
-  const float inv = lt_two_to(-e), lim = lt_mx8_lim(e, max_exp);
+  const float inv = lt_two_to(-e), lim = lt_mx8_lim(a, e, max_exp);
   int w[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t)

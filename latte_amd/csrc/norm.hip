@@ -717,7 +717,7 @@ __global__ __launch_bounds__(256) void k_bn_apply_mx8(const float* __restrict__ 
     a = fmaxf(a, __shfl_xor(a, 2, 64));
     a = fmaxf(a, __shfl_xor(a, 4, 64));
     const int e = lt_mx8_exp(a);
-    const float inv = lt_two_to(-e), lim = lt_mx8_lim(e, 127);
+    const float inv = lt_two_to(-e), lim = lt_mx8_lim(a, e, 127);
     bits = ok ? bits : 0u;
     const unsigned other = __shfl_xor(bits, 1, 64);
     if (ok) {

@@ -228,3 +228,19 @@ def test_sixteen_bit_gradients_keep_what_is_kept(size, dt, act):
                                  (gb, DZ.sum(0), summed.sum(0), zabs.sum(0), M + 2)):
         e = e + n * U * mag
         _close(got, want, e + h * (want.abs() + e) + lo, act)
+
+
+def test_rms_norm_mx8_output_beyond_half():
+    """y is computed in fp32 whatever the operands' type: beyond the largest float16 it is held like any other"""
+    from latte_amd import functional as LF
+    g = torch.Generator(device="cuda").manual_seed(8)
+    x = torch.randn(300, 96, generator=g, device="cuda").half()
+    for top in (20000.0, 30000.0, 60000.0):
+        w = (torch.rand(96, generator=g, device="cuda") * top + 3000).half()
+        q = LF.rms_norm(x, w, eps=2.0 ** -20, out="mx8")
+        X = x.double()
+        Y = X / torch.sqrt(X.square().mean(1, keepdim=True) + 2.0 ** -20) * w.double()
+        scale = R.two_to(q.scales.to(torch.int64) - 127).repeat_interleave(32, 1)
+        bound = Y.abs() * 2.0 ** -4 + scale * 2.0 ** -10
+        _close(q.dequantize(), Y, bound * (1 + 116 * U), "y8")
+        assert bool((Y.abs() > 65504).any())         # x reaches 4 in 28800 draws, w 20000 and more
