@@ -131,7 +131,10 @@ __global__ __launch_bounds__(256) void k_dz(const T* __restrict__ dy, int64_t ld
       if constexpr (sizeof(T) == 2 && (DK == LT_DERIV_BYTE || DK == LT_DERIV_FULL)) {
         if (dz2) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) d[i] = g[i] - (float)(T)g[i];
+          for (int i = 0; i < 4; ++i) {
+            const float t = (float)(T)g[i];
+            d[i] = lt_finite_abs(t) == fabsf(t) ? g[i] - t : 0.f;   // an infinity has no rest (it would be NaN)
+          }
           lt_stv<T, 4>(dz2 + row * lddz + col, nz, d);
         }
       }

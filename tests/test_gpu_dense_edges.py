@@ -244,3 +244,25 @@ def test_rms_norm_mx8_output_beyond_half():
         bound = Y.abs() * 2.0 ** -4 + scale * 2.0 ** -10
         _close(q.dequantize(), Y, bound * (1 + 116 * U), "y8")
         assert bool((Y.abs() > 65504).any())         # x reaches 4 in 28800 draws, w 20000 and more
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("M", [8, 300])
+def test_infinite_gradients(dt, M):
+    """an infinity in dy reaches the gradients as one, by the sign of what it meets, whether dz goes in as one term or two"""
+    from latte_amd import functional as LF
+    K, N = 40, 16
+    x, w, b, _, dy = _inputs(M, K, N, dt, seed=9)
+    w[w == 0], x[x == 0] = 1, 1                      # 0 times an infinity would be NaN
+    for act in ("silu", "gelu"):
+        d = dy.clone()
+        d[2, 3], d[5, 7] = float("inf"), float("-inf")
+        t = [v.clone().requires_grad_(True) for v in (x, w, b)]
+        gx, gw, gb = torch.autograd.grad(LF.linear(*t, act=act), t, d)
+        D = R.act(x.double() @ w.double().t() + b.double(), act)[1]
+        for i, j, s in ((2, 3, 1.0), (5, 7, -1.0)):
+            s = s * float(torch.sign(D[i, j]))
+            inf = torch.tensor(float("inf"), device="cuda")
+            assert torch.equal(gx[i].float(), s * torch.sign(w[j].float()) * inf) and torch.equal(gw[j].float(), s * torch.sign(x[i].float()) * inf)
+            assert float(gb[j]) == s * float("inf")
+        assert int((~torch.isfinite(gx)).any(1).sum()) == 2 and int((~torch.isfinite(gw)).any(1).sum()) == 2 and not bool(torch.isnan(gb).any())
