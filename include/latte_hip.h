@@ -309,9 +309,8 @@ int lt_devoxelize_cell_bwd(const float* gout, const int32_t* cells, const int32_
                            float* gfeats /*[V,C]*/, int64_t N, int64_t V, int32_t C, lt_stream_t stream);
 
 /* ------------------------------------------------------------------ dense layers: linear, 8-bit checkpoints
- * nn.Linear with its epilogue and its backward (point branches and heads: latte/models/spvcnn.py:95-111,
- * latte/models/xmuda_arch.py:326-335), where a layer trains or keeps its activations in 8 bits.  Matrices are row-major
- * with a row stride (ld*, in elements; rows may start at any element, a stride of 0 repeats a row); y, deriv and the
+ * nn.Linear with its epilogue and its backward, at the widths of the point branches and heads (latte/models/spvcnn.py:95-111,
+ * latte/models/xmuda_arch.py:326-335) and beyond, for models built on this library.  Matrices are row-major with a row stride (ld*, in elements; rows may start at any element, a stride of 0 repeats a row); y, deriv and the
  * gradients are contiguous.  dt = LT_DT_*: the type of x, w, bias, res, y and of the gradients; sums are fp32.
  * mx8: e4m3 values [M][K] and one scale byte per 32 neighbours [M][ceil(K/32)], value * 2^(scale - 127); the scale is the
  * smallest power of two that brings the block's largest finite magnitude to at most 448, rounding is to nearest even (down to

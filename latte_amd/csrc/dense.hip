@@ -6,8 +6,9 @@
 // 1/384; 16 bits beside 16-bit types, 1e-5), and the backward pass needs no exponential.  dz is rounded to the operands'
 // type, as the matrix instructions take it.
 //
-// Replaces the library products of nn.Linear (point branches and heads: latte/models/spvcnn.py:95-111,
-// latte/models/xmuda_arch.py:326-335) where a layer trains or keeps its activations in 8 bits.
+// An nn.Linear for models built on this framework: the widths are those of the point branches and heads (latte/models/spvcnn.py:
+// 95-111, latte/models/xmuda_arch.py:326-335).  Those layers themselves do not call it: a point branch has a BatchNorm behind its
+// product, where no epilogue can stand, and the heads are gathered in head.hip.
 #include "dense_plan.h"
 
 template <> int lt_gemm_launch<float>(const LtGemm&, const LtPlan&, float*, hipStream_t);
@@ -164,6 +165,8 @@ static DzPlan dz_plan(int64_t M, int N) {
   while (p.tx < cg && p.tx < 64) p.tx <<= 1;
   p.gx = (cg + p.tx - 1) / p.tx;
   const int ty = 256 / p.tx;
+  // 2048 workgroups (a training step with 256, 512, 1024, 2048, 4096 of them, us: 16384 x 1024 -> 4096 bf16 747, 630, 547, 531,
+  // 529; 100000 x 300 -> 300 bf16 486, 399, 359, 333, 337)
   int64_t s = (2048 + p.gx - 1) / p.gx, most = (M + ty * 4 - 1) / (ty * 4);   // four rows a thread at least
   if (M <= ty * 16) most = 1;   // one slab is db: no join to launch (64 x 128 -> 128 bf16, a training step: 70.4 -> 66.0 us)
   if (s > most) s = most;

@@ -5,7 +5,7 @@
 // k in steps of 128 bytes (64 16-bit or 32 fp32 values) through two LDS buffers, one barrier a step: while the step's
 // matrix instructions run, the next step's tiles are on the way.  Tiles go from memory straight into LDS where lines are
 // 16-byte aligned, through registers elsewhere (and where mx8 is widened on the way).
-//   8192 x 4096 -> 4096, bf16: 220 us, 1250 TFLOP/s (243 us with a residual); steps of 64 bytes through four buffers, three
+//   8192 x 4096 -> 4096, bf16: 210 to 219 us, 1250 to 1310 TFLOP/s (224 us with a residual); steps of 64 bytes through four buffers, three
 //   steps ahead: 253 us -- the barriers and the 64-byte requests cost more than the distance gives.
 //
 // LDS images, 16-byte chunks:

@@ -17,8 +17,8 @@ static inline LtPlan lt_gemm_plan(int64_t rows, int cols, int64_t depth, int dt,
   p.direct = direct;
   p.splits = 1;
   p.slice = depth;
-  // up to 32 rows the tile kernels would leave most of a tile idle; both operands must run along k (64 rows, 4096 -> 4096
-  // bf16: 22 us this way, 17 us on tiles)
+  // up to 32 rows the tile kernels would leave most of a tile idle; both operands must run along k (4096 -> 4096 bf16, this way and
+  // on tiles, us: 1 row 9.9 and 11.2, 16 rows 10.2 and 12.1, 32 rows 13.9 and 13.5, 64 rows 22 and 17; 1024 -> 1024, 32 rows: 5.3 and 7.9)
   p.few = nn && rows <= 32;
   if (p.few || rows <= 0 || depth <= 0) return p;
   p.rows = nn && (dt == LT_DT_F32 ? lt_rows_fwd_ok<float>(rows, cols, (int)depth) : lt_rows_fwd_ok<lt_bf16>(rows, cols, (int)depth));
@@ -28,7 +28,8 @@ static inline LtPlan lt_gemm_plan(int64_t rows, int cols, int64_t depth, int dt,
   int br, bc;
   // the widest tile needs the fewest operand bytes a product, and one workgroup a CU: 192 of them, or fewer whose k is long
   // enough to be split into at least 32 steps each (training 16384 x 1024 -> 4096, bf16: its dW on 128 x 128 tiles 618 us a
-  // step, on 256 x 256 tiles split four ways 554 us).  256 x 128 tiles, also one a CU, lose to two of 128 x 128 (training
+  // step, on 256 x 256 tiles split four ways 554 us; forward x 1024 -> 4096 bf16 on the widest and on 128 x 128, us: 128 tiles of the
+  // widest 42 and 22, 192 of them 36.4 and 36.4, 256 of them 38.9 and 41.7).  256 x 128 tiles, also one a CU, lose to two of 128 x 128 (training
   // 4096 x 2048 -> 2048, bf16: 187 us a step and 146).
   const int64_t t256 = tiles(256, 256);
   const bool wide = direct && dt != LT_DT_F32 && cols >= 192 && rows >= 192;
@@ -36,7 +37,8 @@ static inline LtPlan lt_gemm_plan(int64_t rows, int cols, int64_t depth, int dt,
   else if (cols <= 32 && direct) p.tile = LT_TILE_256x32, br = 256, bc = 32;
   else if (cols <= 64 && direct) p.tile = LT_TILE_128x64, br = 128, bc = 64;
   // 128 x 128 tiles where they nearly fill the chip, else 64 x 64, four of which share a CU (1777 x 1000 -> 1000 bf16: 26 us
-  // on 112 of the larger, split four ways, 12 us on 448 of the smaller).  fp32 is bound by the matrix rate alone, so there the
+  // on 112 of the larger, split four ways, 12 us on 448 of the smaller).  x 1024 -> 2048 bf16 on the larger and the smaller, us: 160
+  // of the larger 25 and 13, 224 of them 27 and 16 (split in two), 256 of them 16.6 and 16.2, 320 of them 19.7 and 24.3.  fp32 is bound by the matrix rate alone, so there the
   // smaller tiles cost 6 % (8192 x 1024 -> 1024: 137 and 144 us) and a chip half idle in its last turn costs more (3000 x 1500
   // -> 1500: 191 and 154 us): the larger ones where the turns of two a CU are 93 % full.
   else if (dt == LT_DT_F32 ? (double)rows * cols >= 0.93 * 128 * 128 * 512 * ((tiles(128, 128) + 511) / 512) : tiles(128, 128) >= 224) p.tile = LT_TILE_128x128, br = 128, bc = 128;
@@ -45,7 +47,8 @@ static inline LtPlan lt_gemm_plan(int64_t rows, int cols, int64_t depth, int dt,
   p.tc = (cols + bc - 1) / bc;
   // Fewer tiles than the chip runs at once: split k, at least four steps each.  The join reads and writes splits + 1 times
   // the output, so where the chip is full once (256 tiles) only a long k is split (1024 x 4096 -> 1024 bf16: 36 us whole,
-  // 25 us in four; 1777 x 1000 -> 1000: 12 us whole, 24 us in two).
+  // 25 us in four; 1777 x 1000 -> 1000: 12 us whole, 24 us in two).  64 x 64 tiles from 48 steps on: 256 tiles split and whole, us, 32
+  // steps 21 and 14, 40 steps 23 and 19, 50 steps 23 and 30, 64 steps 24 and 37; 512 tiles, 40 steps 27 and 26, 50 steps 29 and 31.
   const int64_t t = (int64_t)p.tr * p.tc, steps = (depth + bk - 1) / bk;
   const int64_t full = p.tile == LT_TILE_256x256 ? 256 : steps >= 48 ? 1024 : 512;
   if (t < (p.tile == LT_TILE_256x256 ? 192 : p.tile == LT_TILE_64x64 && steps >= 48 ? 513 : 256)) {

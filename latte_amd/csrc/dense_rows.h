@@ -1,4 +1,4 @@
-// Long and narrow layers (a few hundred channels, many rows -- the point branches): forward and backward in one pass over
+// Long and narrow layers (a few hundred channels, many rows: layers over all points): forward and backward in one pass over
 // the rows.  Tiles would pad 96 columns to 128 and read dz and x once per product; here W stays in LDS for the whole launch,
 // in fragment order, and rows stream past it.
 #pragma once
@@ -67,8 +67,8 @@ __global__ __launch_bounds__(512) void k_rows_fwd(LtTileArgs a) {
 // One pass: a workgroup takes tiles of R rows, forms dz = dy act' on the way into LDS (its column sums stay in registers),
 // and from the two tiles dz [R][N] and x [R][K] its waves compute dx = dz W (W in LDS) and add dz^T x to the workgroup's
 // own dW, which they hold in registers until the end.  dy, act' and x are read once, dz is never written.
-//   310017 x 128 -> 96, fp32: 238 us, half of it the two products at 55 % of the fp32 matrix rate (dz, dx and dW apart: 282
-//   us); bf16: 73 us.
+//   310017 x 128 -> 96, fp32: 223 us alone, matrix pipes busy 46 % of the cycles, 37 % of the LDS cycles are conflicts (dz, dx
+//   and dW apart: 282 us); bf16: 73 us.
 struct LtRowsBwdArgs {
   const void* dy;
   const void* x;
@@ -306,7 +306,10 @@ __global__ __launch_bounds__(1024) void k_rows_bwd(LtRowsBwdArgs a) {
 }
 
 // ------------------------------------------------------------------ host
-// forward: at least 8192 rows, both widths at most 256 and multiples of 8, W and the turned rows within half a CU's LDS (two workgroups a CU)
+// forward: at least 8192 rows, both widths at most 256 and multiples of 8, W and the turned rows within half a CU's LDS (two workgroups a CU).
+// This kernel and tiles, us: 64 -> 64 fp32 7.7 and 8.5 at 8192 rows, 9.2 and 10.0 at 32768; 128 -> 96 fp32 14.0 and 7.5 at 8192, 17.2 and
+// 17.9 at 32768, 103 and 145 at 310017; 32 -> 256 fp32 17.5 and 7.4, 20.8 and 20.4; 128 -> 96 bf16 6.7 and 4.2, 7.7 and 8.1.  The
+// wider layers pay for laying out W in every workgroup up to some 30000 rows.
 template <class T>
 static int lt_rows_kc(int K) {
   const int kf = 4 * (16 / (int)sizeof(T)), n = (K + kf - 1) / kf;

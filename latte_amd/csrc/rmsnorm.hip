@@ -224,7 +224,8 @@ __global__ __launch_bounds__(256) void k_rms_bwd(LtRmsBwdArgs a) {
 }
 
 // ------------------------------------------------------------------ host
-// lanes per row: the row fits 8 neighbours a lane as far as it can, a wave from 264 columns on, a workgroup from 2056 on
+// lanes per row: the row fits 8 neighbours a lane as far as it can, a wave from 264 columns on, a workgroup from 2056 on (forward
+// with a residual, bf16, 8192 rows, a wave and a workgroup a row, us: 1024 columns 15.5 and 16.3, 2048 columns 30.7 and 21.9)
 static int rms_lanes(int C) {
   if (C > 2048) return 256;
   int l = 4;
@@ -234,6 +235,8 @@ static int rms_lanes(int C) {
 static int rms_bwd_grid(int64_t M, int C) {
   const int64_t rpb = 256 / rms_lanes(C);
   int64_t g = (M + rpb * 4 - 1) / (rpb * 4);   // four rows a lane group at least, so that the column sums stay few
+  // trained with at most 256, 512, 1024, 2048, 4096 workgroups, us: 8192 x 4096 bf16 174, 129, 112, 126, 127; 34816 x 256 fp32 48, 47,
+  // 47, 50, 50.  Rows a lane group at least, 1, 4 and 16: 2000 x 256 fp32 12, 13 and 21; 8192 x 4096 bf16 112, 115 and 130
   if (g > 1024) g = 1024;
   return (int)(g < 1 ? 1 : g);
 }
@@ -280,7 +283,7 @@ extern "C" int lt_rms_norm_fwd(const void* x, int64_t ldx, const void* res, int6
   const LtRmsArgs a = {x, res, w, ldx, ldres, M, C, eps, h, y, (uint8_t*)y8, (uint8_t*)y8_scales, (uint8_t*)h8, (uint8_t*)h8_scales, rstd};
   const int64_t rpb = 256 / rms_lanes(C);
   int64_t g = (M + rpb - 1) / rpb;
-  if (g > 4096) g = 4096;
+  if (g > 4096) g = 4096;   // 8192 x 4096 bf16 with 512, 1024, 4096, 16384: 56, 43.6, 44.1, 47.2 us
   LT_DENSE_TYPES(dt, rms_dispatch<T, RmsFwdLaunch>(C, a, (int)g, stream));
   LT_LAUNCH_CHECK();
   return LT_OK;

@@ -259,7 +259,7 @@ class RMSNorm(nn.Module):
 
 def set_activation_checkpoint(model: nn.Module, mode: str | None) -> nn.Module:
     """Every BatchNorm, Linear and RMSNorm of `model` keeps what its backward pass reads of its input in 8 bits ("mx8"), or in
-    full (None).  A SPVCNN with checkpoints walks its module tree where gradients are on (the one-call pass keeps its buffers
+    full (None).  In a SPVCNN that reaches its BatchNorms: its dense layers are nn.Linear.  A SPVCNN with checkpoints walks its module tree where gradients are on (the one-call pass keeps its buffers
     in full); tta_step.LatteStep(activation_checkpoint="mx8") sets it for the student."""
     if mode not in (None, "mx8"):
         raise ValueError(f"set_activation_checkpoint: mode must be None or 'mx8', got {mode!r}")
